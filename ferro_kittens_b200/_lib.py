@@ -7,7 +7,7 @@ operation of this package raises. The bindings below are the Python spelling of
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_uint16, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_uint16, c_uint32, c_uint64, c_void_p
 
 from .build import LIBRARY, build_library
 
@@ -48,6 +48,13 @@ class Plan(ctypes.Structure):
     """``fk_plan_t``."""
 
     _fields_ = [("bytes", c_uint64)]
+
+
+class CacheView(ctypes.Structure):
+    """``fk_cache_t``."""
+
+    _fields_ = [(name, c_void_p) for name in ("k_codes", "k_params", "v_codes", "v_params")] + [
+        (name, c_uint32) for name in ("pages", "page_size", "kv_heads", "head_dim", "group", "element")]
 
 
 # name -> (restype, argtypes); also the list the symbol test walks.
@@ -114,6 +121,14 @@ SIGNATURES = {
     "fk_softmax_rows": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_void_p, c_void_p]),
     "fk_layernorm_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_uint32, c_float, c_void_p, c_void_p]),
     "fk_groupnorm_tile": (c_int, [c_void_p, c_void_p, c_uint32, c_float, c_void_p, c_void_p]),
+    "fk_cache_write": (c_int, [POINTER(CacheView), c_void_p, c_void_p] + [c_int64] * 4 + [
+        c_void_p, c_uint32, c_uint32, c_void_p, c_void_p]),
+    "fk_cache_read": (c_int, [POINTER(CacheView), c_void_p, c_void_p] + [c_int64] * 4 + [
+        c_void_p, c_uint32, c_uint32, c_int, c_void_p, c_void_p]),
+    "fk_cache_attention_workspace_bytes": (c_uint64, [c_uint32]),
+    "fk_cache_attention": (c_int, [POINTER(CacheView), c_void_p] + [c_int64] * 3 + [c_void_p] * 4 + [
+        c_int64, c_uint32, c_uint32, c_uint32, c_uint32, c_float, c_uint32, c_uint32, c_void_p, c_uint64, c_void_p,
+        c_void_p]),
     "fk_wait_stream": (c_int, [c_void_p, c_uint32]),
     "fk_wait_event": (c_int, [c_void_p, c_uint32]),
     "fk_launch_budget_ms": (c_uint32, []),

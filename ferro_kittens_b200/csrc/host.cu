@@ -466,6 +466,13 @@ extern "C" int fk_status_check(const uint32_t* device_status, void* stream) {
     const int waited = fk::wait_stream(static_cast<cudaStream_t>(stream));
     if (waited != FK_OK) return waited;
     if (words[0] == 0) return FK_OK;
+    // The cache kernels note an index they had to skip, not a stall.
+    if (words[0] == 0x501)
+        return fk_fail(FK_ERR_INVALID, "slot %u of token %u lies outside the cache", words[3], words[2]);
+    if (words[0] == 0x502)
+        return fk_fail(FK_ERR_INVALID, "page %u in the table of sequence %u lies outside the cache", words[3], words[2]);
+    if (words[0] == 0x503)
+        return fk_fail(FK_ERR_INVALID, "length %u of sequence %u is past its page table", words[3], words[2]);
     return fk_fail(FK_ERR_DEVICE_STALL, "device stall: %s (code %#x) in block %u, step %u, parity %u",
                    stall_role(words[0]), words[0], words[1], words[2], words[3]);
 }

@@ -344,6 +344,81 @@ int fk_layernorm_rows(const void* source, const void* gamma, const void* beta, v
 int fk_groupnorm_tile(const void* source, void* destination, uint32_t rows, float epsilon,
                       void* stream, uint32_t* device_status);
 
+/* ---------------------------------------------------------------- key/value cache in 4 bits
+ *
+ * No counterpart in the reference, whose attention (examples/src/flash_forward.rs:151-158) reads whole
+ * planes of bf16 keys and values. A serving program keeps those of the tokens seen so far, and the time of
+ * one decoding step is the time to read them: at 4 bits a value (4.5 with the parameters of groups of 64) a
+ * step moves 3.5 times fewer bytes than from bf16.
+ *
+ * The cache is four packed device buffers, one row per (page, kv head, place in the page):
+ *   k_codes, v_codes    [pages, kv_heads, page_size, head_dim / 2] bytes, two codes each, low nibble first
+ *   k_params, v_params  [pages, kv_heads, page_size, head_dim / group, 2] of the cache's type: scale, low
+ * A row's channels are cut into groups of `group`. Of a group, `low` is the smallest value, `scale` the
+ * largest value of the cache's type not above (high - low) / 15 (so that nothing read back lies outside
+ * [low, high]), and a channel's code 0..15 the number of k in 0..14 with x - low >= (k + 1/2) * scale, in exact
+ * arithmetic. It stands for low + code * scale, at most scale / 2 from x (a group whose scale underflows the
+ * type reads back as low). A group that holds a NaN or an infinity reads back as NaN throughout.
+ * The order of a row's nibbles is the one the attention's matrix instructions want:
+ *   keys    a matrix [4][head_dim / 32] of runs of 8 nibbles; run [c][w] holds channels 8 * (4 w + c) + 0..7
+ *   values  a matrix [8][head_dim / 8] of nibbles; nibble [l][n] is channel 8 n + l
+ *
+ * head_dim is 64 or 128, group 32, 64 or 128 and at most head_dim, element FK_BF16 or FK_F16 (of the
+ * parameters and of the tensors that are written, read or asked with). Buffers are 16-byte aligned.
+ * A slot is page * page_size + place. Indices live on the device, so a bad one is found there: it is
+ * skipped (nothing is read or written out of bounds) and noted in `device_status`, which may be null
+ * (fk_status_check then says FK_ERR_INVALID with the index). All calls are asynchronous on `stream`. */
+typedef struct {
+    void* k_codes;
+    void* k_params;
+    void* v_codes;
+    void* v_params;
+    uint32_t pages;
+    uint32_t page_size; /* tokens, any number from 1 */
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t group;
+    uint32_t element; /* FK_BF16 or FK_F16 */
+} fk_cache_t;
+
+/* Quantise tokens into the cache: token i's keys k[i, head, :] and values v[i, head, :] go to slot slots[i]; a
+ * negative slot skips its token. Strides are in elements, multiples of 8 (rows move by 16-byte accesses); the
+ * head_dim values of a row are contiguous. `slots` holds `tokens` integers of `slot_bytes` (4 or 8) bytes; those
+ * that are not negative are distinct (of a slot named twice in one call the row is unspecified). */
+int fk_cache_write(const fk_cache_t* cache, const void* k, const void* v, int64_t k_token_stride,
+                   int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void* slots,
+                   uint32_t slot_bytes, uint32_t tokens, void* stream, uint32_t* device_status);
+
+/* Read rows back: k[i, head, :] and v[i, head, :] become the values of slot slots[i] (which may repeat), rounded
+ * once to the cache's type. Rows of negative slots are left as they were, or zeroed with `clear_skipped`. */
+int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_stride, int64_t k_head_stride,
+                  int64_t v_token_stride, int64_t v_head_stride, const void* slots, uint32_t slot_bytes,
+                  uint32_t tokens, int clear_skipped, void* stream, uint32_t* device_status);
+
+/* Attention of each sequence's newest tokens over its rows of the cache, theirs included.
+ *   q        [batch, queries, heads, head_dim], strides in elements, multiples of 8; heads is a multiple of
+ *            kv_heads, and query head h reads kv head h / (heads / kv_heads)
+ *   out      packed [batch, queries, heads, head_dim] of the cache's type; lse null or packed
+ *            [batch, queries, heads] fp32 (natural log)
+ *   lengths  [batch] int32: tokens of each sequence, its `queries` newest among them; 0 or less is an empty
+ *            sequence, and one shorter than `queries` has its first rows before its first token
+ *   table    row b (of table_pages entries, table_stride apart) names sequence b's pages in order, and entries behind its
+ *            length are never read; null: sequence b owns page b
+ * Query t of a sequence sits at i = length - queries + t and sees token j when j <= i and (window == 0, or
+ * j > i - window, or j < sinks). A row that sees nothing is zero, its lse -inf. Tokens that no row of a sequence
+ * sees are not read, and what a row does not see may hold anything, NaN included.
+ * Scores, softmax statistics and sums are fp32; a weight times its group's scale is rounded to fp16 (11 bits,
+ * scaled so that the range always fits) for the product with the value codes, which are exact.
+ * `workspace` is fk_cache_attention_workspace_bytes(sm_count) bytes, 16-byte aligned, ALL ZERO before its first
+ * use; every call leaves its counters zero again, so it is cleared once. Calls that share a workspace must not
+ * overlap on the device (two streams, or two captured graphs that may run together, want one each). */
+uint64_t fk_cache_attention_workspace_bytes(uint32_t sm_count);
+int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_t q_batch_stride, int64_t q_token_stride,
+                       int64_t q_head_stride, void* out, float* lse, const int32_t* lengths, const int32_t* table,
+                       int64_t table_stride, uint32_t table_pages, uint32_t batch, uint32_t queries, uint32_t heads,
+                       float scale, uint32_t window, uint32_t sinks, void* workspace, uint64_t workspace_bytes,
+                       void* stream, uint32_t* device_status);
+
 /* ---------------------------------------------------------------- waits and status
  *
  * `watchdog::wait` / `wait_event` (src/watchdog.rs:300-332): poll with a

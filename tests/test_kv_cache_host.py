@@ -1,0 +1,106 @@
+"""What the 4-bit cache's entries refuse before they reach a device, and the plain definition the GPU tests compare with."""
+import ctypes
+import re
+
+import numpy as np
+import pytest
+import torch
+
+from ferro_kittens_b200 import kv_cache
+from ferro_kittens_b200._lib import FK_BF16, FK_ERR_ALIGNMENT, FK_ERR_INVALID, FK_ERR_SHAPE, FK_F32, FK_OK, CacheView, last_error, library
+
+from kv_cache_plain import key_nibble, quantise, value_nibble
+
+BASE = 0x7F00_0000  # a device address is never dereferenced on the host
+
+
+def _cache(**changed):
+    fields = {"k_codes": BASE, "k_params": BASE, "v_codes": BASE, "v_params": BASE, "pages": 4, "page_size": 16,
+              "kv_heads": 2, "head_dim": 128, "group": 64, "element": FK_BF16} | changed
+    return CacheView(*fields.values())
+
+
+def _write(cache, k=BASE, v=BASE, strides=(256, 128, 256, 128), slots=BASE, slot_bytes=4, tokens=3):
+    return library().fk_cache_write(ctypes.byref(cache) if cache else None, k, v, *strides, slots, slot_bytes, tokens, None, None)
+
+
+def _read(cache, k=BASE, v=BASE, strides=(256, 128, 256, 128), slots=BASE, slot_bytes=4, tokens=3):
+    return library().fk_cache_read(ctypes.byref(cache) if cache else None, k, v, *strides, slots, slot_bytes, tokens, 0, None, None)
+
+
+def _attend(cache, q=BASE, strides=(1024, 1024, 128), out=BASE, lse=BASE, lengths=BASE, table=BASE, table_pages=2, batch=3,
+            queries=1, heads=8, workspace=BASE, workspace_bytes=1 << 30):
+    return library().fk_cache_attention(ctypes.byref(cache) if cache else None, q, *strides, out, lse, lengths, table, table_pages,
+                                        table_pages, batch, queries, heads, 0.1, 0, 0, workspace, workspace_bytes, None, None)
+
+
+@pytest.mark.parametrize("entry", [_write, _read, _attend])
+@pytest.mark.parametrize("changed,code,word", [
+    ({"k_codes": None}, FK_ERR_INVALID, "buffer is null"), ({"v_params": None}, FK_ERR_INVALID, "buffer is null"),
+    ({"v_codes": BASE + 8}, FK_ERR_ALIGNMENT, "16-byte"), ({"element": FK_F32}, FK_ERR_INVALID, "bf16 or fp16"),
+    ({"head_dim": 96}, FK_ERR_SHAPE, "head_dim 96"), ({"group": 16}, FK_ERR_SHAPE, "groups of 16"),
+    ({"head_dim": 64, "group": 128}, FK_ERR_SHAPE, "groups of 128"), ({"pages": 0}, FK_ERR_SHAPE, "is empty"),
+    ({"page_size": 0}, FK_ERR_SHAPE, "is empty"), ({"kv_heads": 0}, FK_ERR_SHAPE, "is empty"),
+    ({"pages": 1 << 31, "page_size": 1 << 31, "kv_heads": 1 << 31}, FK_ERR_SHAPE, "more than 2\\^31"),
+    ({"pages": 1 << 20, "page_size": 1 << 10}, FK_ERR_SHAPE, "more than 2\\^31")])
+def test_caches_refused(entry, changed, code, word):
+    assert entry(_cache(**changed)) == code
+    assert re.search(word, last_error()), last_error()
+
+
+def test_a_null_cache_is_refused():
+    for entry in (_write, _read, _attend):
+        assert entry(None) == FK_ERR_INVALID and "null" in last_error()
+
+
+@pytest.mark.parametrize("entry", [_write, _read])
+@pytest.mark.parametrize("changed,code,word", [
+    ({"k": None}, FK_ERR_INVALID, "null"), ({"slots": None}, FK_ERR_INVALID, "null"), ({"v": BASE + 2}, FK_ERR_ALIGNMENT, "16-byte"),
+    ({"slot_bytes": 2}, FK_ERR_INVALID, "4 or 8"), ({"slots": BASE + 4, "slot_bytes": 8}, FK_ERR_ALIGNMENT, "8 bytes"),
+    ({"strides": (256, 132, 256, 128)}, FK_ERR_ALIGNMENT, "132"), ({"strides": (256, 128, 257, 128)}, FK_ERR_ALIGNMENT, "257"),
+    ({"tokens": 1 << 30}, FK_ERR_SHAPE, "more than 2^31")])
+def test_rows_refused(entry, changed, code, word):
+    assert entry(_cache(), **changed) == code
+    assert word in last_error()
+
+
+@pytest.mark.parametrize("changed,code,word", [
+    ({"heads": 7}, FK_ERR_SHAPE, "7 query heads"), ({"heads": 0}, FK_ERR_SHAPE, "0 query heads"), ({"q": None}, FK_ERR_INVALID, "null"),
+    ({"out": None}, FK_ERR_INVALID, "null"), ({"lengths": None}, FK_ERR_INVALID, "null"), ({"workspace": None}, FK_ERR_INVALID, "null"),
+    ({"q": BASE + 8}, FK_ERR_ALIGNMENT, "16-byte"), ({"lse": BASE + 2}, FK_ERR_ALIGNMENT, "4-byte"),
+    ({"strides": (1024, 1020, 128)}, FK_ERR_ALIGNMENT, "1020"), ({"table_pages": 0}, FK_ERR_SHAPE, "no columns"),
+    ({"table": None, "batch": 5}, FK_ERR_SHAPE, "own a page each"), ({"table_pages": 1 << 30}, FK_ERR_SHAPE, "tokens a sequence")])
+def test_attention_refused(changed, code, word):
+    assert _attend(_cache(), **changed) == code
+    assert word in last_error()
+
+
+def test_empty_calls_need_no_device():
+    assert _write(_cache(), tokens=0) == FK_OK and _read(_cache(), tokens=0) == FK_OK
+    assert _attend(_cache(), batch=0) == FK_OK and _attend(_cache(), queries=0) == FK_OK
+
+
+def test_tensors_on_the_cpu_are_refused():
+    codes, params = torch.zeros(1, 1, 16, 64, dtype=torch.uint8), torch.zeros(1, 1, 16, 2, 2, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv_cache.Cache(codes, params, codes, params)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_the_layouts_place_every_channel_once(dim):
+    for place in (key_nibble, value_nibble):
+        assert sorted(place(d, dim) for d in range(dim)) == list(range(dim))
+
+
+def test_the_plain_rule():
+    """Ends read back near themselves, every value within half a scale, ties upwards."""
+    x = np.array([-1.0, 0.875, -0.9375, -0.8125] + [0.0] * 28)
+    codes, scale, low = quantise(x, 32, torch.bfloat16)
+    assert scale[0] == 0.125 and low[0] == -1.0
+    assert codes[:4].tolist() == [0, 15, 1, 2] and (codes[4:] == 8).all()
+    rng = np.random.default_rng(0)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = torch.from_numpy(rng.standard_normal(128)).to(dtype).double().numpy()
+        codes, scale, low = quantise(x, 64, dtype)
+        back = np.repeat(low, 64) + codes * np.repeat(scale, 64)
+        assert (np.abs(back - x) <= np.repeat(scale, 64) / 2).all() and codes.max() == 15 and codes.min() == 0
