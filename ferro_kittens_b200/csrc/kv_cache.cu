@@ -296,102 +296,618 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant
 // ---------------------------------------------------------------- attention
 
 struct AttentionArguments {
-    const uint8_t* k_codes;
-    const uint32_t* k_params;
-    const uint8_t* v_codes;
-    const uint32_t* v_params;
+    const uint8_t* codes[2];  // keys, values
+    const uint8_t* params[2];
     const uint8_t* q;
     int64_t q_batch_stride, q_token_stride, q_head_stride;  // bytes
-    void* out;
+    uint16_t* out;
     float* lse;
     const int32_t* lengths;
     const int32_t* table;
     int64_t table_stride;
     uint32_t table_pages, pages, page_size;
     uint32_t batch, queries, heads, kv_heads;
+    uint32_t rows, row_tiles;  // query rows of a (sequence, kv head): queries * heads / kv_heads
     float scale;
-    uint32_t window, sinks;
-    Divider page;
+    int32_t window, sinks;
+    Divider page, ratio;
+    uint32_t least_units;  // units a block takes before another block is put to work
+    uint32_t* arrivals;    // workspace: a counter for each block, then the partial results
+    float* partials;
 };
 
-constexpr uint32_t kAttentionThreads = 128;
+constexpr uint32_t kWarpTokens = 32;
+constexpr uint32_t kStages = 3;
+constexpr uint32_t kMostBlocksPerSm = 4;
+constexpr uint32_t kMostRows = 32;
+/// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
+constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
 
-// One block per (query row, sequence), a warp per token in turn with a running maximum and sum of its own.
-template <int D, int G, bool BF16>
-__global__ void __launch_bounds__(kAttentionThreads) attention_kernel(const __grid_constant__ AttentionArguments args,
-                                                                      uint32_t* status) {
+template <int D, int G, int NT>
+struct AttentionShape {
+    static constexpr uint32_t kGroups = D / G;
+    static constexpr uint32_t kRows = 8 * NT;
+    static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
+    static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
+    static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes + kWarpTokens * 4;
+    static constexpr uint32_t kRingBytes = kStages * kStageBytes;
+    static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
+    static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
+    static constexpr uint32_t kWarpBytes = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
+    static constexpr uint32_t kMostByRegisters = NT == 1 ? 16 : NT == 2 ? 12 : 8;  // 128, 168, 255 a thread
+    static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048) / kWarpBytes;
+    static constexpr uint32_t kMostWarps = kMostByRegisters < kMostByMemory ? kMostByRegisters : kMostByMemory;
+};
+
+/// What of a sequence is read: its tokens, less those between the sinks and the window that no query row sees.
+struct Extent {
+    int32_t length, first;  // tokens; the first query's position (0 if it lies before the first token)
+    int32_t kept, skipped;  // tokens read before the gap, and the gap's length
+    __device__ __forceinline__ int32_t visible() const { return length - skipped; }
+    __device__ __forceinline__ int32_t token(int32_t at) const { return at < kept ? at : at + skipped; }
+};
+
+__device__ __forceinline__ Extent extent_of(const AttentionArguments& args, uint32_t b, uint32_t* status) {
+    Extent e;
+    e.length = max(args.lengths[b], 0);
+    const int32_t capacity = static_cast<int32_t>(args.table_pages * args.page_size);
+    if (e.length > capacity) {
+        note(status, kBadLength, b, static_cast<uint32_t>(e.length));
+        e.length = capacity;
+    }
+    e.first = max(e.length - static_cast<int32_t>(args.queries), 0);
+    const int32_t start = args.window ? max(e.first + 1 - args.window, 0) : 0;
+    e.kept = min(args.sinks, start);
+    e.skipped = start - e.kept;
+    return e;
+}
+
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+/// BYTES of a row's parameters, or zeros where the row is not to be read.
+template <int BYTES>
+__device__ __forceinline__ void copy_async_params(uint32_t dst, const void* src, bool real) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16u : 0u) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(real ? BYTES : 0)
+                     : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+/// D[16, 8] += A[16, 16] . B[16, 8] in fp16 with fp32 sums.
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    return d;
+}
+__device__ __forceinline__ float power_of_two(int32_t biased) { return __int_as_float(biased << 23); }
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const uint8_t* from) {
+    if constexpr (WORDS == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(from);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (WORDS == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(from);
+        w[0] = x.x, w[1] = x.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(from);
+    }
+}
+
+template <int D, int G, int NT, bool BF16>
+__global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
+    attention_kernel(const __grid_constant__ AttentionArguments args, uint32_t* status) {
     using E = Element<BF16>;
-    constexpr uint32_t kWarps = kAttentionThreads / 32, kEach = D / 32;
-    __shared__ float sums[kWarps][D];
-    __shared__ float peaks[kWarps], totals[kWarps];
-    const uint32_t b = blockIdx.y, query = blockIdx.x / args.heads, head = blockIdx.x % args.heads;
-    const uint32_t kv_head = head / (args.heads / args.kv_heads);
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint64_t capacity = static_cast<uint64_t>(args.table_pages) * args.page_size;
-    int64_t length = max(args.lengths[b], 0);
-    if (static_cast<uint64_t>(length) > capacity) {
-        if (threadIdx.x == 0) note(status, kBadLength, b, static_cast<uint32_t>(length));
-        length = static_cast<int64_t>(capacity);
-    }
-    const int64_t at = length - args.queries + query;
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(args.q + b * args.q_batch_stride +
-                                                          query * args.q_token_stride + head * args.q_head_stride);
-    float mine[kEach], sum[kEach];
+    using Shape = AttentionShape<D, G, NT>;
+    constexpr uint32_t kGroups = Shape::kGroups, kRows = Shape::kRows, kPitch = Shape::kPitch;
+    constexpr uint32_t kKeyWords = D / 32, kValueWords = D / 64, kTiles = D / 16;
+    extern __shared__ __align__(16) uint8_t shared[];
+    __shared__ uint32_t scan[18];
+    const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t unit_tokens = warps * kWarpTokens;
+    const uint32_t l4 = lane / 4, c4 = lane % 4;
+
+    // ---- this block's share: units of unit_tokens tokens, sequence by sequence, (kv head, row tile) by (kv head,
+    // row tile), cut evenly over the blocks whatever the lengths are.
+    const uint32_t segments = args.kv_heads * args.row_tiles;  // of one sequence
+    const auto units_of = [&](const Extent& e) {
+        return max((static_cast<uint32_t>(e.visible()) + unit_tokens - 1) / unit_tokens, 1u);
+    };
+    uint32_t mine = 0;
+    for (uint32_t b = threadIdx.x; b < args.batch; b += blockDim.x) mine += units_of(extent_of(args, b, status));
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) {
-        mine[e] = E::low(q[lane + 32 * e]) * args.scale;
-        sum[e] = 0.0f;
-    }
-    float peak = -INFINITY, total = 0.0f;
-    for (int64_t j = warp; j <= at; j += kWarps) {
-        if (args.window && j <= at - static_cast<int64_t>(args.window) && j >= static_cast<int64_t>(args.sinks)) continue;
-        const uint32_t entry = args.page.quotient(static_cast<uint32_t>(j));
-        const uint32_t page = args.table ? static_cast<uint32_t>(args.table[b * args.table_stride + entry]) : b;
-        if (page >= args.pages) {
-            if (lane == 0) note(status, kBadPage, b, page);
-            continue;
-        }
-        const uint64_t row = (static_cast<uint64_t>(page) * args.kv_heads + kv_head) * args.page_size +
-                             (static_cast<uint32_t>(j) - entry * args.page_size);
-        float score = 0.0f, v[kEach];
-#pragma unroll
-        for (uint32_t e = 0; e < kEach; ++e) {
-            const uint32_t d = lane + 32 * e, run = d / 8;
-            const uint32_t kn = key_word<D>(run) * 8 + d % 8, vn = (d % 8) * (D / 8) + run;
-            const uint32_t kc = (args.k_codes[row * (D / 2) + kn / 2] >> (4 * (kn & 1))) & 15u;
-            const uint32_t vc = (args.v_codes[row * (D / 2) + vn / 2] >> (4 * (vn & 1))) & 15u;
-            const uint32_t kp = args.k_params[row * (D / G) + d / G], vp = args.v_params[row * (D / G) + d / G];
-            score += mine[e] * fmaf(static_cast<float>(kc), E::low(kp), E::high(kp));
-            v[e] = fmaf(static_cast<float>(vc), E::low(vp), E::high(vp));
-        }
-#pragma unroll
-        for (uint32_t mask = 16; mask > 0; mask >>= 1) score += __shfl_xor_sync(0xffffffffu, score, mask);
-        const float higher = fmaxf(peak, score);
-        const float keep = higher == peak ? 1.0f : __expf(peak - higher), weight = __expf(score - higher);
-        peak = higher;
-        total = total * keep + weight;
-#pragma unroll
-        for (uint32_t e = 0; e < kEach; ++e) sum[e] = fmaf(weight, v[e], sum[e] * keep);
-    }
-#pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) sums[warp][lane + 32 * e] = sum[e];
-    if (lane == 0) {
-        peaks[warp] = peak;
-        totals[warp] = total;
-    }
+    for (uint32_t mask = 16; mask > 0; mask >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, mask);
+    if (lane == 0) scan[warp] = mine;
     __syncthreads();
-    float top = peaks[0], all = 0.0f, y = 0.0f;
-    for (uint32_t w = 1; w < kWarps; ++w) top = fmaxf(top, peaks[w]);
-    const uint64_t place = (static_cast<uint64_t>(b) * args.queries + query) * args.heads + head;
-    for (uint32_t w = 0; w < kWarps; ++w) {
-        const float share = peaks[w] == -INFINITY ? 0.0f : __expf(peaks[w] - top);
-        all += totals[w] * share;
-        if (threadIdx.x < D) y += sums[w][threadIdx.x] * share;
+    uint32_t total = 0;
+    for (uint32_t w = 0; w < warps; ++w) total += scan[w];
+    total *= segments;
+    const uint32_t blocks = min(gridDim.x, max(total / args.least_units, 1u));
+    if (blockIdx.x >= blocks) return;
+    const auto first_of = [&](uint32_t block) {
+        return static_cast<uint32_t>(static_cast<uint64_t>(block) * total / blocks);
+    };
+    const auto block_of = [&](uint32_t unit) {
+        return static_cast<uint32_t>(((static_cast<uint64_t>(unit) + 1) * blocks - 1) / total);
+    };
+    uint32_t at = first_of(blockIdx.x);
+    const uint32_t end = first_of(blockIdx.x + 1);
+    // The sequence the first unit lies in: a scan over the lengths, blockDim.x of them at a time.
+    uint32_t b = 0, before = 0;
+    for (uint32_t chunk = 0;; chunk += blockDim.x) {
+        __syncthreads();
+        const uint32_t i = chunk + threadIdx.x;
+        const uint32_t units = i < args.batch ? units_of(extent_of(args, i, nullptr)) * segments : 0;
+        uint32_t sum = units;
+#pragma unroll
+        for (uint32_t d = 1; d < 32; d *= 2) {
+            const uint32_t other = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += other;
+        }
+        if (lane == 31) scan[warp] = sum;
+        __syncthreads();
+        uint32_t ahead = before, all = before;
+        for (uint32_t w = 0; w < warps; ++w) {
+            if (w < warp) ahead += scan[w];
+            all += scan[w];
+        }
+        if (i < args.batch && at >= ahead + sum - units && at < ahead + sum) {
+            scan[16] = i;
+            scan[17] = ahead + sum - units;
+        }
+        __syncthreads();
+        if (at < all) {
+            b = scan[16];
+            before = scan[17];
+            break;
+        }
+        before = all;
     }
-    if (threadIdx.x < D)
-        static_cast<uint16_t*>(args.out)[place * D + threadIdx.x] =
-            static_cast<uint16_t>(E::pack(all == 0.0f ? 0.0f : y / all, 0.0f));
-    if (threadIdx.x == 0 && args.lse) args.lse[place] = all == 0.0f ? -INFINITY : top + logf(all);
+
+    uint8_t* const own = shared + warp * Shape::kWarpBytes;
+    Extent extent = extent_of(args, b, nullptr);
+    uint32_t units = units_of(extent);
+    uint32_t segment = (at - before) / units, from = (at - before) % units;
+
+    while (at < end) {
+        const uint32_t to = min(units, from + (end - at));
+        const uint32_t kv_head = segment / args.row_tiles, first_row = (segment % args.row_tiles) * kRows;
+
+        // ---- copies: each warp keeps a ring of its own, 32 tokens a stage, lane = token for addresses and
+        // parameters.
+        uint32_t masked = 0;  // bit s: some row may not see some token of stage s
+        const auto issue = [&](uint32_t unit, uint32_t stage) {
+            const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens + lane);
+            const int32_t token = extent.token(place);
+            bool real = place < extent.visible();
+            uint32_t row = 0;
+            if (real) {
+                const uint32_t entry = args.page.quotient(static_cast<uint32_t>(token));
+                const uint32_t page =
+                    args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + entry)) : b;
+                real = page < args.pages;
+                if (real)
+                    row = (page * args.kv_heads + kv_head) * args.page_size + (static_cast<uint32_t>(token) - entry * args.page_size);
+                else
+                    note(status, kBadPage, b, page);
+            }
+            const uint32_t stage_at = smem_u32(own + stage * Shape::kStageBytes);
+            constexpr uint32_t kChunks = D / 32;  // 16-byte pieces of a row's codes
+#pragma unroll
+            for (uint32_t i = 0; i < kChunks; ++i) {
+                const uint32_t owner = i * (32 / kChunks) + lane / kChunks;
+                const uint32_t its_row = __shfl_sync(0xffffffffu, row, owner);
+                const bool its_real = __shfl_sync(0xffffffffu, static_cast<uint32_t>(real), owner) != 0;
+                const uint64_t offset = static_cast<uint64_t>(its_row) * (D / 2) + (lane % kChunks) * 16;
+                const uint32_t to_at = stage_at + (i * 32 + lane) * 16;
+                if (its_real) {
+                    copy_async_16(to_at, args.codes[0] + offset);
+                    copy_async_16(to_at + Shape::kCodeBytes, args.codes[1] + offset);
+                }
+            }
+            const uint64_t param_offset = static_cast<uint64_t>(row) * (kGroups * 4);
+            const uint32_t param_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
+            copy_async_params<kGroups * 4>(param_at, args.params[0] + param_offset, real);
+            copy_async_params<kGroups * 4>(param_at + Shape::kParamBytes, args.params[1] + param_offset, real);
+            // A place that holds no token lies behind every query.
+            *reinterpret_cast<int32_t*>(own + stage * Shape::kStageBytes + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes +
+                                        lane * 4) = real ? token : 0x7fffffff;
+            const bool partly = !real || token > extent.first ||
+                                (args.window && token >= args.sinks &&
+                                 token <= extent.length - 1 - args.window);
+            masked = (masked & ~(1u << stage)) | (__any_sync(0xffffffffu, partly) ? 1u << stage : 0u);
+        };
+#pragma unroll
+        for (uint32_t s = 0; s < kStages - 1; ++s) {
+            if (from + s < to) issue(from + s, s);
+            copy_async_commit();
+        }
+
+        // ---- queries as the second operand of the scores' product: lane (l4, c4) holds row l4 of each 8, in the
+        // channel order of the key codes. A row is scaled by a power of two so that its largest value lies in
+        // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second half of each pair of registers
+        // carries 1/16 for the codes that stay in the upper nibble.
+        uint32_t qf[NT][D / 16][2];
+        float q_sum[NT][kGroups][2], to_log2[NT][2];
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n) {
+            const uint32_t r = first_row + 8 * n + l4;
+            float v[kKeyWords][8];
+            float most = 0.0f;
+            const uint32_t t = args.ratio.quotient(min(r, args.rows - 1));
+            const uint8_t* q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
+                               (kv_head * args.ratio.divisor + (min(r, args.rows - 1) - t * args.ratio.divisor)) * args.q_head_stride;
+#pragma unroll
+            for (uint32_t w = 0; w < kKeyWords; ++w) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < args.rows) x = __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4);
+                const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    v[w][2 * i] = E::low(words[i]);
+                    v[w][2 * i + 1] = E::high(words[i]);
+                    most = fmaxf(most, fmaxf(fabsf(v[w][2 * i]), fabsf(v[w][2 * i + 1])));
+                }
+            }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int32_t exponent = static_cast<int32_t>(__float_as_uint(most) >> 23);
+            const int32_t biased = most == 0.0f ? 127 : min(max(268 - exponent, 1), 254);
+            const float up = args.scale < 0.0f ? -power_of_two(biased) : power_of_two(biased);
+            float sums[kGroups] = {};
+#pragma unroll
+            for (uint32_t w = 0; w < kKeyWords; ++w) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) {
+                    v[w][i] *= up;
+                    sums[w * 32 / G] += v[w][i];
+                }
+                qf[n][2 * w][0] = Element<false>::pack(v[w][0], v[w][4]);
+                qf[n][2 * w][1] = Element<false>::pack(v[w][1] * 0.0625f, v[w][5] * 0.0625f);
+                qf[n][2 * w + 1][0] = Element<false>::pack(v[w][2], v[w][6]);
+                qf[n][2 * w + 1][1] = Element<false>::pack(v[w][3] * 0.0625f, v[w][7] * 0.0625f);
+            }
+            // Scores come out in units of 2^24 / up; a factor of zero would make NaN of a hidden token's -inf.
+            const float factor = fmaxf(fabsf(args.scale) * 1.4426950408889634f * 0x1p24f * power_of_two(254 - biased), 1e-37f);
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) to_log2[n][e] = __shfl_sync(0xffffffffu, factor, 8 * c4 + 4 * e);
+#pragma unroll
+            for (uint32_t g = 0; g < kGroups; ++g) {
+                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
+                sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
+                sums[g] *= 0x1p-24f;
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) q_sum[n][g][e] = __shfl_sync(0xffffffffu, sums[g], 8 * c4 + 4 * e);
+            }
+        }
+
+        float out[kTiles][NT][4] = {}, eights[kGroups][NT][4] = {}, lows[kGroups][NT][2] = {};
+        float peak[NT][2], sum[NT][2] = {};
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n) peak[n][0] = peak[n][1] = -INFINITY;
+        int32_t top = 0;  // biased exponent of the largest value scale so far
+
+        // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
+        // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
+        const uint32_t own_token = (l4 >> 1) + 4 * (l4 & 1);
+
+        for (uint32_t unit = from; unit < to; ++unit) {
+            const uint32_t stage = (unit - from) % kStages;
+            {
+                const uint32_t ahead = unit + kStages - 1;
+                __syncwarp();  // every lane is done with the stage that is filled next
+                if (ahead < to) issue(ahead, (ahead - from) % kStages);
+                copy_async_commit();
+                copy_async_wait<kStages - 1>();
+                __syncwarp();
+            }
+            const uint8_t* const keys = own + stage * Shape::kStageBytes;
+            const uint8_t* const values = keys + Shape::kCodeBytes;
+            const uint8_t* const key_params = keys + 2 * Shape::kCodeBytes;
+            const uint8_t* const value_params = key_params + Shape::kParamBytes;
+            const int32_t* const tokens = reinterpret_cast<const int32_t*>(value_params + Shape::kParamBytes);
+
+            // ---- scores of 32 tokens, transposed. A code in the low nibble of a half word IS the fp16 number code *
+            // 2^-24 (a subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
+            float x[2][NT][4];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                uint32_t a[2][kKeyWords], pairs[2][kGroups];
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    const uint32_t row = 16 * h + 8 * half + own_token;
+                    load_words(a[half], keys + row * (D / 2) + c4 * (D / 8));
+                    load_words(pairs[half], key_params + row * (kGroups * 4));
+                }
+#pragma unroll
+                for (uint32_t g = 0; g < kGroups; ++g) {
+                    float part[NT][4] = {};
+#pragma unroll
+                    for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w) {
+                        const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n) {
+                            mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
+                                        a[1][w] & 0x00f000f0u, qf[n][2 * w][0], qf[n][2 * w][1]);
+                            mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u,
+                                        qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
+                        }
+                    }
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const float rest = g == 0 ? E::high(pairs[i / 2][g]) * q_sum[n][g][i % 2]
+                                                      : fmaf(E::high(pairs[i / 2][g]), q_sum[n][g][i % 2], x[h][n][i]);
+                            x[h][n][i] = fmaf(E::low(pairs[i / 2][g]), part[n][i], rest);
+                        }
+                }
+            }
+            if (masked >> stage & 1u) {
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        const uint32_t t = args.ratio.quotient(min(first_row + 8 * n + 2 * c4 + e, args.rows - 1));
+                        const int32_t i = extent.length - static_cast<int32_t>(args.queries) + static_cast<int32_t>(t);
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                            for (uint32_t half = 0; half < 2; ++half) {
+                                const int32_t j = tokens[16 * h + 8 * half + own_token];
+                                const bool seen = j <= i && (!args.window || j > i - args.window || j < args.sinks);
+                                if (!seen) x[h][n][2 * half + e] = -INFINITY;
+                            }
+                    }
+            }
+
+            // ---- the running maximum of each row, and of the value scales' exponents; what was summed so far is
+            // rescaled only when one of them grows.
+            uint32_t scale_pairs[2][2][kGroups];
+            uint32_t widest = 0;
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    load_words(scale_pairs[h][half], value_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        const uint32_t bits = scale_pairs[h][half][g] & 0x7fffu;
+                        widest = max(widest, bits < (BF16 ? 0x7f80u : 0x7c00u) ? bits : 0u);
+                    }
+                }
+            widest = __reduce_max_sync(0xffffffffu, widest);
+            const int32_t unit_top = static_cast<int32_t>(__float_as_uint(E::low(widest)) >> 23);
+            float higher[NT][2];
+            bool grows = unit_top > top;
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    float m = fmaxf(fmaxf(x[0][n][e], x[0][n][2 + e]), fmaxf(x[1][n][e], x[1][n][2 + e]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    higher[n][e] = fmaxf(m, peak[n][e]);
+                    grows |= higher[n][e] > peak[n][e];
+                }
+            if (__any_sync(0xffffffffu, grows)) {
+                const int32_t new_top = max(top, unit_top);
+                const float shrink = power_of_two(max(127 + top - new_top, 0));
+                top = new_top;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) {
+                    float keep[2];
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        keep[e] = higher[n][e] > peak[n][e] ? ex2_approx((peak[n][e] - higher[n][e]) * to_log2[n][e]) : 1.0f;
+                        peak[n][e] = higher[n][e];
+                        sum[n][e] *= keep[e];
+#pragma unroll
+                        for (uint32_t g = 0; g < kGroups; ++g) lows[g][n][e] *= keep[e];
+                        keep[e] *= shrink;
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+#pragma unroll
+                        for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= keep[i % 2];
+#pragma unroll
+                        for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= keep[i % 2];
+                    }
+                }
+            }
+            // Weights times scales fit fp16 with their largest at 2^14 whatever the scales' size.
+            const float fit = power_of_two(min(267 - top, 254));
+
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                // ---- weights, their sums, and weight * scale in fp16, turned to be the values' second operand.
+                uint32_t weights[kGroups][NT][2];
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) {
+                    float p[4];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const float base = peak[n][i % 2] == -INFINITY ? 0.0f : peak[n][i % 2] * to_log2[n][i % 2];
+                        p[i] = ex2_approx(fmaf(x[h][n][i], to_log2[n][i % 2], -base));
+                        sum[n][i % 2] += p[i];
+                    }
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        float weight[4];
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t pair = scale_pairs[h][i / 2][g];
+                            const float scale = E::low(pair);
+                            // A token that is not seen may carry NaN.
+                            const bool seen = x[h][n][i] != -INFINITY;
+                            lows[g][n][i % 2] += seen ? p[i] * fmaf(8.0f, scale, E::high(pair)) : 0.0f;
+                            weight[i] = seen ? p[i] * (scale * fit) : 0.0f;
+                        }
+                        weights[g][n][0] = transpose_8x8(Element<false>::pack(weight[0], weight[1]));
+                        weights[g][n][1] = transpose_8x8(Element<false>::pack(weight[2], weight[3]));
+                    }
+                }
+                // ---- O^T += V^T . (P scale)^T. Two tokens' nibbles of a channel side by side are a pair of the first
+                // operand; the odd fragment rows' channels come 16 times too large. `eights` sums 8 * weight as rounded:
+                // codes count from their middle, and the rest, in fp32, is in `lows`.
+#pragma unroll
+                for (uint32_t g = 0; g < kGroups; ++g)
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n)
+                        mma_16x8x16(eights[g][n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, weights[g][n][0],
+                                    weights[g][n][1]);
+                uint32_t v[4][kValueWords];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    load_words(v[i], values + (16 * h + 4 * i + c4) * (D / 2) + l4 * (D / 16));
+#pragma unroll
+                for (uint32_t w = 0; w < kValueWords; ++w)
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; ++half) {
+                        uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
+                        uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (uint32_t byte = 0; byte < 2; ++byte) {
+                            const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
+#pragma unroll
+                            for (uint32_t n = 0; n < NT; ++n)
+                                mma_16x8x16(out[j][n], lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u,
+                                            weights[g][n][0], weights[g][n][1]);
+                            lo >>= 8;
+                            hi >>= 8;
+                        }
+                    }
+            }
+        }
+
+        // ---- the warps' parts of the piece, through shared memory
+        copy_async_wait<0>();
+        __syncthreads();
+        {
+            float* const merged = reinterpret_cast<float*>(own);
+            float* const stats = merged + kRows * kPitch;
+            const float unfit = power_of_two(254 - min(267 - top, 254));
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    float s = sum[n][e];
+                    float low[kGroups];
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) low[g] = lows[g][n][e];
+#pragma unroll
+                    for (uint32_t mask = 4; mask < 32; mask *= 2) {
+                        s += __shfl_xor_sync(0xffffffffu, s, mask);
+#pragma unroll
+                        for (uint32_t g = 0; g < kGroups; ++g) low[g] += __shfl_xor_sync(0xffffffffu, low[g], mask);
+                    }
+                    const uint32_t row = 8 * n + 2 * c4 + e;
+#pragma unroll
+                    for (uint32_t j = 0; j < kTiles; ++j) {
+                        const uint32_t g = 16 * j / G;
+                        merged[row * kPitch + 16 * j + l4] = fmaf((out[j][n][e] - eights[g][n][e]) * 0x1p24f, unfit, low[g]);
+                        merged[row * kPitch + 16 * j + 8 + l4] =
+                            fmaf((out[j][n][2 + e] * 0.0625f - eights[g][n][e]) * 0x1p24f, unfit, low[g]);
+                    }
+                    if (l4 == 0) {
+                        stats[2 * row] = peak[n][e] == -INFINITY ? -INFINITY : peak[n][e] * to_log2[n][e];
+                        stats[2 * row + 1] = s;
+                    }
+                }
+        }
+        __syncthreads();
+        const uint32_t rows_here = min(kRows, args.rows - first_row);
+        const bool whole = from == 0 && to == units;
+        const uint32_t segment_first = at - from;
+        // A segment cut over blocks: the block it begins in keeps its part in its second place, the others in their first.
+        const uint32_t owner = whole ? 0 : block_of(segment_first);
+        float* const part = args.partials + (2 * blockIdx.x + (owner == blockIdx.x ? 1 : 0)) * static_cast<size_t>(kPartialFloats);
+        const auto finish = [&](uint32_t row, uint32_t d, float y, float s, float m) {
+            const uint32_t r = first_row + row, t = args.ratio.quotient(r);
+            const uint64_t place = (static_cast<uint64_t>(b) * args.queries + t) * args.heads + kv_head * args.ratio.divisor +
+                                   (r - t * args.ratio.divisor);
+            args.out[place * D + d] = static_cast<uint16_t>(E::pack(s == 0.0f ? 0.0f : __fdividef(y, s), 0.0f));
+            if (d == 0 && args.lse) args.lse[place] = s == 0.0f ? -INFINITY : (m + log2f(s)) * 0.6931471805599453f;
+        };
+        for (uint32_t i = threadIdx.x; i < rows_here * D; i += blockDim.x) {
+            const uint32_t row = i / D, d = i % D;
+            float m = -INFINITY, y = 0.0f, s = 0.0f;
+            for (uint32_t w = 0; w < warps; ++w)
+                m = fmaxf(m, reinterpret_cast<const float*>(shared + w * Shape::kWarpBytes)[kRows * kPitch + 2 * row]);
+            for (uint32_t w = 0; w < warps; ++w) {
+                const float* const theirs = reinterpret_cast<const float*>(shared + w * Shape::kWarpBytes);
+                const float its_peak = theirs[kRows * kPitch + 2 * row];
+                const float share = its_peak == -INFINITY ? 0.0f : ex2_approx(its_peak - m);
+                y = fmaf(theirs[row * kPitch + d], share, y);
+                s = fmaf(theirs[kRows * kPitch + 2 * row + 1], share, s);
+            }
+            if (whole) {
+                finish(row, d, y, s, m);
+            } else {
+                part[row * D + d] = y;
+                if (d == 0) {
+                    part[kMostRows * 128 + 2 * row] = m;
+                    part[kMostRows * 128 + 2 * row + 1] = s;
+                }
+            }
+        }
+        if (!whole) {
+            // The block that comes last adds the parts up, always in the same order.
+            const uint32_t parts = block_of(segment_first + units - 1) - owner + 1;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const uint32_t came = atomicAdd(args.arrivals + owner, 1u);
+                if (came == parts - 1) args.arrivals[owner] = 0;
+                scan[0] = came == parts - 1;
+            }
+            __syncthreads();
+            if (scan[0]) {
+                __threadfence();
+                const float* const base = args.partials + 2 * owner * static_cast<size_t>(kPartialFloats);
+                for (uint32_t i = threadIdx.x; i < rows_here * D; i += blockDim.x) {
+                    const uint32_t row = i / D, d = i % D;
+                    const auto part_of = [&](uint32_t p) { return base + (2 * p + (p == 0)) * static_cast<size_t>(kPartialFloats); };
+                    float m = -INFINITY, y = 0.0f, s = 0.0f;
+#pragma unroll 8
+                    for (uint32_t p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(part_of(p) + kMostRows * 128 + 2 * row));
+#pragma unroll 8
+                    for (uint32_t p = 0; p < parts; ++p) {
+                        const float its_peak = __ldcg(part_of(p) + kMostRows * 128 + 2 * row);
+                        const float share = its_peak == -INFINITY ? 0.0f : ex2_approx(its_peak - m);
+                        y = fmaf(__ldcg(part_of(p) + row * D + d), share, y);
+                        s = fmaf(__ldcg(part_of(p) + kMostRows * 128 + 2 * row + 1), share, s);
+                    }
+                    finish(row, d, y, s, m);
+                }
+            }
+        }
+        __syncthreads();  // the merged rows lie where the rings are
+
+        at += to - from;
+        from = 0;
+        if (to == units && ++segment == segments && at < end) {
+            segment = 0;
+            ++b;
+            extent = extent_of(args, b, nullptr);
+            units = units_of(extent);
+        }
+    }
 }
 
 }  // namespace cache
@@ -520,7 +1036,35 @@ extern "C" int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t 
                      tokens, clear_skipped, stream, device_status);
 }
 
-extern "C" uint64_t fk_cache_attention_workspace_bytes(uint32_t sm_count) { return 16ull * sm_count; }
+// Per resident block a counter and the parts of the two segments that its share may begin and end inside of.
+extern "C" uint64_t fk_cache_attention_workspace_bytes(uint32_t sm_count) {
+    const uint64_t blocks = static_cast<uint64_t>(sm_count) * cache::kMostBlocksPerSm;
+    return (blocks * 4 + 127) / 128 * 128 + blocks * 2 * cache::kPartialFloats * 4;
+}
+
+template <int D, int G, int NT, bool BF16>
+static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& facts, void* stream, uint32_t* device_status) {
+    using Shape = cache::AttentionShape<D, G, NT>;
+    const auto kernel = cache::attention_kernel<D, G, NT, BF16>;
+    uint32_t limit = 0;
+    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::kMostWarps * Shape::kWarpBytes, &limit);
+    if (admitted != FK_OK) return admitted;
+    args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
+    const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
+    const uint32_t small = 4;
+    const uint32_t warps = segments >= 2ull * facts.sm_count ? small : Shape::kMostWarps;
+    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (warps == small ? Shape::kMostWarps / small : 1);
+    const uint64_t unit_tokens = warps * cache::kWarpTokens;
+    const uint64_t most_units = segments * ((static_cast<uint64_t>(args.table_pages) * args.page_size + unit_tokens - 1) / unit_tokens);
+    if (most_units >= (1ull << 31))
+        return fk_fail(FK_ERR_SHAPE, "%u sequences of up to %llu tokens on %u heads are more than a launch counts", args.batch,
+                       static_cast<unsigned long long>(args.table_pages) * args.page_size, args.kv_heads);
+    args.least_units = 1;
+    const uint32_t grid = most_units < resident ? static_cast<uint32_t>(most_units) : resident;
+    kernel<<<grid, warps * 32, warps * Shape::kWarpBytes, static_cast<cudaStream_t>(stream)>>>(args, device_status);
+    FK_CUDA(cudaGetLastError());
+    return FK_OK;
+}
 
 extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_t q_batch_stride,
                                   int64_t q_token_stride, int64_t q_head_stride, void* out, float* lse,
@@ -559,16 +1103,19 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
         return fk_fail(FK_ERR_SHAPE, "a workspace of %llu bytes is under the %llu of this device",
                        static_cast<unsigned long long>(workspace_bytes),
                        static_cast<unsigned long long>(fk_cache_attention_workspace_bytes(facts.sm_count)));
+    const uint64_t rows = static_cast<uint64_t>(queries) * (heads / cache->kv_heads);
+    if (rows >= (1ull << 30))
+        return fk_fail(FK_ERR_SHAPE, "%u queries of %u heads are more rows than a launch counts", queries, heads);
     cache::AttentionArguments args;
-    args.k_codes = static_cast<const uint8_t*>(cache->k_codes);
-    args.k_params = static_cast<const uint32_t*>(cache->k_params);
-    args.v_codes = static_cast<const uint8_t*>(cache->v_codes);
-    args.v_params = static_cast<const uint32_t*>(cache->v_params);
+    args.codes[0] = static_cast<const uint8_t*>(cache->k_codes);
+    args.codes[1] = static_cast<const uint8_t*>(cache->v_codes);
+    args.params[0] = static_cast<const uint8_t*>(cache->k_params);
+    args.params[1] = static_cast<const uint8_t*>(cache->v_params);
     args.q = static_cast<const uint8_t*>(q);
     args.q_batch_stride = 2 * q_batch_stride;
     args.q_token_stride = 2 * q_token_stride;
     args.q_head_stride = 2 * q_head_stride;
-    args.out = out;
+    args.out = static_cast<uint16_t*>(out);
     args.lse = lse;
     args.lengths = lengths;
     args.table = table;
@@ -580,15 +1127,18 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
     args.queries = queries;
     args.heads = heads;
     args.kv_heads = cache->kv_heads;
+    args.rows = static_cast<uint32_t>(rows);
     args.scale = scale;
-    args.window = window;
-    args.sinks = sinks;
+    args.window = static_cast<int32_t>(window < 0x7fffffffu ? window : 0x7fffffffu);
+    args.sinks = static_cast<int32_t>(sinks < 0x7fffffffu ? sinks : 0x7fffffffu);
     args.page = cache::Divider(cache->page_size);
+    args.ratio = cache::Divider(heads / cache->kv_heads);
+    args.arrivals = static_cast<uint32_t*>(workspace);
+    const uint64_t counters = (static_cast<uint64_t>(facts.sm_count) * cache::kMostBlocksPerSm * 4 + 127) / 128 * 128;
+    args.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + counters);
     return for_cache(cache, [&](auto dim, auto group, auto bf16) {
-        cache::attention_kernel<dim, group, bf16>
-            <<<dim3(queries * heads, batch), cache::kAttentionThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-                args, device_status);
-        FK_CUDA(cudaGetLastError());
-        return static_cast<int>(FK_OK);
+        if (rows <= 8) return launch_attention<dim, group, 1, bf16>(args, facts, stream, device_status);
+        if (rows <= 16) return launch_attention<dim, group, 2, bf16>(args, facts, stream, device_status);
+        return launch_attention<dim, group, 4, bf16>(args, facts, stream, device_status);
     });
 }
