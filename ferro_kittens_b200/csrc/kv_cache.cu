@@ -311,7 +311,8 @@ struct AttentionArguments {
     float scale;
     int32_t window, sinks;
     Divider page, ratio;
-    uint32_t least_units;  // units a block takes before another block is put to work
+    uint32_t least_units;   // units a block takes before another block is put to work
+    uint32_t segment_cost;  // what beginning and ending a segment takes, in units
     uint32_t* arrivals;    // workspace: a counter for each block, then the partial results
     float* partials;
 };
@@ -322,21 +323,30 @@ constexpr uint32_t kMostBlocksPerSm = 4;
 constexpr uint32_t kMostRows = 32;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
 constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
+constexpr uint32_t kStallCodes = 0x504;  // a warp waiting for a stage of codes
 
 template <int D, int G, int NT>
 struct AttentionShape {
     static constexpr uint32_t kGroups = D / G;
     static constexpr uint32_t kRows = 8 * NT;
+    // One row tile's queries stay in registers; of more, the fragments and sums lie in shared memory.
+    static constexpr bool kSharedQueries = NT > 1;
+    static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 : 0;
+    // A warp's memory: a ring of stages, the unit's parameters as floats, the stages' barriers; the merge of the warps'
+    // results lies over the first two.
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
     static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
     static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes + kWarpTokens * 4;
-    static constexpr uint32_t kRingBytes = kStages * kStageBytes;
+    static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 8;
+    static constexpr uint32_t kRingBytes = kStages * kStageBytes + 2 * kWideBytes;
     static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
     static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
-    static constexpr uint32_t kWarpBytes = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
+    static constexpr uint32_t kBarriers = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
+    static constexpr uint32_t kWarpBytes = kBarriers + (kStages * 8 + 15) / 16 * 16;
     static constexpr uint32_t kMostByRegisters = NT == 1 ? 16 : NT == 2 ? 12 : 8;  // 128, 168, 255 a thread
-    static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048) / kWarpBytes;
+    static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
     static constexpr uint32_t kMostWarps = kMostByRegisters < kMostByMemory ? kMostByRegisters : kMostByMemory;
+    static constexpr uint32_t shared_bytes(uint32_t warps) { return kQueryBytes + warps * kWarpBytes; }
 };
 
 /// What of a sequence is read: its tokens, less those between the sinks and the window that no query row sees.
@@ -362,8 +372,11 @@ __device__ __forceinline__ Extent extent_of(const AttentionArguments& args, uint
     return e;
 }
 
-__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+        "l"(src), "r"(bytes), "r"(bar)
+        : "memory");
 }
 /// BYTES of a row's parameters, or zeros where the row is not to be read.
 template <int BYTES>
@@ -393,19 +406,34 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
     return d;
 }
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 __device__ __forceinline__ float power_of_two(int32_t biased) { return __int_as_float(biased << 23); }
 
 template <int WORDS>
-__device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const uint8_t* from) {
-    if constexpr (WORDS == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(from);
+__device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const void* from) {
+    if constexpr (WORDS == 8) {
+        const uint4 x = static_cast<const uint4*>(from)[0], y = static_cast<const uint4*>(from)[1];
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+    } else if constexpr (WORDS == 4) {
+        const uint4 x = *static_cast<const uint4*>(from);
         w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else if constexpr (WORDS == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(from);
+        const uint2 x = *static_cast<const uint2*>(from);
         w[0] = x.x, w[1] = x.y;
     } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(from);
+        w[0] = *static_cast<const uint32_t*>(from);
     }
+}
+
+template <int PAIRS>
+__device__ __forceinline__ void store_floats(void* to, const float2 (&x)[PAIRS]) {
+    if constexpr (PAIRS == 1) *static_cast<float2*>(to) = x[0];
+#pragma unroll
+    for (int i = 0; i + 1 < PAIRS; i += 2) static_cast<float4*>(to)[i / 2] = make_float4(x[i].x, x[i].y, x[i + 1].x, x[i + 1].y);
 }
 
 template <int D, int G, int NT, bool BF16>
@@ -415,389 +443,499 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     using Shape = AttentionShape<D, G, NT>;
     constexpr uint32_t kGroups = Shape::kGroups, kRows = Shape::kRows, kPitch = Shape::kPitch;
     constexpr uint32_t kKeyWords = D / 32, kValueWords = D / 64, kTiles = D / 16;
+    constexpr uint32_t kSteps = NT == 4 ? 1 : 2;      // steps of 16 tokens between looks at the running maximum
+    constexpr bool kEights = NT == 1;                 // see `eights` below
     extern __shared__ __align__(16) uint8_t shared[];
-    __shared__ uint32_t scan[18];
+    __shared__ uint32_t last_to_come, stop_flag;
     const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
     const uint32_t l4 = lane / 4, c4 = lane % 4;
+    uint8_t* const own = shared + Shape::kQueryBytes + warp * Shape::kWarpBytes;
+    const uint32_t barriers = smem_u32(own + Shape::kBarriers);
 
     // ---- this block's share: units of unit_tokens tokens, sequence by sequence, (kv head, row tile) by (kv head,
-    // row tile), cut evenly over the blocks whatever the lengths are.
+    // row tile), cut evenly over the blocks whatever the lengths are. A segment, one sequence's units of one (kv
+    // head, row tile), begins with args.segment_cost units of no work: what beginning and ending it takes. Every warp
+    // goes through the lengths by itself.
     const uint32_t segments = args.kv_heads * args.row_tiles;  // of one sequence
-    const auto units_of = [&](const Extent& e) {
-        return max((static_cast<uint32_t>(e.visible()) + unit_tokens - 1) / unit_tokens, 1u);
+    const auto cost_of = [&](const Extent& e) {
+        return max((static_cast<uint32_t>(e.visible()) + unit_tokens - 1) / unit_tokens, 1u) + args.segment_cost;
     };
-    uint32_t mine = 0;
-    for (uint32_t b = threadIdx.x; b < args.batch; b += blockDim.x) mine += units_of(extent_of(args, b, status));
-#pragma unroll
-    for (uint32_t mask = 16; mask > 0; mask >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, mask);
-    if (lane == 0) scan[warp] = mine;
-    __syncthreads();
     uint32_t total = 0;
-    for (uint32_t w = 0; w < warps; ++w) total += scan[w];
-    total *= segments;
+    for (uint32_t i = lane; i < args.batch; i += 32) total += cost_of(extent_of(args, i, status));
+    total = __reduce_add_sync(0xffffffffu, total) * segments;
     const uint32_t blocks = min(gridDim.x, max(total / args.least_units, 1u));
     if (blockIdx.x >= blocks) return;
     const auto first_of = [&](uint32_t block) {
         return static_cast<uint32_t>(static_cast<uint64_t>(block) * total / blocks);
     };
-    const auto block_of = [&](uint32_t unit) {
-        return static_cast<uint32_t>(((static_cast<uint64_t>(unit) + 1) * blocks - 1) / total);
+    const auto block_of = [&](uint32_t place) {
+        return static_cast<uint32_t>(((static_cast<uint64_t>(place) + 1) * blocks - 1) / total);
     };
     uint32_t at = first_of(blockIdx.x);
     const uint32_t end = first_of(blockIdx.x + 1);
-    // The sequence the first unit lies in: a scan over the lengths, blockDim.x of them at a time.
     uint32_t b = 0, before = 0;
-    for (uint32_t chunk = 0;; chunk += blockDim.x) {
-        __syncthreads();
-        const uint32_t i = chunk + threadIdx.x;
-        const uint32_t units = i < args.batch ? units_of(extent_of(args, i, nullptr)) * segments : 0;
-        uint32_t sum = units;
+    for (uint32_t chunk = 0;; chunk += 32) {
+        const uint32_t i = chunk + lane;
+        const uint32_t cost = i < args.batch ? cost_of(extent_of(args, i, nullptr)) * segments : 0;
+        uint32_t sum = cost;
 #pragma unroll
         for (uint32_t d = 1; d < 32; d *= 2) {
             const uint32_t other = __shfl_up_sync(0xffffffffu, sum, d);
             if (lane >= d) sum += other;
         }
-        if (lane == 31) scan[warp] = sum;
-        __syncthreads();
-        uint32_t ahead = before, all = before;
-        for (uint32_t w = 0; w < warps; ++w) {
-            if (w < warp) ahead += scan[w];
-            all += scan[w];
-        }
-        if (i < args.batch && at >= ahead + sum - units && at < ahead + sum) {
-            scan[16] = i;
-            scan[17] = ahead + sum - units;
-        }
-        __syncthreads();
-        if (at < all) {
-            b = scan[16];
-            before = scan[17];
+        // The lane whose sequence the share begins in: the first whose sum passes it.
+        const uint32_t past = __ballot_sync(0xffffffffu, at < before + sum);
+        if (past) {
+            const uint32_t found = __ffs(past) - 1;
+            b = chunk + found;
+            before += __shfl_sync(0xffffffffu, sum - cost, found);
             break;
         }
-        before = all;
+        before += __shfl_sync(0xffffffffu, sum, 31);
     }
 
-    uint8_t* const own = shared + warp * Shape::kWarpBytes;
+    if (lane == 0)
+        for (uint32_t s = 0; s < kStages; ++s) mbar_init(barriers + 8 * s, 1);
+    if (threadIdx.x == 0) stop_flag = 0;
+    fence_mbarrier_init();
+    __syncthreads();
+    const StallSite site{status, &stop_flag, 0};
+
     Extent extent = extent_of(args, b, nullptr);
-    uint32_t units = units_of(extent);
-    uint32_t segment = (at - before) / units, from = (at - before) % units;
+    uint32_t cost = cost_of(extent);
+    uint32_t segment = (at - before) / cost;
+    uint32_t offset = (at - before) - segment * cost;  // of `at` in its segment
+    uint32_t fill_stage = 0, use_stage = 0, use_parity = 0;
 
     while (at < end) {
-        const uint32_t to = min(units, from + (end - at));
+        const uint32_t length = min(cost - offset, end - at);  // of the share that lies in this segment
+        const uint32_t units = cost - args.segment_cost;
+        const uint32_t from = offset > args.segment_cost ? offset - args.segment_cost : 0;
+        const uint32_t to = offset + length > args.segment_cost ? offset + length - args.segment_cost : 0;
+        const uint32_t segment_at = at - offset + args.segment_cost;  // the place of its first unit
+        if (from < to) {
         const uint32_t kv_head = segment / args.row_tiles, first_row = (segment % args.row_tiles) * kRows;
 
-        // ---- copies: each warp keeps a ring of its own, 32 tokens a stage, lane = token for addresses and
-        // parameters.
+        // ---- copies: each warp keeps a ring of its own, 32 tokens a stage, lane = token. Tokens that follow each other
+        // in the cache are copied as one run of each code matrix by the lane of the run's first token; parameters come
+        // lane by lane (their rows are too short for bulk copies) as zeros where there is no token. The rows are looked up
+        // one unit ahead of their copies.
         uint32_t masked = 0;  // bit s: some row may not see some token of stage s
-        const auto issue = [&](uint32_t unit, uint32_t stage) {
+        struct Place {
+            int32_t row, token;  // row -1: nothing to read
+        };
+        const auto locate = [&](uint32_t unit) {
             const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens + lane);
-            const int32_t token = extent.token(place);
-            bool real = place < extent.visible();
-            uint32_t row = 0;
-            if (real) {
-                const uint32_t entry = args.page.quotient(static_cast<uint32_t>(token));
+            Place p{-1, extent.token(place)};
+            if (place < extent.visible()) {
+                const uint32_t entry = args.page.quotient(static_cast<uint32_t>(p.token));
                 const uint32_t page =
                     args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + entry)) : b;
-                real = page < args.pages;
-                if (real)
-                    row = (page * args.kv_heads + kv_head) * args.page_size + (static_cast<uint32_t>(token) - entry * args.page_size);
+                if (page < args.pages)
+                    p.row = static_cast<int32_t>((page * args.kv_heads + kv_head) * args.page_size +
+                                                 (static_cast<uint32_t>(p.token) - entry * args.page_size));
                 else
                     note(status, kBadPage, b, page);
             }
-            const uint32_t stage_at = smem_u32(own + stage * Shape::kStageBytes);
-            constexpr uint32_t kChunks = D / 32;  // 16-byte pieces of a row's codes
-#pragma unroll
-            for (uint32_t i = 0; i < kChunks; ++i) {
-                const uint32_t owner = i * (32 / kChunks) + lane / kChunks;
-                const uint32_t its_row = __shfl_sync(0xffffffffu, row, owner);
-                const bool its_real = __shfl_sync(0xffffffffu, static_cast<uint32_t>(real), owner) != 0;
-                const uint64_t offset = static_cast<uint64_t>(its_row) * (D / 2) + (lane % kChunks) * 16;
-                const uint32_t to_at = stage_at + (i * 32 + lane) * 16;
-                if (its_real) {
-                    copy_async_16(to_at, args.codes[0] + offset);
-                    copy_async_16(to_at + Shape::kCodeBytes, args.codes[1] + offset);
-                }
-            }
-            const uint64_t param_offset = static_cast<uint64_t>(row) * (kGroups * 4);
-            const uint32_t param_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
-            copy_async_params<kGroups * 4>(param_at, args.params[0] + param_offset, real);
-            copy_async_params<kGroups * 4>(param_at + Shape::kParamBytes, args.params[1] + param_offset, real);
-            // A place that holds no token lies behind every query.
-            *reinterpret_cast<int32_t*>(own + stage * Shape::kStageBytes + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes +
-                                        lane * 4) = real ? token : 0x7fffffff;
-            const bool partly = !real || token > extent.first ||
-                                (args.window && token >= args.sinks &&
-                                 token <= extent.length - 1 - args.window);
-            masked = (masked & ~(1u << stage)) | (__any_sync(0xffffffffu, partly) ? 1u << stage : 0u);
+            return p;
         };
+        const auto issue = [&](const Place& p) {
+            uint8_t* const stage = own + fill_stage * Shape::kStageBytes;
+            const uint32_t stage_at = smem_u32(stage), bar = barriers + 8 * fill_stage;
+            const int32_t ahead = __shfl_up_sync(0xffffffffu, p.row, 1);
+            const bool begins = p.row >= 0 && (lane == 0 || ahead < 0 || ahead + 1 != p.row);
+            const uint32_t begin = __ballot_sync(0xffffffffu, begins), real = __ballot_sync(0xffffffffu, p.row >= 0);
+            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(real) * D);
+            if (begins) {
+                const uint32_t next = ((begin | ~real) >> lane) >> 1;
+                const uint32_t bytes = (next ? __ffs(next) : 32 - lane) * (D / 2);
+                const uint64_t source = static_cast<uint64_t>(p.row) * (D / 2);
+                bulk_load(stage_at + lane * (D / 2), args.codes[0] + source, bytes, bar);
+                bulk_load(stage_at + Shape::kCodeBytes + lane * (D / 2), args.codes[1] + source, bytes, bar);
+            }
+            const uint64_t params = static_cast<uint64_t>(max(p.row, 0)) * (kGroups * 4);
+            const uint32_t params_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
+            copy_async_params<kGroups * 4>(params_at, args.params[0] + params, p.row >= 0);
+            copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, p.row >= 0);
+            // A place that holds no token lies behind every query.
+            reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
+                p.row >= 0 ? p.token : 0x7fffffff;
+            const bool partly = p.row < 0 || p.token > extent.first ||
+                                (args.window && p.token >= args.sinks && p.token <= extent.length - 1 - args.window);
+            masked = (masked & ~(1u << fill_stage)) | (__any_sync(0xffffffffu, partly) ? 1u << fill_stage : 0u);
+            fill_stage = fill_stage == kStages - 1 ? 0 : fill_stage + 1;
+        };
+        Place next = locate(from);
 #pragma unroll
         for (uint32_t s = 0; s < kStages - 1; ++s) {
-            if (from + s < to) issue(from + s, s);
+            if (from + s < to) {
+                issue(next);
+                next = locate(from + s + 1);
+            }
             copy_async_commit();
         }
 
         // ---- queries as the second operand of the scores' product: lane (l4, c4) holds row l4 of each 8, in the
-        // channel order of the key codes. A row is scaled by a power of two so that its largest value lies in
-        // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second half of each pair of registers
-        // carries 1/16 for the codes that stay in the upper nibble.
-        uint32_t qf[NT][D / 16][2];
-        float q_sum[NT][kGroups][2], to_log2[NT][2];
+        // channel order of the key codes. The tile is scaled by a power of two so that its largest value lies in
+        // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second register of each pair carries 1/16 for
+        // the codes that stay in the upper nibble. q_sum is a group's sum, for the smallest values; to_log2 makes scores
+        // of the products, in powers of two.
+        uint32_t qf[Shape::kSharedQueries ? 1 : D / 16][2];
+        float q_sum[Shape::kSharedQueries ? 1 : kGroups][2];
+        uint4* const shared_q = reinterpret_cast<uint4*>(shared);
+        float* const shared_sums = reinterpret_cast<float*>(shared + kRows * D * 2);
+        const auto row_of = [&](uint32_t n) {
+            const uint32_t r = min(first_row + 8 * n + l4, args.rows - 1), t = args.ratio.quotient(r);
+            return args.q + b * args.q_batch_stride + t * args.q_token_stride +
+                   (kv_head * args.ratio.divisor + (r - t * args.ratio.divisor)) * args.q_head_stride;
+        };
+        uint4 raw[NT][kKeyWords];
+        float most = 0.0f;
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) {
-            const uint32_t r = first_row + 8 * n + l4;
-            float v[kKeyWords][8];
-            float most = 0.0f;
-            const uint32_t t = args.ratio.quotient(min(r, args.rows - 1));
-            const uint8_t* q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
-                               (kv_head * args.ratio.divisor + (min(r, args.rows - 1) - t * args.ratio.divisor)) * args.q_head_stride;
+            const uint8_t* const q = row_of(n);
 #pragma unroll
             for (uint32_t w = 0; w < kKeyWords; ++w) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < args.rows) x = __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4);
-                const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+                raw[n][w] = make_uint4(0, 0, 0, 0);
+                if (first_row + 8 * n + l4 < args.rows) raw[n][w] = __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4);
+                const uint32_t words[4] = {raw[n][w].x, raw[n][w].y, raw[n][w].z, raw[n][w].w};
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    v[w][2 * i] = E::low(words[i]);
-                    v[w][2 * i + 1] = E::high(words[i]);
-                    most = fmaxf(most, fmaxf(fabsf(v[w][2 * i]), fabsf(v[w][2 * i + 1])));
-                }
+                for (uint32_t i = 0; i < 4; ++i)
+                    most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
             }
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int32_t exponent = static_cast<int32_t>(__float_as_uint(most) >> 23);
-            const int32_t biased = most == 0.0f ? 127 : min(max(268 - exponent, 1), 254);
-            const float up = args.scale < 0.0f ? -power_of_two(biased) : power_of_two(biased);
+        }
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u));
+        const int32_t biased = most == 0.0f ? 127 : min(268 - static_cast<int32_t>(__float_as_uint(most) >> 23), 254);
+        const float up = power_of_two(biased);
+        const float to_log2 = args.scale * 1.4426950408889634f * 0x1p24f * power_of_two(254 - biased);
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n) {
             float sums[kGroups] = {};
 #pragma unroll
             for (uint32_t w = 0; w < kKeyWords; ++w) {
+                const uint32_t words[4] = {raw[n][w].x, raw[n][w].y, raw[n][w].z, raw[n][w].w};
+                float v[8];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    v[w][i] *= up;
-                    sums[w * 32 / G] += v[w][i];
+                for (uint32_t i = 0; i < 4; ++i) {
+                    v[2 * i] = E::low(words[i]) * up;
+                    v[2 * i + 1] = E::high(words[i]) * up;
+                    sums[w * 32 / G] += v[2 * i] + v[2 * i + 1];
                 }
-                qf[n][2 * w][0] = Element<false>::pack(v[w][0], v[w][4]);
-                qf[n][2 * w][1] = Element<false>::pack(v[w][1] * 0.0625f, v[w][5] * 0.0625f);
-                qf[n][2 * w + 1][0] = Element<false>::pack(v[w][2], v[w][6]);
-                qf[n][2 * w + 1][1] = Element<false>::pack(v[w][3] * 0.0625f, v[w][7] * 0.0625f);
+                uint4 f;
+                f.x = Element<false>::pack(v[0], v[4]);
+                f.y = Element<false>::pack(v[1] * 0.0625f, v[5] * 0.0625f);
+                f.z = Element<false>::pack(v[2], v[6]);
+                f.w = Element<false>::pack(v[3] * 0.0625f, v[7] * 0.0625f);
+                if constexpr (Shape::kSharedQueries) {
+                    if (warp == n % warps) shared_q[(n * kKeyWords + w) * 32 + lane] = f;
+                } else {
+                    qf[2 * w][0] = f.x, qf[2 * w][1] = f.y, qf[2 * w + 1][0] = f.z, qf[2 * w + 1][1] = f.w;
+                }
             }
-            // Scores come out in units of 2^24 / up; a factor of zero would make NaN of a hidden token's -inf.
-            const float factor = fmaxf(fabsf(args.scale) * 1.4426950408889634f * 0x1p24f * power_of_two(254 - biased), 1e-37f);
-#pragma unroll
-            for (uint32_t e = 0; e < 2; ++e) to_log2[n][e] = __shfl_sync(0xffffffffu, factor, 8 * c4 + 4 * e);
 #pragma unroll
             for (uint32_t g = 0; g < kGroups; ++g) {
                 sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
                 sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
                 sums[g] *= 0x1p-24f;
+                if constexpr (Shape::kSharedQueries) {
+                    if (warp == n % warps && c4 == 0) shared_sums[g * kRows + 8 * n + l4] = sums[g];
+                } else {
 #pragma unroll
-                for (uint32_t e = 0; e < 2; ++e) q_sum[n][g][e] = __shfl_sync(0xffffffffu, sums[g], 8 * c4 + 4 * e);
+                    for (uint32_t e = 0; e < 2; ++e) q_sum[g][e] = __shfl_sync(0xffffffffu, sums[g], 8 * c4 + 4 * e);
+                }
             }
         }
+        if constexpr (Shape::kSharedQueries) __syncthreads();
 
-        float out[kTiles][NT][4] = {}, eights[kGroups][NT][4] = {}, lows[kGroups][NT][2] = {};
+        float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {}, lows[kGroups][NT][2] = {};
         float peak[NT][2], sum[NT][2] = {};
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) peak[n][0] = peak[n][1] = -INFINITY;
         int32_t top = 0;  // biased exponent of the largest value scale so far
+        float fit = power_of_two(254);
 
         // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
         // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
         const uint32_t own_token = (l4 >> 1) + 4 * (l4 & 1);
+        uint8_t* const wide_keys = own + kStages * Shape::kStageBytes;  // (scale, low) * to_log2 of each token and group
+        uint8_t* const wide_values = wide_keys + Shape::kWideBytes;     // (scale * fit, low + 8 * scale)
 
+#pragma unroll 1
         for (uint32_t unit = from; unit < to; ++unit) {
-            const uint32_t stage = (unit - from) % kStages;
-            {
-                const uint32_t ahead = unit + kStages - 1;
-                __syncwarp();  // every lane is done with the stage that is filled next
-                if (ahead < to) issue(ahead, (ahead - from) % kStages);
-                copy_async_commit();
-                copy_async_wait<kStages - 1>();
-                __syncwarp();
+            __syncwarp();  // every lane is done with the stage that is filled next, and with the wide parameters
+            if (unit + kStages - 1 < to) {
+                issue(next);
+                next = locate(unit + kStages);
             }
-            const uint8_t* const keys = own + stage * Shape::kStageBytes;
+            copy_async_commit();
+            copy_async_wait<kStages - 1>();
+            mbar_wait(barriers + 8 * use_stage, use_parity, site, kStallCodes, unit);
+            __syncwarp();
+            const uint8_t* const keys = own + use_stage * Shape::kStageBytes;
             const uint8_t* const values = keys + Shape::kCodeBytes;
             const uint8_t* const key_params = keys + 2 * Shape::kCodeBytes;
             const uint8_t* const value_params = key_params + Shape::kParamBytes;
             const int32_t* const tokens = reinterpret_cast<const int32_t*>(value_params + Shape::kParamBytes);
+            const bool is_masked = masked >> use_stage & 1u;
+            bool careful = false;  // some token that some row may not see has values that are not finite
 
-            // ---- scores of 32 tokens, transposed. A code in the low nibble of a half word IS the fp16 number code *
-            // 2^-24 (a subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
-            float x[2][NT][4];
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                uint32_t a[2][kKeyWords], pairs[2][kGroups];
-#pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {
-                    const uint32_t row = 16 * h + 8 * half + own_token;
-                    load_words(a[half], keys + row * (D / 2) + c4 * (D / 8));
-                    load_words(pairs[half], key_params + row * (kGroups * 4));
-                }
+            // ---- parameters as floats, lane = token, and the power of two that lets weight * scale fit fp16 with its
+            // largest at 2^14, whatever the scales' size; what was summed so far follows when it changes.
+            {
+                uint32_t pairs[kGroups];
+                float scales[kGroups], widest = 0.0f;
+                load_words(pairs, value_params + lane * (kGroups * 4));
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g) {
-                    float part[NT][4] = {};
+                    scales[g] = E::low(pairs[g]);
+                    widest = fmaxf(widest, fabsf(scales[g]));
+                }
+                if (is_masked) {
+                    bool finite = true;
 #pragma unroll
-                    for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w) {
-                        const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
+                    for (uint32_t g = 0; g < kGroups; ++g)
+                        finite = finite && fabsf(scales[g]) < INFINITY && fabsf(E::high(pairs[g])) < INFINITY;
+                    careful = !__all_sync(0xffffffffu, finite);
+                }
+                uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(widest));
+                if (bits >= 0x7f800000u) {  // an infinity says nothing about the others
+                    widest = 0.0f;
 #pragma unroll
-                        for (uint32_t n = 0; n < NT; ++n) {
-                            mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
-                                        a[1][w] & 0x00f000f0u, qf[n][2 * w][0], qf[n][2 * w][1]);
-                            mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u,
-                                        qf[n][2 * w + 1][0], qf[n][2 * w + 1][1]);
-                        }
-                    }
+                    for (uint32_t g = 0; g < kGroups; ++g)
+                        if (fabsf(scales[g]) < INFINITY) widest = fmaxf(widest, fabsf(scales[g]));
+                    bits = __reduce_max_sync(0xffffffffu, __float_as_uint(widest));
+                }
+                const int32_t unit_top = static_cast<int32_t>(bits >> 23);
+                if (unit_top > top) {
+                    const float shrink = power_of_two(max(127 + min(267 - unit_top, 254) - min(267 - top, 254), 0));
+                    top = unit_top;
+                    fit = power_of_two(min(267 - top, 254));
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i) {
-                            const float rest = g == 0 ? E::high(pairs[i / 2][g]) * q_sum[n][g][i % 2]
-                                                      : fmaf(E::high(pairs[i / 2][g]), q_sum[n][g][i % 2], x[h][n][i]);
-                            x[h][n][i] = fmaf(E::low(pairs[i / 2][g]), part[n][i], rest);
+#pragma unroll
+                            for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= shrink;
+                            if constexpr (kEights) {
+#pragma unroll
+                                for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= shrink;
+                            }
                         }
                 }
+                float2 wide[kGroups];
+#pragma unroll
+                for (uint32_t g = 0; g < kGroups; ++g)
+                    wide[g] = make_float2(scales[g] * fit, fmaf(8.0f, scales[g], E::high(pairs[g])));
+                store_floats(wide_values + lane * (kGroups * 8), wide);
+                load_words(pairs, key_params + lane * (kGroups * 4));
+#pragma unroll
+                for (uint32_t g = 0; g < kGroups; ++g) wide[g] = make_float2(E::low(pairs[g]) * to_log2, E::high(pairs[g]) * to_log2);
+                store_floats(wide_keys + lane * (kGroups * 8), wide);
             }
-            if (masked >> stage & 1u) {
+            __syncwarp();
+
+#pragma unroll
+            for (uint32_t round = 0; round < 2 / kSteps; ++round) {
+                // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
+                // subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
+                float x[kSteps][NT][4];
+#pragma unroll
+                for (uint32_t h = 0; h < kSteps; ++h) {
+                    uint32_t a[2][kKeyWords], wide[2][2 * kGroups];
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; ++half) {
+                        const uint32_t row = 16 * (round * kSteps + h) + 8 * half + own_token;
+                        load_words(a[half], keys + row * (D / 2) + c4 * (D / 8));
+                        load_words(wide[half], wide_keys + row * (kGroups * 8));
+                    }
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        float part[NT][4] = {};
+#pragma unroll
+                        for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w) {
+                            const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
+#pragma unroll
+                            for (uint32_t n = 0; n < NT; ++n) {
+                                uint4 f;
+                                if constexpr (Shape::kSharedQueries)
+                                    f = shared_q[(n * kKeyWords + w) * 32 + lane];
+                                else
+                                    f = make_uint4(qf[2 * w][0], qf[2 * w][1], qf[2 * w + 1][0], qf[2 * w + 1][1]);
+                                mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
+                                            a[1][w] & 0x00f000f0u, f.x, f.y);
+                                mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u,
+                                            y1 & 0x00f000f0u, f.z, f.w);
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n) {
+                            float2 sums;
+                            if constexpr (Shape::kSharedQueries)
+                                sums = *reinterpret_cast<const float2*>(shared_sums + g * kRows + 8 * n + 2 * c4);
+                            else
+                                sums = make_float2(q_sum[g][0], q_sum[g][1]);
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) {
+                                const float scale = __uint_as_float(wide[i / 2][2 * g]);
+                                const float low = __uint_as_float(wide[i / 2][2 * g + 1]);
+                                const float s = i % 2 ? sums.y : sums.x;
+                                const float rest = g == 0 ? low * s : fmaf(low, s, x[h][n][i]);
+                                x[h][n][i] = fmaf(scale, part[n][i], rest);
+                            }
+                        }
+                    }
+                }
+                if (is_masked) {
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                        for (uint32_t e = 0; e < 2; ++e) {
+                            const uint32_t t = args.ratio.quotient(min(first_row + 8 * n + 2 * c4 + e, args.rows - 1));
+                            const int32_t i = extent.length - static_cast<int32_t>(args.queries) + static_cast<int32_t>(t);
+#pragma unroll
+                            for (uint32_t h = 0; h < kSteps; ++h)
+#pragma unroll
+                                for (uint32_t half = 0; half < 2; ++half) {
+                                    const int32_t j = tokens[16 * (round * kSteps + h) + 8 * half + own_token];
+                                    const bool seen = j <= i && (!args.window || j > i - args.window || j < args.sinks);
+                                    if (!seen) x[h][n][2 * half + e] = -INFINITY;
+                                }
+                        }
+                }
+
+                // ---- the running maximum of each row; sums are rescaled only when one grows.
+                float higher[NT][2];
+                bool grows = false;
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) {
-                        const uint32_t t = args.ratio.quotient(min(first_row + 8 * n + 2 * c4 + e, args.rows - 1));
-                        const int32_t i = extent.length - static_cast<int32_t>(args.queries) + static_cast<int32_t>(t);
+                        float m = fmaxf(x[0][n][e], x[0][n][2 + e]);
+                        if constexpr (kSteps == 2) m = fmaxf(m, fmaxf(x[1][n][e], x[1][n][2 + e]));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                        higher[n][e] = m;
+                        grows |= m > peak[n][e];
+                    }
+                if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h)
+                    for (uint32_t n = 0; n < NT; ++n) {
+                        float keep[2];
 #pragma unroll
-                            for (uint32_t half = 0; half < 2; ++half) {
-                                const int32_t j = tokens[16 * h + 8 * half + own_token];
-                                const bool seen = j <= i && (!args.window || j > i - args.window || j < args.sinks);
-                                if (!seen) x[h][n][2 * half + e] = -INFINITY;
+                        for (uint32_t e = 0; e < 2; ++e) {
+                            keep[e] = 1.0f;
+                            if (higher[n][e] > peak[n][e]) {
+                                keep[e] = ex2_approx(peak[n][e] - higher[n][e]);
+                                peak[n][e] = higher[n][e];
                             }
-                    }
-            }
-
-            // ---- the running maximum of each row, and of the value scales' exponents; what was summed so far is
-            // rescaled only when one of them grows.
-            uint32_t scale_pairs[2][2][kGroups];
-            uint32_t widest = 0;
+                            sum[n][e] *= keep[e];
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                for (uint32_t half = 0; half < 2; ++half) {
-                    load_words(scale_pairs[h][half], value_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) {
-                        const uint32_t bits = scale_pairs[h][half][g] & 0x7fffu;
-                        widest = max(widest, bits < (BF16 ? 0x7f80u : 0x7c00u) ? bits : 0u);
-                    }
-                }
-            widest = __reduce_max_sync(0xffffffffu, widest);
-            const int32_t unit_top = static_cast<int32_t>(__float_as_uint(E::low(widest)) >> 23);
-            float higher[NT][2];
-            bool grows = unit_top > top;
-#pragma unroll
-            for (uint32_t n = 0; n < NT; ++n)
-#pragma unroll
-                for (uint32_t e = 0; e < 2; ++e) {
-                    float m = fmaxf(fmaxf(x[0][n][e], x[0][n][2 + e]), fmaxf(x[1][n][e], x[1][n][2 + e]));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    higher[n][e] = fmaxf(m, peak[n][e]);
-                    grows |= higher[n][e] > peak[n][e];
-                }
-            if (__any_sync(0xffffffffu, grows)) {
-                const int32_t new_top = max(top, unit_top);
-                const float shrink = power_of_two(max(127 + top - new_top, 0));
-                top = new_top;
-#pragma unroll
-                for (uint32_t n = 0; n < NT; ++n) {
-                    float keep[2];
-#pragma unroll
-                    for (uint32_t e = 0; e < 2; ++e) {
-                        keep[e] = higher[n][e] > peak[n][e] ? ex2_approx((peak[n][e] - higher[n][e]) * to_log2[n][e]) : 1.0f;
-                        peak[n][e] = higher[n][e];
-                        sum[n][e] *= keep[e];
-#pragma unroll
-                        for (uint32_t g = 0; g < kGroups; ++g) lows[g][n][e] *= keep[e];
-                        keep[e] *= shrink;
-                    }
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-#pragma unroll
-                        for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= keep[i % 2];
-#pragma unroll
-                        for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= keep[i % 2];
-                    }
-                }
-            }
-            // Weights times scales fit fp16 with their largest at 2^14 whatever the scales' size.
-            const float fit = power_of_two(min(267 - top, 254));
-
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                // ---- weights, their sums, and weight * scale in fp16, turned to be the values' second operand.
-                uint32_t weights[kGroups][NT][2];
-#pragma unroll
-                for (uint32_t n = 0; n < NT; ++n) {
-                    float p[4];
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const float base = peak[n][i % 2] == -INFINITY ? 0.0f : peak[n][i % 2] * to_log2[n][i % 2];
-                        p[i] = ex2_approx(fmaf(x[h][n][i], to_log2[n][i % 2], -base));
-                        sum[n][i % 2] += p[i];
-                    }
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) {
-                        float weight[4];
+                            for (uint32_t g = 0; g < kGroups; ++g) lows[g][n][e] *= keep[e];
+                        }
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i) {
-                            const uint32_t pair = scale_pairs[h][i / 2][g];
-                            const float scale = E::low(pair);
-                            // A token that is not seen may carry NaN.
-                            const bool seen = x[h][n][i] != -INFINITY;
-                            lows[g][n][i % 2] += seen ? p[i] * fmaf(8.0f, scale, E::high(pair)) : 0.0f;
-                            weight[i] = seen ? p[i] * (scale * fit) : 0.0f;
+#pragma unroll
+                            for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= keep[i % 2];
+                            if constexpr (kEights) {
+#pragma unroll
+                                for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= keep[i % 2];
+                            }
                         }
-                        weights[g][n][0] = transpose_8x8(Element<false>::pack(weight[0], weight[1]));
-                        weights[g][n][1] = transpose_8x8(Element<false>::pack(weight[2], weight[3]));
                     }
                 }
-                // ---- O^T += V^T . (P scale)^T. Two tokens' nibbles of a channel side by side are a pair of the first
-                // operand; the odd fragment rows' channels come 16 times too large. `eights` sums 8 * weight as rounded:
-                // codes count from their middle, and the rest, in fp32, is in `lows`.
+
 #pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g)
+                for (uint32_t h = 0; h < kSteps; ++h) {
+                    // ---- weights, their sums, and weight * scale in fp16, turned to be the values' second operand.
+                    const uint32_t first_token = 16 * (round * kSteps + h);
+                    uint32_t wide[2][2 * kGroups];
 #pragma unroll
-                    for (uint32_t n = 0; n < NT; ++n)
-                        mma_16x8x16(eights[g][n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, weights[g][n][0],
-                                    weights[g][n][1]);
-                uint32_t v[4][kValueWords];
+                    for (uint32_t half = 0; half < 2; ++half)
+                        load_words(wide[half], wide_values + (first_token + 8 * half + own_token) * (kGroups * 8));
+                    uint32_t weights[kGroups][NT][2];
+                    const auto weigh = [&](auto guarded) {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-                    load_words(v[i], values + (16 * h + 4 * i + c4) * (D / 2) + l4 * (D / 16));
+                        for (uint32_t n = 0; n < NT; ++n) {
+                            float p[4];
 #pragma unroll
-                for (uint32_t w = 0; w < kValueWords; ++w)
+                            for (uint32_t i = 0; i < 4; ++i) {
+                                // A row that has seen nothing has a peak of -inf, and so have its scores.
+                                p[i] = ex2_approx(x[h][n][i] - (peak[n][i % 2] == -INFINITY ? 0.0f : peak[n][i % 2]));
+                                sum[n][i % 2] += p[i];
+                            }
 #pragma unroll
-                    for (uint32_t half = 0; half < 2; ++half) {
-                        uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
-                        uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+                            for (uint32_t g = 0; g < kGroups; ++g) {
+                                float weight[4];
 #pragma unroll
-                        for (uint32_t byte = 0; byte < 2; ++byte) {
-                            const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
+                                for (uint32_t i = 0; i < 4; ++i) {
+                                    const float scale = __uint_as_float(wide[i / 2][2 * g]);
+                                    const float low = __uint_as_float(wide[i / 2][2 * g + 1]);
+                                    const bool seen = !decltype(guarded)::value || x[h][n][i] != -INFINITY;
+                                    lows[g][n][i % 2] = fmaf(p[i], seen ? low : 0.0f, lows[g][n][i % 2]);
+                                    weight[i] = p[i] * (seen ? scale : 0.0f);
+                                }
+                                const uint32_t packed[2] = {Element<false>::pack(weight[0], weight[1]),
+                                                            Element<false>::pack(weight[2], weight[3])};
+                                weights[g][n][0] = transpose_8x8(packed[0]);
+                                weights[g][n][1] = transpose_8x8(packed[1]);
+                            }
+                        }
+                    };
+                    if (careful)
+                        weigh(std::true_type{});
+                    else
+                        weigh(std::false_type{});
+                    // ---- O^T += V^T . (P scale)^T. Two tokens' nibbles of a channel side by side are a pair of the first
+                    // operand; the odd fragment rows' channels come 16 times too large. Codes count from their middle, 8,
+                    // with 8 * weight in fp32 in `lows`. For one row tile `eights`, a product with a constant, sums 8 * weight
+                    // as rounded, to be taken off at the end; for more, whose registers are full, the codes are made normal
+                    // numbers and 8 is subtracted from them.
+                    if constexpr (kEights) {
+#pragma unroll
+                        for (uint32_t g = 0; g < kGroups; ++g)
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n)
-                                mma_16x8x16(out[j][n], lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u,
+                                mma_16x8x16(eights[g][n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u,
                                             weights[g][n][0], weights[g][n][1]);
-                            lo >>= 8;
-                            hi >>= 8;
-                        }
                     }
+                    uint32_t v[4][kValueWords];
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        load_words(v[i], values + (first_token + 4 * i + c4) * (D / 2) + l4 * (D / 16));
+#pragma unroll
+                    for (uint32_t w = 0; w < kValueWords; ++w)
+#pragma unroll
+                        for (uint32_t half = 0; half < 2; ++half) {
+                            uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
+                            uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                            for (uint32_t byte = 0; byte < 2; ++byte) {
+                                const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
+                                uint32_t codes[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+                                if constexpr (!kEights) {
+                                    codes[0] = add_f16x2(codes[0] | 0x64006400u, 0xe408e408u);  // 1024 + code - 1032
+                                    codes[1] = add_f16x2(codes[1] | 0x64006400u, 0xe480e480u);  // 1024 + 16 code - 1152
+                                    codes[2] = add_f16x2(codes[2] | 0x64006400u, 0xe408e408u);
+                                    codes[3] = add_f16x2(codes[3] | 0x64006400u, 0xe480e480u);
+                                }
+#pragma unroll
+                                for (uint32_t n = 0; n < NT; ++n)
+                                    mma_16x8x16(out[j][n], codes[0], codes[1], codes[2], codes[3], weights[g][n][0], weights[g][n][1]);
+                                lo >>= 8;
+                                hi >>= 8;
+                            }
+                        }
+                }
             }
+            use_stage = use_stage == kStages - 1 ? 0 : use_stage + 1;
+            use_parity ^= use_stage == 0;
         }
 
         // ---- the warps' parts of the piece, through shared memory
         copy_async_wait<0>();
-        __syncthreads();
+        __syncwarp();
         {
             float* const merged = reinterpret_cast<float*>(own);
             float* const stats = merged + kRows * kPitch;
@@ -820,12 +958,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
 #pragma unroll
                     for (uint32_t j = 0; j < kTiles; ++j) {
                         const uint32_t g = 16 * j / G;
-                        merged[row * kPitch + 16 * j + l4] = fmaf((out[j][n][e] - eights[g][n][e]) * 0x1p24f, unfit, low[g]);
-                        merged[row * kPitch + 16 * j + 8 + l4] =
-                            fmaf((out[j][n][2 + e] * 0.0625f - eights[g][n][e]) * 0x1p24f, unfit, low[g]);
+                        float y = out[j][n][e], odd_y = out[j][n][2 + e] * 0.0625f;
+                        if constexpr (kEights) {
+                            y = (y - eights[g][n][e]) * 0x1p24f;
+                            odd_y = (odd_y - eights[g][n][e]) * 0x1p24f;
+                        }
+                        merged[row * kPitch + 16 * j + l4] = fmaf(y, unfit, low[g]);
+                        merged[row * kPitch + 16 * j + 8 + l4] = fmaf(odd_y, unfit, low[g]);
                     }
                     if (l4 == 0) {
-                        stats[2 * row] = peak[n][e] == -INFINITY ? -INFINITY : peak[n][e] * to_log2[n][e];
+                        stats[2 * row] = peak[n][e];
                         stats[2 * row + 1] = s;
                     }
                 }
@@ -833,9 +975,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         __syncthreads();
         const uint32_t rows_here = min(kRows, args.rows - first_row);
         const bool whole = from == 0 && to == units;
-        const uint32_t segment_first = at - from;
-        // A segment cut over blocks: the block it begins in keeps its part in its second place, the others in their first.
-        const uint32_t owner = whole ? 0 : block_of(segment_first);
+        // A segment cut over blocks: the block its first unit lies in keeps its part in its second place, the others in
+        // their first.
+        const uint32_t owner = whole ? 0 : block_of(segment_at);
         float* const part = args.partials + (2 * blockIdx.x + (owner == blockIdx.x ? 1 : 0)) * static_cast<size_t>(kPartialFloats);
         const auto finish = [&](uint32_t row, uint32_t d, float y, float s, float m) {
             const uint32_t r = first_row + row, t = args.ratio.quotient(r);
@@ -846,15 +988,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         };
         for (uint32_t i = threadIdx.x; i < rows_here * D; i += blockDim.x) {
             const uint32_t row = i / D, d = i % D;
+            const uint8_t* const theirs = shared + Shape::kQueryBytes;
             float m = -INFINITY, y = 0.0f, s = 0.0f;
             for (uint32_t w = 0; w < warps; ++w)
-                m = fmaxf(m, reinterpret_cast<const float*>(shared + w * Shape::kWarpBytes)[kRows * kPitch + 2 * row]);
+                m = fmaxf(m, reinterpret_cast<const float*>(theirs + w * Shape::kWarpBytes)[kRows * kPitch + 2 * row]);
             for (uint32_t w = 0; w < warps; ++w) {
-                const float* const theirs = reinterpret_cast<const float*>(shared + w * Shape::kWarpBytes);
-                const float its_peak = theirs[kRows * kPitch + 2 * row];
+                const float* const its = reinterpret_cast<const float*>(theirs + w * Shape::kWarpBytes);
+                const float its_peak = its[kRows * kPitch + 2 * row];
                 const float share = its_peak == -INFINITY ? 0.0f : ex2_approx(its_peak - m);
-                y = fmaf(theirs[row * kPitch + d], share, y);
-                s = fmaf(theirs[kRows * kPitch + 2 * row + 1], share, s);
+                y = fmaf(its[row * kPitch + d], share, y);
+                s = fmaf(its[kRows * kPitch + 2 * row + 1], share, s);
             }
             if (whole) {
                 finish(row, d, y, s, m);
@@ -868,16 +1011,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         }
         if (!whole) {
             // The block that comes last adds the parts up, always in the same order.
-            const uint32_t parts = block_of(segment_first + units - 1) - owner + 1;
+            const uint32_t parts = block_of(segment_at + units - 1) - owner + 1;
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
                 const uint32_t came = atomicAdd(args.arrivals + owner, 1u);
                 if (came == parts - 1) args.arrivals[owner] = 0;
-                scan[0] = came == parts - 1;
+                last_to_come = came == parts - 1;
             }
             __syncthreads();
-            if (scan[0]) {
+            if (last_to_come) {
                 __threadfence();
                 const float* const base = args.partials + 2 * owner * static_cast<size_t>(kPartialFloats);
                 for (uint32_t i = threadIdx.x; i < rows_here * D; i += blockDim.x) {
@@ -897,17 +1040,25 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 }
             }
         }
-        __syncthreads();  // the merged rows lie where the rings are
+        // The merged rows lie where the rings are: they are read before the next copies, which come by another way.
+        fence_proxy_async_shared();
+        __syncthreads();
+        }
 
-        at += to - from;
-        from = 0;
-        if (to == units && ++segment == segments && at < end) {
+        at += length;
+        offset = 0;
+        if (at < end && ++segment == segments) {
             segment = 0;
             ++b;
             extent = extent_of(args, b, nullptr);
-            units = units_of(extent);
+            cost = cost_of(extent);
         }
     }
+    // After a wait that gave up, copies may still be on their way: give them a while before the block's memory goes.
+    if (stop_flag)
+        for (uint32_t s = 0; s < kStages; ++s)
+            for (uint32_t i = 0; i < 1000 && !mbar_try_wait(barriers + 8 * s, use_parity ^ (s < use_stage)); ++i) {
+            }
 }
 
 }  // namespace cache
@@ -1047,7 +1198,7 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     using Shape = cache::AttentionShape<D, G, NT>;
     const auto kernel = cache::attention_kernel<D, G, NT, BF16>;
     uint32_t limit = 0;
-    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::kMostWarps * Shape::kWarpBytes, &limit);
+    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(Shape::kMostWarps), &limit);
     if (admitted != FK_OK) return admitted;
     args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
@@ -1055,13 +1206,14 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     const uint32_t warps = segments >= 2ull * facts.sm_count ? small : Shape::kMostWarps;
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (warps == small ? Shape::kMostWarps / small : 1);
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
-    const uint64_t most_units = segments * ((static_cast<uint64_t>(args.table_pages) * args.page_size + unit_tokens - 1) / unit_tokens);
+    args.least_units = 1;
+    args.segment_cost = 1;
+    const uint64_t most_units = segments * ((static_cast<uint64_t>(args.table_pages) * args.page_size + unit_tokens - 1) / unit_tokens + args.segment_cost);
     if (most_units >= (1ull << 31))
         return fk_fail(FK_ERR_SHAPE, "%u sequences of up to %llu tokens on %u heads are more than a launch counts", args.batch,
                        static_cast<unsigned long long>(args.table_pages) * args.page_size, args.kv_heads);
-    args.least_units = 1;
     const uint32_t grid = most_units < resident ? static_cast<uint32_t>(most_units) : resident;
-    kernel<<<grid, warps * 32, warps * Shape::kWarpBytes, static_cast<cudaStream_t>(stream)>>>(args, device_status);
+    kernel<<<grid, warps * 32, Shape::shared_bytes(warps), static_cast<cudaStream_t>(stream)>>>(args, device_status);
     FK_CUDA(cudaGetLastError());
     return FK_OK;
 }
