@@ -323,6 +323,12 @@ constexpr uint32_t kMostBlocksPerSm = 4;
 constexpr uint32_t kMostRows = 32;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
 constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
+/// How far (in powers of two) a score may lie above its row's reference before the reference is moved. Weights reach
+/// 2^kSlack, so weight * scale, in fp16, has the largest scale at 2^kFit: 2^15 at most, and under 2^-14 (where fp16 loses
+/// bits) only weights 2^-21 of the reference's.
+constexpr float kSlack = 8.0f;
+constexpr int32_t kFit = 6;
+constexpr int32_t kFitBiased = 254 + kFit;  // less a scale's biased exponent: that of the power that brings it to 2^kFit
 constexpr uint32_t kStallCodes = 0x504;  // a warp waiting for a stage of codes
 
 template <int D, int G, int NT>
@@ -447,6 +453,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     constexpr bool kEights = NT == 1;                 // see `eights` below
     extern __shared__ __align__(16) uint8_t shared[];
     __shared__ uint32_t last_to_come, stop_flag;
+    __shared__ float2 row_stats[kRows];  // reference and sum of each row over the warps
     const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
     const uint32_t l4 = lane / 4, c4 = lane % 4;
@@ -461,24 +468,23 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     const auto cost_of = [&](const Extent& e) {
         return max((static_cast<uint32_t>(e.visible()) + unit_tokens - 1) / unit_tokens, 1u) + args.segment_cost;
     };
-    uint32_t total = 0;
-    for (uint32_t i = lane; i < args.batch; i += 32) total += cost_of(extent_of(args, i, status));
+    uint32_t mine = lane < args.batch ? cost_of(extent_of(args, lane, status)) : 0, total = mine;
+    for (uint32_t i = lane + 32; i < args.batch; i += 32) total += cost_of(extent_of(args, i, status));
     total = __reduce_add_sync(0xffffffffu, total) * segments;
     const uint32_t blocks = min(gridDim.x, max(total / args.least_units, 1u));
     if (blockIdx.x >= blocks) return;
-    const auto first_of = [&](uint32_t block) {
-        return static_cast<uint32_t>(static_cast<uint64_t>(block) * total / blocks);
-    };
+    // The first `longer` blocks take a unit more than the others.
+    const uint32_t share = total / blocks, longer = total - share * blocks;
     const auto block_of = [&](uint32_t place) {
-        return static_cast<uint32_t>(((static_cast<uint64_t>(place) + 1) * blocks - 1) / total);
+        const uint32_t behind = longer * (share + 1);
+        return place < behind ? place / (share + 1) : longer + (place - behind) / share;
     };
-    uint32_t at = first_of(blockIdx.x);
-    const uint32_t end = first_of(blockIdx.x + 1);
+    uint32_t at = blockIdx.x * share + min(blockIdx.x, longer);
+    const uint32_t end = at + share + (blockIdx.x < longer ? 1 : 0);
     uint32_t b = 0, before = 0;
     for (uint32_t chunk = 0;; chunk += 32) {
-        const uint32_t i = chunk + lane;
-        const uint32_t cost = i < args.batch ? cost_of(extent_of(args, i, nullptr)) * segments : 0;
-        uint32_t sum = cost;
+        if (chunk) mine = chunk + lane < args.batch ? cost_of(extent_of(args, chunk + lane, nullptr)) : 0;
+        uint32_t sum = mine * segments;
 #pragma unroll
         for (uint32_t d = 1; d < 32; d *= 2) {
             const uint32_t other = __shfl_up_sync(0xffffffffu, sum, d);
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         if (past) {
             const uint32_t found = __ffs(past) - 1;
             b = chunk + found;
-            before += __shfl_sync(0xffffffffu, sum - cost, found);
+            before += __shfl_sync(0xffffffffu, sum - mine * segments, found);
             break;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
@@ -558,12 +564,15 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             const uint32_t params_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
             copy_async_params<kGroups * 4>(params_at, args.params[0] + params, p.row >= 0);
             copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, p.row >= 0);
-            // A place that holds no token lies behind every query.
-            reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
-                p.row >= 0 ? p.token : 0x7fffffff;
-            const bool partly = p.row < 0 || p.token > extent.first ||
-                                (args.window && p.token >= args.sinks && p.token <= extent.length - 1 - args.window);
-            masked = (masked & ~(1u << fill_stage)) | (__any_sync(0xffffffffu, partly) ? 1u << fill_stage : 0u);
+            // Tokens rise from lane to lane. A place that holds none lies behind every query.
+            const int32_t last = __shfl_sync(0xffffffffu, p.token, 31);
+            masked &= ~(1u << fill_stage);
+            if (real != 0xffffffffu || last > extent.first ||
+                (args.window && last >= args.sinks && __shfl_sync(0xffffffffu, p.token, 0) <= extent.length - 1 - args.window)) {
+                masked |= 1u << fill_stage;
+                reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
+                    p.row >= 0 ? p.token : 0x7fffffff;
+            }
             fill_stage = fill_stage == kStages - 1 ? 0 : fill_stage + 1;
         };
         Place next = locate(from);
@@ -680,8 +689,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             const bool is_masked = masked >> use_stage & 1u;
             bool careful = false;  // some token that some row may not see has values that are not finite
 
-            // ---- parameters as floats, lane = token, and the power of two that lets weight * scale fit fp16 with its
-            // largest at 2^14, whatever the scales' size; what was summed so far follows when it changes.
+            // ---- parameters as floats, lane = token, and the power of two that lets weight * scale fit fp16 whatever the
+            // scales' size; what was summed so far follows when it changes.
             {
                 uint32_t pairs[kGroups];
                 float scales[kGroups], widest = 0.0f;
@@ -708,9 +717,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 }
                 const int32_t unit_top = static_cast<int32_t>(bits >> 23);
                 if (unit_top > top) {
-                    const float shrink = power_of_two(max(127 + min(267 - unit_top, 254) - min(267 - top, 254), 0));
+                    const float shrink = power_of_two(max(127 + min(kFitBiased - unit_top, 254) - min(kFitBiased - top, 254), 0));
                     top = unit_top;
-                    fit = power_of_two(min(267 - top, 254));
+                    fit = power_of_two(min(kFitBiased - top, 254));
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
@@ -804,8 +813,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                         }
                 }
 
-                // ---- the running maximum of each row; sums are rescaled only when one grows.
-                float higher[NT][2];
+                // ---- the reference of each row's exponentials: its largest score when it was last set, and set again only
+                // when some score lies more than kSlack above it, so that a weight stays under 2^kSlack.
+                float largest[NT][2];
                 bool grows = false;
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
@@ -813,11 +823,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                     for (uint32_t e = 0; e < 2; ++e) {
                         float m = fmaxf(x[0][n][e], x[0][n][2 + e]);
                         if constexpr (kSteps == 2) m = fmaxf(m, fmaxf(x[1][n][e], x[1][n][2 + e]));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                        higher[n][e] = m;
-                        grows |= m > peak[n][e];
+                        largest[n][e] = m;
+                        grows |= m > peak[n][e] + kSlack;
                     }
                 if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -825,10 +832,14 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                         float keep[2];
 #pragma unroll
                         for (uint32_t e = 0; e < 2; ++e) {
+                            float m = largest[n][e];
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                             keep[e] = 1.0f;
-                            if (higher[n][e] > peak[n][e]) {
-                                keep[e] = ex2_approx(peak[n][e] - higher[n][e]);
-                                peak[n][e] = higher[n][e];
+                            if (m > peak[n][e]) {
+                                keep[e] = ex2_approx(peak[n][e] - m);
+                                peak[n][e] = m;
                             }
                             sum[n][e] *= keep[e];
 #pragma unroll
@@ -939,7 +950,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         {
             float* const merged = reinterpret_cast<float*>(own);
             float* const stats = merged + kRows * kPitch;
-            const float unfit = power_of_two(254 - min(267 - top, 254));
+            const float unfit = power_of_two(254 - min(kFitBiased - top, 254));
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
@@ -975,68 +986,102 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         __syncthreads();
         const uint32_t rows_here = min(kRows, args.rows - first_row);
         const bool whole = from == 0 && to == units;
+        const uint8_t* const rings = shared + Shape::kQueryBytes;
+        // A warp for each row: the warps' shares of it, left in the place of their references.
+        for (uint32_t row = warp; row < rows_here; row += warps) {
+            float2* const its = reinterpret_cast<float2*>(const_cast<uint8_t*>(rings) + min(lane, warps - 1) * Shape::kWarpBytes +
+                                                          kRows * kPitch * 4) + row;
+            const float2 stat = lane < warps ? *its : make_float2(-INFINITY, 0.0f);
+            float m = stat.x;
+#pragma unroll
+            for (uint32_t mask = 16; mask > 0; mask >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, mask));
+            const float factor = stat.x == -INFINITY ? 0.0f : ex2_approx(stat.x - m);
+            float s = stat.y * factor;
+#pragma unroll
+            for (uint32_t mask = 16; mask > 0; mask >>= 1) s += __shfl_xor_sync(0xffffffffu, s, mask);
+            if (lane < warps) its->x = factor;
+            if (lane == 0) {
+                row_stats[row] = make_float2(m, s);
+            }
+        }
+        __syncthreads();
         // A segment cut over blocks: the block its first unit lies in keeps its part in its second place, the others in
         // their first.
         const uint32_t owner = whole ? 0 : block_of(segment_at);
         float* const part = args.partials + (2 * blockIdx.x + (owner == blockIdx.x ? 1 : 0)) * static_cast<size_t>(kPartialFloats);
-        const auto finish = [&](uint32_t row, uint32_t d, float y, float s, float m) {
+        const auto finish = [&](uint32_t row, uint32_t d, float4 y, float2 stat) {
             const uint32_t r = first_row + row, t = args.ratio.quotient(r);
             const uint64_t place = (static_cast<uint64_t>(b) * args.queries + t) * args.heads + kv_head * args.ratio.divisor +
                                    (r - t * args.ratio.divisor);
-            args.out[place * D + d] = static_cast<uint16_t>(E::pack(s == 0.0f ? 0.0f : __fdividef(y, s), 0.0f));
-            if (d == 0 && args.lse) args.lse[place] = s == 0.0f ? -INFINITY : (m + log2f(s)) * 0.6931471805599453f;
+            const float inverse = stat.y == 0.0f ? 0.0f : __fdividef(1.0f, stat.y);
+            if (stat.y == 0.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            *reinterpret_cast<uint2*>(args.out + place * D + d) =
+                make_uint2(E::pack(y.x * inverse, y.y * inverse), E::pack(y.z * inverse, y.w * inverse));
+            if (d == 0 && args.lse) args.lse[place] = stat.y == 0.0f ? -INFINITY : (stat.x + log2f(stat.y)) * 0.6931471805599453f;
         };
-        for (uint32_t i = threadIdx.x; i < rows_here * D; i += blockDim.x) {
-            const uint32_t row = i / D, d = i % D;
-            const uint8_t* const theirs = shared + Shape::kQueryBytes;
-            float m = -INFINITY, y = 0.0f, s = 0.0f;
-            for (uint32_t w = 0; w < warps; ++w)
-                m = fmaxf(m, reinterpret_cast<const float*>(theirs + w * Shape::kWarpBytes)[kRows * kPitch + 2 * row]);
+        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
+            const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (uint32_t w = 0; w < warps; ++w) {
-                const float* const its = reinterpret_cast<const float*>(theirs + w * Shape::kWarpBytes);
-                const float its_peak = its[kRows * kPitch + 2 * row];
-                const float share = its_peak == -INFINITY ? 0.0f : ex2_approx(its_peak - m);
-                y = fmaf(its[row * kPitch + d], share, y);
-                s = fmaf(its[kRows * kPitch + 2 * row + 1], share, s);
+                const float* const its = reinterpret_cast<const float*>(rings + w * Shape::kWarpBytes);
+                const float factor = its[kRows * kPitch + 2 * row];
+                const float4 z = *reinterpret_cast<const float4*>(its + row * kPitch + d);
+                y = make_float4(fmaf(z.x, factor, y.x), fmaf(z.y, factor, y.y), fmaf(z.z, factor, y.z), fmaf(z.w, factor, y.w));
             }
             if (whole) {
-                finish(row, d, y, s, m);
+                finish(row, d, y, row_stats[row]);
             } else {
-                part[row * D + d] = y;
-                if (d == 0) {
-                    part[kMostRows * 128 + 2 * row] = m;
-                    part[kMostRows * 128 + 2 * row + 1] = s;
-                }
+                *reinterpret_cast<float4*>(part + row * D + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
             }
         }
         if (!whole) {
             // The block that comes last adds the parts up, always in the same order.
             const uint32_t parts = block_of(segment_at + units - 1) - owner + 1;
-            __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
+                __threadfence();
                 const uint32_t came = atomicAdd(args.arrivals + owner, 1u);
                 if (came == parts - 1) args.arrivals[owner] = 0;
                 last_to_come = came == parts - 1;
+                __threadfence();
             }
             __syncthreads();
             if (last_to_come) {
-                __threadfence();
                 const float* const base = args.partials + 2 * owner * static_cast<size_t>(kPartialFloats);
-                for (uint32_t i = threadIdx.x; i < rows_here * D; i += blockDim.x) {
-                    const uint32_t row = i / D, d = i % D;
-                    const auto part_of = [&](uint32_t p) { return base + (2 * p + (p == 0)) * static_cast<size_t>(kPartialFloats); };
-                    float m = -INFINITY, y = 0.0f, s = 0.0f;
-#pragma unroll 8
-                    for (uint32_t p = 0; p < parts; ++p) m = fmaxf(m, __ldcg(part_of(p) + kMostRows * 128 + 2 * row));
-#pragma unroll 8
-                    for (uint32_t p = 0; p < parts; ++p) {
-                        const float its_peak = __ldcg(part_of(p) + kMostRows * 128 + 2 * row);
-                        const float share = its_peak == -INFINITY ? 0.0f : ex2_approx(its_peak - m);
-                        y = fmaf(__ldcg(part_of(p) + row * D + d), share, y);
-                        s = fmaf(__ldcg(part_of(p) + kMostRows * 128 + 2 * row + 1), share, s);
+                for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
+                    const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    float2 all = make_float2(-INFINITY, 0.0f);
+                    constexpr uint32_t kBatch = 4;
+                    for (uint32_t p = 0; p < parts; p += kBatch) {
+                        float4 z[kBatch];
+                        float2 stat[kBatch];
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            const uint32_t q = min(p + k, parts - 1);
+                            const float* const its = base + (2 * q + (q == 0)) * static_cast<size_t>(kPartialFloats);
+                            stat[k] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
+                            z[k] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
+                            if (p + k >= parts) stat[k] = make_float2(-INFINITY, 0.0f);
+                        }
+                        float m = all.x;
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) m = fmaxf(m, stat[k].x);
+                        const float keep = all.x == -INFINITY ? 0.0f : ex2_approx(all.x - m);
+                        y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
+                        all = make_float2(m, all.y * keep);
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            const float factor = stat[k].x == -INFINITY ? 0.0f : ex2_approx(stat[k].x - m);
+                            if (p + k < parts) {
+                                y = make_float4(fmaf(z[k].x, factor, y.x), fmaf(z[k].y, factor, y.y), fmaf(z[k].z, factor, y.z),
+                                                fmaf(z[k].w, factor, y.w));
+                                all.y = fmaf(stat[k].y, factor, all.y);
+                            }
+                        }
                     }
-                    finish(row, d, y, s, m);
+                    finish(row, d, y, all);
                 }
             }
         }
@@ -1206,7 +1251,7 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     const uint32_t warps = segments >= 2ull * facts.sm_count ? small : Shape::kMostWarps;
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (warps == small ? Shape::kMostWarps / small : 1);
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
-    args.least_units = 1;
+    args.least_units = 3;
     args.segment_cost = 1;
     const uint64_t most_units = segments * ((static_cast<uint64_t>(args.table_pages) * args.page_size + unit_tokens - 1) / unit_tokens + args.segment_cost);
     if (most_units >= (1ull << 31))
