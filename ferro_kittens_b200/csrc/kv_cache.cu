@@ -318,7 +318,7 @@ struct AttentionArguments {
 };
 
 constexpr uint32_t kWarpTokens = 32;
-constexpr uint32_t kStages = 3;
+constexpr uint32_t kStages = 2;
 constexpr uint32_t kMostBlocksPerSm = 4;
 constexpr uint32_t kMostRows = 32;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
@@ -338,18 +338,20 @@ struct AttentionShape {
     // One row tile's queries stay in registers; of more, the fragments and sums lie in shared memory.
     static constexpr bool kSharedQueries = NT > 1;
     static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 : 0;
-    // A warp's memory: a ring of stages, the unit's parameters as floats, the stages' barriers; the merge of the warps'
-    // results lies over the first two.
+    // A warp's memory: a ring of stages, the unit's parameters as floats, room for the merge of the warps' results where a
+    // stage has too little, the stages' barriers.
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
     static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
     static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes + kWarpTokens * 4;
     static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 8;
-    static constexpr uint32_t kRingBytes = kStages * kStageBytes + 2 * kWideBytes;
     static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
     static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
-    static constexpr uint32_t kBarriers = kRingBytes > kMergeBytes ? kRingBytes : kMergeBytes;
-    static constexpr uint32_t kWarpBytes = kBarriers + (kStages * 8 + 15) / 16 * 16;
-    static constexpr uint32_t kMostByRegisters = NT == 1 ? 16 : NT == 2 ? 12 : 8;  // 128, 168, 255 a thread
+    static constexpr bool kMergeInRing = kMergeBytes <= kStageBytes;
+    static constexpr uint32_t kMergeAt = kStages * kStageBytes + 2 * kWideBytes;
+    static constexpr uint32_t kBarriers = kMergeAt + (kMergeInRing ? 0 : kMergeBytes);
+    static constexpr uint32_t kWarpBytes = kBarriers + 16 * ((kStages + 1) / 2);
+    // Registers a thread: 128, 168 or 255.
+    static constexpr uint32_t kMostByRegisters = NT == 1 ? (kGroups > 2 ? 12 : 16) : NT == 2 ? 12 : 8;
     static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
     static constexpr uint32_t kMostWarps = kMostByRegisters < kMostByMemory ? kMostByRegisters : kMostByMemory;
     static constexpr uint32_t shared_bytes(uint32_t warps) { return kQueryBytes + warps * kWarpBytes; }
@@ -442,6 +444,27 @@ __device__ __forceinline__ void store_floats(void* to, const float2 (&x)[PAIRS])
     for (int i = 0; i + 1 < PAIRS; i += 2) static_cast<float4*>(to)[i / 2] = make_float4(x[i].x, x[i].y, x[i + 1].x, x[i + 1].y);
 }
 
+/// A piece of a segment (of its first row's tile), and if blocks share the segment, in how many parts and which block keeps count.
+struct Cut {
+    uint32_t b, kv_head, first_row, parts, owner;
+};
+
+/// Four channels of a row's output, and with the first its normaliser.
+template <int D, bool BF16>
+__device__ __forceinline__ void finish_row(const AttentionArguments& args, const Cut& piece, uint32_t row, uint32_t d, float4 y,
+                                           float2 stat) {
+    using E = Element<BF16>;
+    const uint32_t r = piece.first_row + row, t = args.ratio.quotient(r);
+    const uint64_t place = (static_cast<uint64_t>(piece.b) * args.queries + t) * args.heads +
+                           piece.kv_head * args.ratio.divisor + (r - t * args.ratio.divisor);
+    const bool empty = stat.y == 0.0f;
+    const float inverse = empty ? 0.0f : __fdividef(1.0f, stat.y);
+    if (empty) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    *reinterpret_cast<uint2*>(args.out + place * D + d) =
+        make_uint2(E::pack(y.x * inverse, y.y * inverse), E::pack(y.z * inverse, y.w * inverse));
+    if (d == 0 && args.lse) args.lse[place] = empty ? -INFINITY : (stat.x + log2f(stat.y)) * 0.6931471805599453f;
+}
+
 template <int D, int G, int NT, bool BF16>
 __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     attention_kernel(const __grid_constant__ AttentionArguments args, uint32_t* status) {
@@ -452,7 +475,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     constexpr uint32_t kSteps = NT == 4 ? 1 : 2;      // steps of 16 tokens between looks at the running maximum
     constexpr bool kEights = NT == 1;                 // see `eights` below
     extern __shared__ __align__(16) uint8_t shared[];
-    __shared__ uint32_t last_to_come, stop_flag;
+    __shared__ uint32_t stop_flag, complete[2];
+    __shared__ Cut cuts[2];              // the parts of segments that are cut over blocks: the one this share begins in, ends in
     __shared__ float2 row_stats[kRows];  // reference and sum of each row over the warps
     const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
@@ -503,7 +527,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
 
     if (lane == 0)
         for (uint32_t s = 0; s < kStages; ++s) mbar_init(barriers + 8 * s, 1);
-    if (threadIdx.x == 0) stop_flag = 0;
+    if (threadIdx.x == 0) stop_flag = cuts[0].parts = cuts[1].parts = 0;
     fence_mbarrier_init();
     __syncthreads();
     const StallSite site{status, &stop_flag, 0};
@@ -513,78 +537,99 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     uint32_t segment = (at - before) / cost;
     uint32_t offset = (at - before) - segment * cost;  // of `at` in its segment
     uint32_t fill_stage = 0, use_stage = 0, use_parity = 0;
-
-    while (at < end) {
-        const uint32_t length = min(cost - offset, end - at);  // of the share that lies in this segment
-        const uint32_t units = cost - args.segment_cost;
-        const uint32_t from = offset > args.segment_cost ? offset - args.segment_cost : 0;
-        const uint32_t to = offset + length > args.segment_cost ? offset + length - args.segment_cost : 0;
-        const uint32_t segment_at = at - offset + args.segment_cost;  // the place of its first unit
-        if (from < to) {
-        const uint32_t kv_head = segment / args.row_tiles, first_row = (segment % args.row_tiles) * kRows;
-
-        // ---- copies: each warp keeps a ring of its own, 32 tokens a stage, lane = token. Tokens that follow each other
-        // in the cache are copied as one run of each code matrix by the lane of the run's first token; parameters come
-        // lane by lane (their rows are too short for bulk copies) as zeros where there is no token. The rows are looked up
-        // one unit ahead of their copies.
-        uint32_t masked = 0;  // bit s: some row may not see some token of stage s
-        struct Place {
-            int32_t row, token;  // row -1: nothing to read
-        };
-        const auto locate = [&](uint32_t unit) {
-            const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens + lane);
-            Place p{-1, extent.token(place)};
-            if (place < extent.visible()) {
-                const uint32_t entry = args.page.quotient(static_cast<uint32_t>(p.token));
-                const uint32_t page =
-                    args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + entry)) : b;
-                if (page < args.pages)
-                    p.row = static_cast<int32_t>((page * args.kv_heads + kv_head) * args.page_size +
-                                                 (static_cast<uint32_t>(p.token) - entry * args.page_size));
-                else
-                    note(status, kBadPage, b, page);
+    uint32_t masked = 0;  // bit s: some row may not see some token of stage s
+    // The piece at hand: units [from, to) of the segment (b, kv_head, rows from first_row).
+    uint32_t length = 0, from = 0, to = 0, kv_head = 0, first_row = 0;
+    const auto units_of = [&](uint32_t its_cost) { return its_cost - args.segment_cost; };
+    const auto find_piece = [&]() {
+        while (at < end) {
+            length = min(cost - offset, end - at);  // of the share that lies in this segment
+            from = offset > args.segment_cost ? offset - args.segment_cost : 0;
+            to = offset + length > args.segment_cost ? offset + length - args.segment_cost : 0;
+            if (from < to) {
+                kv_head = segment / args.row_tiles;
+                first_row = (segment - kv_head * args.row_tiles) * kRows;
+                return true;
             }
-            return p;
-        };
-        const auto issue = [&](const Place& p) {
-            uint8_t* const stage = own + fill_stage * Shape::kStageBytes;
-            const uint32_t stage_at = smem_u32(stage), bar = barriers + 8 * fill_stage;
-            const int32_t ahead = __shfl_up_sync(0xffffffffu, p.row, 1);
-            const bool begins = p.row >= 0 && (lane == 0 || ahead < 0 || ahead + 1 != p.row);
-            const uint32_t begin = __ballot_sync(0xffffffffu, begins), real = __ballot_sync(0xffffffffu, p.row >= 0);
-            if (lane == 0) mbar_arrive_expect_tx(bar, __popc(real) * D);
-            if (begins) {
-                const uint32_t next = ((begin | ~real) >> lane) >> 1;
-                const uint32_t bytes = (next ? __ffs(next) : 32 - lane) * (D / 2);
-                const uint64_t source = static_cast<uint64_t>(p.row) * (D / 2);
-                bulk_load(stage_at + lane * (D / 2), args.codes[0] + source, bytes, bar);
-                bulk_load(stage_at + Shape::kCodeBytes + lane * (D / 2), args.codes[1] + source, bytes, bar);
-            }
-            const uint64_t params = static_cast<uint64_t>(max(p.row, 0)) * (kGroups * 4);
-            const uint32_t params_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
-            copy_async_params<kGroups * 4>(params_at, args.params[0] + params, p.row >= 0);
-            copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, p.row >= 0);
-            // Tokens rise from lane to lane. A place that holds none lies behind every query.
-            const int32_t last = __shfl_sync(0xffffffffu, p.token, 31);
-            masked &= ~(1u << fill_stage);
-            if (real != 0xffffffffu || last > extent.first ||
-                (args.window && last >= args.sinks && __shfl_sync(0xffffffffu, p.token, 0) <= extent.length - 1 - args.window)) {
-                masked |= 1u << fill_stage;
-                reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
-                    p.row >= 0 ? p.token : 0x7fffffff;
-            }
-            fill_stage = fill_stage == kStages - 1 ? 0 : fill_stage + 1;
-        };
-        Place next = locate(from);
-#pragma unroll
-        for (uint32_t s = 0; s < kStages - 1; ++s) {
-            if (from + s < to) {
-                issue(next);
-                next = locate(from + s + 1);
-            }
-            copy_async_commit();
+            at += length;  // only the segment's beginning lies in this share
         }
+        return false;
+    };
+    const auto next_piece = [&]() {
+        at += length;
+        if (at >= end) return false;
+        offset = 0;
+        if (++segment == segments) {
+            segment = 0;
+            ++b;
+            extent = extent_of(args, b, nullptr);
+            cost = cost_of(extent);
+        }
+        return find_piece();
+    };
 
+    // ---- copies: each warp keeps a ring of its own, 32 tokens a stage, lane = token. Tokens that follow each other
+    // in the cache are copied as one run of each code matrix by the lane of the run's first token; parameters come
+    // lane by lane (their rows are too short for bulk copies) as zeros where there is no token. The rows are looked up
+    // one unit ahead of their copies.
+    struct Place {
+        int32_t row, token;  // row -1: nothing to read
+    };
+    const auto locate = [&](uint32_t unit) {
+        const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens + lane);
+        Place p{-1, extent.token(place)};
+        if (place < extent.visible()) {
+            const uint32_t entry = args.page.quotient(static_cast<uint32_t>(p.token));
+            const uint32_t page =
+                args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + entry)) : b;
+            if (page < args.pages)
+                p.row = static_cast<int32_t>((page * args.kv_heads + kv_head) * args.page_size +
+                                             (static_cast<uint32_t>(p.token) - entry * args.page_size));
+            else
+                note(status, kBadPage, b, page);
+        }
+        return p;
+    };
+    const auto issue = [&](const Place& p) {
+        uint8_t* const stage = own + fill_stage * Shape::kStageBytes;
+        const uint32_t stage_at = smem_u32(stage), bar = barriers + 8 * fill_stage;
+        const int32_t ahead = __shfl_up_sync(0xffffffffu, p.row, 1);
+        const bool begins = p.row >= 0 && (lane == 0 || ahead < 0 || ahead + 1 != p.row);
+        const uint32_t begin = __ballot_sync(0xffffffffu, begins), real = __ballot_sync(0xffffffffu, p.row >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(real) * D);
+        if (begins) {
+            const uint32_t next = ((begin | ~real) >> lane) >> 1;
+            const uint32_t bytes = (next ? __ffs(next) : 32 - lane) * (D / 2);
+            const uint64_t source = static_cast<uint64_t>(p.row) * (D / 2);
+            bulk_load(stage_at + lane * (D / 2), args.codes[0] + source, bytes, bar);
+            bulk_load(stage_at + Shape::kCodeBytes + lane * (D / 2), args.codes[1] + source, bytes, bar);
+        }
+        const uint64_t params = static_cast<uint64_t>(max(p.row, 0)) * (kGroups * 4);
+        const uint32_t params_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
+        copy_async_params<kGroups * 4>(params_at, args.params[0] + params, p.row >= 0);
+        copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, p.row >= 0);
+        // Tokens rise from lane to lane. A place that holds none lies behind every query.
+        const int32_t last = __shfl_sync(0xffffffffu, p.token, 31);
+        masked &= ~(1u << fill_stage);
+        if (real != 0xffffffffu || last > extent.first ||
+            (args.window && last >= args.sinks && __shfl_sync(0xffffffffu, p.token, 0) <= extent.length - 1 - args.window)) {
+            masked |= 1u << fill_stage;
+            reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
+                p.row >= 0 ? p.token : 0x7fffffff;
+        }
+        fill_stage ^= 1;
+    };
+    Place next{-1, 0};
+    // A piece's first unit is on its way before the piece before it is merged.
+    const auto start_piece = [&]() {
+        issue(locate(from));
+        copy_async_commit();
+        next = locate(from + 1);
+    };
+
+    bool more = find_piece();
+    if (more) start_piece();
+    while (more) {
         // ---- queries as the second operand of the scores' product: lane (l4, c4) holds row l4 of each 8, in the
         // channel order of the key codes. The tile is scaled by a power of two so that its largest value lies in
         // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second register of each pair carries 1/16 for
@@ -673,12 +718,12 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
 #pragma unroll 1
         for (uint32_t unit = from; unit < to; ++unit) {
             __syncwarp();  // every lane is done with the stage that is filled next, and with the wide parameters
-            if (unit + kStages - 1 < to) {
+            if (unit + 1 < to) {
                 issue(next);
-                next = locate(unit + kStages);
+                next = locate(unit + 2);
             }
             copy_async_commit();
-            copy_async_wait<kStages - 1>();
+            copy_async_wait<1>();
             mbar_wait(barriers + 8 * use_stage, use_parity, site, kStallCodes, unit);
             __syncwarp();
             const uint8_t* const keys = own + use_stage * Shape::kStageBytes;
@@ -940,15 +985,26 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                         }
                 }
             }
-            use_stage = use_stage == kStages - 1 ? 0 : use_stage + 1;
+            use_stage ^= 1;
             use_parity ^= use_stage == 0;
         }
 
-        // ---- the warps' parts of the piece, through shared memory
-        copy_async_wait<0>();
+        // ---- the next piece's first unit is sent for; then the warps' parts of this one meet in shared memory, where
+        // its last unit was (and for more than one row tile, whose rows are more than a stage holds, beside the ring).
+        Cut piece{b, kv_head, first_row, from == 0 && to == units_of(cost) ? 0u : 1u, 0};
+        uint32_t which = 0;
+        if (piece.parts) {
+            const uint32_t first_unit = at - offset + args.segment_cost;
+            piece.owner = block_of(first_unit);
+            piece.parts = block_of(first_unit + units_of(cost) - 1) - piece.owner + 1;
+            which = piece.owner == blockIdx.x;
+        }
         __syncwarp();
+        more = next_piece();
+        if (more) start_piece();
+        const uint32_t merge_at = Shape::kMergeInRing ? (use_stage ^ 1) * Shape::kStageBytes : Shape::kMergeAt;
         {
-            float* const merged = reinterpret_cast<float*>(own);
+            float* const merged = reinterpret_cast<float*>(own + merge_at);
             float* const stats = merged + kRows * kPitch;
             const float unfit = power_of_two(254 - min(kFitBiased - top, 254));
 #pragma unroll
@@ -984,13 +1040,11 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 }
         }
         __syncthreads();
-        const uint32_t rows_here = min(kRows, args.rows - first_row);
-        const bool whole = from == 0 && to == units;
-        const uint8_t* const rings = shared + Shape::kQueryBytes;
+        const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
+        uint8_t* const rings = shared + Shape::kQueryBytes + merge_at;
         // A warp for each row: the warps' shares of it, left in the place of their references.
         for (uint32_t row = warp; row < rows_here; row += warps) {
-            float2* const its = reinterpret_cast<float2*>(const_cast<uint8_t*>(rings) + min(lane, warps - 1) * Shape::kWarpBytes +
-                                                          kRows * kPitch * 4) + row;
+            float2* const its = reinterpret_cast<float2*>(rings + min(lane, warps - 1) * Shape::kWarpBytes + kRows * kPitch * 4) + row;
             const float2 stat = lane < warps ? *its : make_float2(-INFINITY, 0.0f);
             float m = stat.x;
 #pragma unroll
@@ -1000,103 +1054,93 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
 #pragma unroll
             for (uint32_t mask = 16; mask > 0; mask >>= 1) s += __shfl_xor_sync(0xffffffffu, s, mask);
             if (lane < warps) its->x = factor;
-            if (lane == 0) {
-                row_stats[row] = make_float2(m, s);
-            }
+            if (lane == 0) row_stats[row] = make_float2(m, s);
         }
         __syncthreads();
-        // A segment cut over blocks: the block its first unit lies in keeps its part in its second place, the others in
-        // their first.
-        const uint32_t owner = whole ? 0 : block_of(segment_at);
-        float* const part = args.partials + (2 * blockIdx.x + (owner == blockIdx.x ? 1 : 0)) * static_cast<size_t>(kPartialFloats);
-        const auto finish = [&](uint32_t row, uint32_t d, float4 y, float2 stat) {
-            const uint32_t r = first_row + row, t = args.ratio.quotient(r);
-            const uint64_t place = (static_cast<uint64_t>(b) * args.queries + t) * args.heads + kv_head * args.ratio.divisor +
-                                   (r - t * args.ratio.divisor);
-            const float inverse = stat.y == 0.0f ? 0.0f : __fdividef(1.0f, stat.y);
-            if (stat.y == 0.0f) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            *reinterpret_cast<uint2*>(args.out + place * D + d) =
-                make_uint2(E::pack(y.x * inverse, y.y * inverse), E::pack(y.z * inverse, y.w * inverse));
-            if (d == 0 && args.lse) args.lse[place] = stat.y == 0.0f ? -INFINITY : (stat.x + log2f(stat.y)) * 0.6931471805599453f;
-        };
+        // A part of a segment that is cut over blocks: the block its first unit lies in keeps it in its second place, the others in
+        // their first. Parts are handed in together at the end.
+        float* const part = args.partials + (2 * blockIdx.x + which) * static_cast<size_t>(kPartialFloats);
+        if (piece.parts && threadIdx.x == 0) cuts[which] = piece;
         for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
             const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
             for (uint32_t w = 0; w < warps; ++w) {
                 const float* const its = reinterpret_cast<const float*>(rings + w * Shape::kWarpBytes);
                 const float factor = its[kRows * kPitch + 2 * row];
                 const float4 z = *reinterpret_cast<const float4*>(its + row * kPitch + d);
                 y = make_float4(fmaf(z.x, factor, y.x), fmaf(z.y, factor, y.y), fmaf(z.z, factor, y.z), fmaf(z.w, factor, y.w));
             }
-            if (whole) {
-                finish(row, d, y, row_stats[row]);
+            if (piece.parts == 0) {
+                finish_row<D, BF16>(args, piece, row, d, y, row_stats[row]);
             } else {
                 *reinterpret_cast<float4*>(part + row * D + d) = y;
                 if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
             }
         }
-        if (!whole) {
-            // The block that comes last adds the parts up, always in the same order.
-            const uint32_t parts = block_of(segment_at + units - 1) - owner + 1;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                __threadfence();
-                const uint32_t came = atomicAdd(args.arrivals + owner, 1u);
-                if (came == parts - 1) args.arrivals[owner] = 0;
-                last_to_come = came == parts - 1;
-                __threadfence();
-            }
-            __syncthreads();
-            if (last_to_come) {
-                const float* const base = args.partials + 2 * owner * static_cast<size_t>(kPartialFloats);
-                for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
-                    const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
-                    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float2 all = make_float2(-INFINITY, 0.0f);
-                    constexpr uint32_t kBatch = 4;
-                    for (uint32_t p = 0; p < parts; p += kBatch) {
-                        float4 z[kBatch];
-                        float2 stat[kBatch];
-#pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) {
-                            const uint32_t q = min(p + k, parts - 1);
-                            const float* const its = base + (2 * q + (q == 0)) * static_cast<size_t>(kPartialFloats);
-                            stat[k] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
-                            z[k] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
-                            if (p + k >= parts) stat[k] = make_float2(-INFINITY, 0.0f);
-                        }
-                        float m = all.x;
-#pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) m = fmaxf(m, stat[k].x);
-                        const float keep = all.x == -INFINITY ? 0.0f : ex2_approx(all.x - m);
-                        y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
-                        all = make_float2(m, all.y * keep);
-#pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) {
-                            const float factor = stat[k].x == -INFINITY ? 0.0f : ex2_approx(stat[k].x - m);
-                            if (p + k < parts) {
-                                y = make_float4(fmaf(z[k].x, factor, y.x), fmaf(z[k].y, factor, y.y), fmaf(z[k].z, factor, y.z),
-                                                fmaf(z[k].w, factor, y.w));
-                                all.y = fmaf(stat[k].y, factor, all.y);
-                            }
-                        }
-                    }
-                    finish(row, d, y, all);
-                }
-            }
-        }
-        // The merged rows lie where the rings are: they are read before the next copies, which come by another way.
+        // Copies to where the merged rows lay come by another way than these reads.
         fence_proxy_async_shared();
         __syncthreads();
-        }
+    }
 
-        at += length;
-        offset = 0;
-        if (at < end && ++segment == segments) {
-            segment = 0;
-            ++b;
-            extent = extent_of(args, b, nullptr);
-            cost = cost_of(extent);
+    // ---- the parts of segments that are cut over blocks: the block that comes last to one adds them up, always in the same
+    // order, and leaves the counter at zero.
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        complete[0] = complete[1] = 0;
+        if (cuts[0].parts || cuts[1].parts) {
+            __threadfence();
+            uint32_t came[2] = {};
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c)
+                if (cuts[c].parts) came[c] = atomicAdd(args.arrivals + cuts[c].owner, 1u);
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c)
+                if (cuts[c].parts && came[c] == cuts[c].parts - 1) {
+                    args.arrivals[cuts[c].owner] = 0;
+                    complete[c] = 1;
+                }
+            __threadfence();
+        }
+    }
+    __syncthreads();
+    for (uint32_t c = 0; c < 2; ++c) {
+        if (!complete[c]) continue;
+        const Cut piece = cuts[c];
+        const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
+        const float* const base = args.partials + 2 * piece.owner * static_cast<size_t>(kPartialFloats);
+        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
+            const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float2 all = make_float2(-INFINITY, 0.0f);
+            constexpr uint32_t kBatch = 4;
+#pragma unroll 1
+            for (uint32_t p = 0; p < piece.parts; p += kBatch) {
+                float4 z[kBatch];
+                float2 stat[kBatch];
+#pragma unroll
+                for (uint32_t k = 0; k < kBatch; ++k) {
+                    const uint32_t q = min(p + k, piece.parts - 1);
+                    const float* const its = base + (2 * q + (q == 0)) * static_cast<size_t>(kPartialFloats);
+                    stat[k] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
+                    z[k] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
+                }
+                float m = all.x;
+#pragma unroll
+                for (uint32_t k = 0; k < kBatch; ++k) m = fmaxf(m, stat[k].x);
+                const float keep = all.x == -INFINITY ? 0.0f : ex2_approx(all.x - m);
+                y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
+                all = make_float2(m, all.y * keep);
+#pragma unroll
+                for (uint32_t k = 0; k < kBatch; ++k) {
+                    if (p + k >= piece.parts || stat[k].x == -INFINITY) continue;
+                    const float factor = ex2_approx(stat[k].x - m);
+                    y = make_float4(fmaf(z[k].x, factor, y.x), fmaf(z[k].y, factor, y.y), fmaf(z[k].z, factor, y.z),
+                                    fmaf(z[k].w, factor, y.w));
+                    all.y = fmaf(stat[k].y, factor, all.y);
+                }
+            }
+            finish_row<D, BF16>(args, piece, row, d, y, all);
         }
     }
     // After a wait that gave up, copies may still be on their way: give them a while before the block's memory goes.
