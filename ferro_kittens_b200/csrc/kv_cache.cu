@@ -573,41 +573,48 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     // lane by lane (their rows are too short for bulk copies) as zeros where there is no token. The rows are looked up
     // one unit ahead of their copies.
     struct Place {
-        int32_t row, token;  // row -1: nothing to read
+        uint32_t page;
+        int32_t token;  // -1: nothing to read
     };
+    // Only asks for the page: a unit of work passes before issue() looks at the answer.
     const auto locate = [&](uint32_t unit) {
         const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens + lane);
-        Place p{-1, extent.token(place)};
+        Place p{b, -1};
         if (place < extent.visible()) {
-            const uint32_t entry = args.page.quotient(static_cast<uint32_t>(p.token));
-            const uint32_t page =
-                args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + entry)) : b;
-            if (page < args.pages)
-                p.row = static_cast<int32_t>((page * args.kv_heads + kv_head) * args.page_size +
-                                             (static_cast<uint32_t>(p.token) - entry * args.page_size));
-            else
-                note(status, kBadPage, b, page);
+            p.token = extent.token(place);
+            if (args.table)
+                p.page = static_cast<uint32_t>(
+                    __ldg(args.table + b * args.table_stride + args.page.quotient(static_cast<uint32_t>(p.token))));
         }
         return p;
     };
     const auto issue = [&](const Place& p) {
+        int32_t row = -1;
+        if (p.token >= 0) {
+            const uint32_t token = static_cast<uint32_t>(p.token);
+            if (p.page < args.pages)
+                row = static_cast<int32_t>((p.page * args.kv_heads + kv_head) * args.page_size +
+                                           (token - args.page.quotient(token) * args.page_size));
+            else
+                note(status, kBadPage, b, p.page);
+        }
         uint8_t* const stage = own + fill_stage * Shape::kStageBytes;
         const uint32_t stage_at = smem_u32(stage), bar = barriers + 8 * fill_stage;
-        const int32_t ahead = __shfl_up_sync(0xffffffffu, p.row, 1);
-        const bool begins = p.row >= 0 && (lane == 0 || ahead < 0 || ahead + 1 != p.row);
-        const uint32_t begin = __ballot_sync(0xffffffffu, begins), real = __ballot_sync(0xffffffffu, p.row >= 0);
+        const int32_t ahead = __shfl_up_sync(0xffffffffu, row, 1);
+        const bool begins = row >= 0 && (lane == 0 || ahead < 0 || ahead + 1 != row);
+        const uint32_t begin = __ballot_sync(0xffffffffu, begins), real = __ballot_sync(0xffffffffu, row >= 0);
         if (lane == 0) mbar_arrive_expect_tx(bar, __popc(real) * D);
         if (begins) {
             const uint32_t next = ((begin | ~real) >> lane) >> 1;
             const uint32_t bytes = (next ? __ffs(next) : 32 - lane) * (D / 2);
-            const uint64_t source = static_cast<uint64_t>(p.row) * (D / 2);
+            const uint64_t source = static_cast<uint64_t>(row) * (D / 2);
             bulk_load(stage_at + lane * (D / 2), args.codes[0] + source, bytes, bar);
             bulk_load(stage_at + Shape::kCodeBytes + lane * (D / 2), args.codes[1] + source, bytes, bar);
         }
-        const uint64_t params = static_cast<uint64_t>(max(p.row, 0)) * (kGroups * 4);
+        const uint64_t params = static_cast<uint64_t>(max(row, 0)) * (kGroups * 4);
         const uint32_t params_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
-        copy_async_params<kGroups * 4>(params_at, args.params[0] + params, p.row >= 0);
-        copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, p.row >= 0);
+        copy_async_params<kGroups * 4>(params_at, args.params[0] + params, row >= 0);
+        copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, row >= 0);
         // Tokens rise from lane to lane. A place that holds none lies behind every query.
         const int32_t last = __shfl_sync(0xffffffffu, p.token, 31);
         masked &= ~(1u << fill_stage);
@@ -615,11 +622,11 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             (args.window && last >= args.sinks && __shfl_sync(0xffffffffu, p.token, 0) <= extent.length - 1 - args.window)) {
             masked |= 1u << fill_stage;
             reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
-                p.row >= 0 ? p.token : 0x7fffffff;
+                row >= 0 ? p.token : 0x7fffffff;
         }
         fill_stage ^= 1;
     };
-    Place next{-1, 0};
+    Place next{0, -1};
     // A piece's first unit is on its way before the piece before it is merged.
     const auto start_piece = [&]() {
         issue(locate(from));
