@@ -329,7 +329,7 @@ constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
 constexpr float kSlack = 8.0f;
 constexpr int32_t kFit = 6;
 constexpr int32_t kFitBiased = 254 + kFit;  // less a scale's biased exponent: that of the power that brings it to 2^kFit
-constexpr uint32_t kStallCodes = 0x504;  // a warp waiting for a stage of codes
+constexpr uint32_t kStallCodes = 0x504;  // a warp waiting for a stage of tokens
 
 template <int D, int G, int NT>
 struct AttentionShape {
@@ -338,18 +338,17 @@ struct AttentionShape {
     // One row tile's queries stay in registers; of more, the fragments and sums lie in shared memory.
     static constexpr bool kSharedQueries = NT > 1;
     static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 : 0;
-    // A warp's memory: a ring of stages, the unit's parameters as floats, room for the merge of the warps' results where a
-    // stage has too little, the stages' barriers.
+    // A warp's memory: a ring of stages; the unit's parameters as floats, and over them the merge of the warps' results; for
+    // each stage a barrier and a word that says which of its tokens are there.
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
     static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
-    static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes + kWarpTokens * 4;
+    static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes;
     static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 8;
     static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
     static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
-    static constexpr bool kMergeInRing = kMergeBytes <= kStageBytes;
-    static constexpr uint32_t kMergeAt = kStages * kStageBytes + 2 * kWideBytes;
-    static constexpr uint32_t kBarriers = kMergeAt + (kMergeInRing ? 0 : kMergeBytes);
-    static constexpr uint32_t kWarpBytes = kBarriers + 16 * ((kStages + 1) / 2);
+    static constexpr uint32_t kMergeAt = kStages * kStageBytes;
+    static constexpr uint32_t kBarriers = kMergeAt + (2 * kWideBytes > kMergeBytes ? 2 * kWideBytes : kMergeBytes);
+    static constexpr uint32_t kWarpBytes = kBarriers + kStages * 16;
     // Registers a thread: 128, 168 or 255.
     static constexpr uint32_t kMostByRegisters = NT == 1 ? (kGroups > 2 ? 12 : 16) : NT == 2 ? 12 : 8;
     static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
@@ -386,21 +385,18 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
         "l"(src), "r"(bytes), "r"(bar)
         : "memory");
 }
-/// BYTES of a row's parameters, or zeros where the row is not to be read.
+/// BYTES of a row's parameters.
 template <int BYTES>
-__device__ __forceinline__ void copy_async_params(uint32_t dst, const void* src, bool real) {
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
     if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16u : 0u) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(real ? BYTES : 0)
-                     : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+/// The barrier's phase also waits for this thread's copy_async so far (one more arrival, made when they have landed).
+__device__ __forceinline__ void copy_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-
 /// D[16, 8] += A[16, 16] . B[16, 8] in fp16 with fp32 sums.
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                             uint32_t b1) {
@@ -480,9 +476,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     __shared__ float2 row_stats[kRows];  // reference and sum of each row over the warps
     const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
-    const uint32_t l4 = lane / 4, c4 = lane % 4;
-    uint8_t* const own = shared + Shape::kQueryBytes + warp * Shape::kWarpBytes;
-    const uint32_t barriers = smem_u32(own + Shape::kBarriers);
+    const auto memory_of = [&](uint32_t w) { return shared + Shape::kQueryBytes + w * Shape::kWarpBytes; };
 
     // ---- this block's share: units of unit_tokens tokens, sequence by sequence, (kv head, row tile) by (kv head,
     // row tile), cut evenly over the blocks whatever the lengths are. A segment, one sequence's units of one (kv
@@ -525,19 +519,20 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
 
+    uint8_t* const own = memory_of(warp);
     if (lane == 0)
-        for (uint32_t s = 0; s < kStages; ++s) mbar_init(barriers + 8 * s, 1);
+        for (uint32_t s = 0; s < kStages; ++s) mbar_init(smem_u32(own + Shape::kBarriers + 16 * s), 1);
     if (threadIdx.x == 0) stop_flag = cuts[0].parts = cuts[1].parts = 0;
     fence_mbarrier_init();
     __syncthreads();
     const StallSite site{status, &stop_flag, 0};
+    bool live = true;  // until a wait gives up: nothing is waited for after that
 
     Extent extent = extent_of(args, b, nullptr);
     uint32_t cost = cost_of(extent);
     uint32_t segment = (at - before) / cost;
     uint32_t offset = (at - before) - segment * cost;  // of `at` in its segment
-    uint32_t fill_stage = 0, use_stage = 0, use_parity = 0;
-    uint32_t masked = 0;  // bit s: some row may not see some token of stage s
+    uint32_t stage = 0, parity = 0;
     // The piece at hand: units [from, to) of the segment (b, kv_head, rows from first_row).
     uint32_t length = 0, from = 0, to = 0, kv_head = 0, first_row = 0;
     const auto units_of = [&](uint32_t its_cost) { return its_cost - args.segment_cost; };
@@ -568,72 +563,78 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         return find_piece();
     };
 
-    // ---- copies: each warp keeps a ring of its own, 32 tokens a stage, lane = token. Tokens that follow each other
-    // in the cache are copied as one run of each code matrix by the lane of the run's first token; parameters come
-    // lane by lane (their rows are too short for bulk copies) as zeros where there is no token. The rows are looked up
-    // one unit ahead of their copies.
-    struct Place {
-        uint32_t page;
-        int32_t token;  // -1: nothing to read
+    // ---- copies. Each warp keeps a ring of its own, 32 tokens a stage: tokens that follow each other in a page are one
+    // run, copied in bulk by one thread, codes and parameters of both sides. (Parameters of runs that do not begin and end
+    // on 16 bytes go token by token.) The page of a unit's first run is asked for a unit before it is needed.
+    uint32_t fill_stage = 0, next_page = 0;
+    const auto page_at = [&](int32_t place) {
+        return args.table ? static_cast<uint32_t>(
+                                __ldg(args.table + b * args.table_stride + args.page.quotient(extent.token(place))))
+                          : b;
     };
-    // Only asks for the page: a unit of work passes before issue() looks at the answer.
-    const auto locate = [&](uint32_t unit) {
-        const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens + lane);
-        Place p{b, -1};
-        if (place < extent.visible()) {
-            p.token = extent.token(place);
-            if (args.table)
-                p.page = static_cast<uint32_t>(
-                    __ldg(args.table + b * args.table_stride + args.page.quotient(static_cast<uint32_t>(p.token))));
-        }
-        return p;
+    const auto place_of = [&](uint32_t unit) { return static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens); };
+    const auto ask = [&](uint32_t unit) {
+        if (place_of(unit) < extent.visible()) next_page = page_at(place_of(unit));
     };
-    const auto issue = [&](const Place& p) {
-        int32_t row = -1;
-        if (p.token >= 0) {
-            const uint32_t token = static_cast<uint32_t>(p.token);
-            if (p.page < args.pages)
-                row = static_cast<int32_t>((p.page * args.kv_heads + kv_head) * args.page_size +
-                                           (token - args.page.quotient(token) * args.page_size));
-            else
-                note(status, kBadPage, b, p.page);
+    const auto issue = [&](uint32_t unit) {
+        const int32_t place = place_of(unit);
+        const uint32_t full = smem_u32(own + Shape::kBarriers + 16 * fill_stage);
+        const uint32_t memory_at = smem_u32(own + fill_stage * Shape::kStageBytes);
+        if (elect_one()) {
+            const int32_t count = min(extent.visible() - place, static_cast<int32_t>(kWarpTokens));
+            uint32_t real = 0, bytes = 0, page = next_page;
+            bool single = false;
+#pragma unroll 1
+            for (int32_t i = 0; i < count;) {
+                const uint32_t token = static_cast<uint32_t>(extent.token(place + i));
+                const uint32_t inside = token - args.page.quotient(token) * args.page_size;
+                uint32_t run = min(static_cast<uint32_t>(count - i), args.page_size - inside);
+                if (place + i < extent.kept) run = min(run, static_cast<uint32_t>(extent.kept - place - i));
+                const int32_t then = i + static_cast<int32_t>(run);
+                const uint32_t then_page = then < count ? page_at(place + then) : 0;
+                if (page < args.pages) {
+                    const uint64_t row = (page * args.kv_heads + kv_head) * args.page_size + inside;
+                    const uint32_t to_at = memory_at + i * (D / 2);
+                    bulk_load(to_at, args.codes[0] + row * (D / 2), run * (D / 2), full);
+                    bulk_load(to_at + Shape::kCodeBytes, args.codes[1] + row * (D / 2), run * (D / 2), full);
+                    bytes += run * D;
+                    const uint32_t params_at = memory_at + 2 * Shape::kCodeBytes + i * (kGroups * 4);
+                    const uint64_t params = row * (kGroups * 4);
+                    if (((static_cast<uint32_t>(params) | params_at | run * (kGroups * 4)) & 15u) == 0) {
+                        bulk_load(params_at, args.params[0] + params, run * (kGroups * 4), full);
+                        bulk_load(params_at + Shape::kParamBytes, args.params[1] + params, run * (kGroups * 4), full);
+                        bytes += run * (kGroups * 8);
+                    } else {
+                        single = true;
+#pragma unroll 1
+                        for (uint32_t r = 0; r < run; ++r) {
+                            copy_async<kGroups * 4>(params_at + r * (kGroups * 4), args.params[0] + params + r * (kGroups * 4));
+                            copy_async<kGroups * 4>(params_at + Shape::kParamBytes + r * (kGroups * 4),
+                                                    args.params[1] + params + r * (kGroups * 4));
+                        }
+                    }
+                    real |= (run == 32 ? 0xffffffffu : (1u << run) - 1) << i;
+                } else {
+                    note(status, kBadPage, b, page);
+                }
+                i = then;
+                page = then_page;
+            }
+            *reinterpret_cast<uint32_t*>(own + Shape::kBarriers + 16 * fill_stage + 8) = real;
+            if (single) copy_async_arrive(full);
+            mbar_arrive_expect_tx(full, bytes);
         }
-        uint8_t* const stage = own + fill_stage * Shape::kStageBytes;
-        const uint32_t stage_at = smem_u32(stage), bar = barriers + 8 * fill_stage;
-        const int32_t ahead = __shfl_up_sync(0xffffffffu, row, 1);
-        const bool begins = row >= 0 && (lane == 0 || ahead < 0 || ahead + 1 != row);
-        const uint32_t begin = __ballot_sync(0xffffffffu, begins), real = __ballot_sync(0xffffffffu, row >= 0);
-        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(real) * D);
-        if (begins) {
-            const uint32_t next = ((begin | ~real) >> lane) >> 1;
-            const uint32_t bytes = (next ? __ffs(next) : 32 - lane) * (D / 2);
-            const uint64_t source = static_cast<uint64_t>(row) * (D / 2);
-            bulk_load(stage_at + lane * (D / 2), args.codes[0] + source, bytes, bar);
-            bulk_load(stage_at + Shape::kCodeBytes + lane * (D / 2), args.codes[1] + source, bytes, bar);
-        }
-        const uint64_t params = static_cast<uint64_t>(max(row, 0)) * (kGroups * 4);
-        const uint32_t params_at = stage_at + 2 * Shape::kCodeBytes + lane * kGroups * 4;
-        copy_async_params<kGroups * 4>(params_at, args.params[0] + params, row >= 0);
-        copy_async_params<kGroups * 4>(params_at + Shape::kParamBytes, args.params[1] + params, row >= 0);
-        // Tokens rise from lane to lane. A place that holds none lies behind every query.
-        const int32_t last = __shfl_sync(0xffffffffu, p.token, 31);
-        masked &= ~(1u << fill_stage);
-        if (real != 0xffffffffu || last > extent.first ||
-            (args.window && last >= args.sinks && __shfl_sync(0xffffffffu, p.token, 0) <= extent.length - 1 - args.window)) {
-            masked |= 1u << fill_stage;
-            reinterpret_cast<int32_t*>(stage + 2 * Shape::kCodeBytes + 2 * Shape::kParamBytes)[lane] =
-                row >= 0 ? p.token : 0x7fffffff;
-        }
+        __syncwarp();
         fill_stage ^= 1;
     };
-    Place next{0, -1};
     // A piece's first unit is on its way before the piece before it is merged.
     const auto start_piece = [&]() {
-        issue(locate(from));
-        copy_async_commit();
-        next = locate(from + 1);
+        ask(from);
+        issue(from);
+        ask(from + 1);
     };
 
+    const uint32_t l4 = lane / 4, c4 = lane % 4;
     bool more = find_piece();
     if (more) start_piece();
     while (more) {
@@ -656,6 +657,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) {
             const uint8_t* const q = row_of(n);
+            float row_most = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kKeyWords; ++w) {
                 raw[n][w] = make_uint4(0, 0, 0, 0);
@@ -663,10 +665,11 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 const uint32_t words[4] = {raw[n][w].x, raw[n][w].y, raw[n][w].z, raw[n][w].w};
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
-                    most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
+                    row_most = fmaxf(row_most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
             }
+            if (row_most < INFINITY) most = fmaxf(most, row_most);  // a row that holds an infinity says nothing about others
         }
-        most = __uint_as_float(__reduce_max_sync(0xffffffffu, most < INFINITY ? __float_as_uint(most) : 0u));
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
         const int32_t biased = most == 0.0f ? 127 : min(268 - static_cast<int32_t>(__float_as_uint(most) >> 23), 254);
         const float up = power_of_two(biased);
         const float to_log2 = args.scale * 1.4426950408889634f * 0x1p24f * power_of_two(254 - biased);
@@ -719,26 +722,28 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
         // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
         const uint32_t own_token = (l4 >> 1) + 4 * (l4 & 1);
-        uint8_t* const wide_keys = own + kStages * Shape::kStageBytes;  // (scale, low) * to_log2 of each token and group
+        uint8_t* const wide_keys = own + Shape::kMergeAt;  // (scale, low) * to_log2 of each token and group
         uint8_t* const wide_values = wide_keys + Shape::kWideBytes;     // (scale * fit, low + 8 * scale)
 
 #pragma unroll 1
         for (uint32_t unit = from; unit < to; ++unit) {
-            __syncwarp();  // every lane is done with the stage that is filled next, and with the wide parameters
             if (unit + 1 < to) {
-                issue(next);
-                next = locate(unit + 2);
+                issue(unit + 1);
+                ask(unit + 2);
             }
-            copy_async_commit();
-            copy_async_wait<1>();
-            mbar_wait(barriers + 8 * use_stage, use_parity, site, kStallCodes, unit);
-            __syncwarp();
-            const uint8_t* const keys = own + use_stage * Shape::kStageBytes;
+            const uint32_t full = smem_u32(own + Shape::kBarriers + 16 * stage);
+            if (live) live = mbar_wait(full, parity, site, kStallCodes, unit);
+            const uint8_t* const keys = own + stage * Shape::kStageBytes;
             const uint8_t* const values = keys + Shape::kCodeBytes;
             const uint8_t* const key_params = keys + 2 * Shape::kCodeBytes;
             const uint8_t* const value_params = key_params + Shape::kParamBytes;
-            const int32_t* const tokens = reinterpret_cast<const int32_t*>(value_params + Shape::kParamBytes);
-            const bool is_masked = masked >> use_stage & 1u;
+            // Which of the 32 tokens are there, and whether some row may not see some token (they rise from place to place).
+            const uint32_t real = *reinterpret_cast<const uint32_t*>(own + Shape::kBarriers + 16 * stage + 8);
+            const int32_t place = place_of(unit);
+            const bool is_masked = real != 0xffffffffu || extent.token(place + 31) > extent.first ||
+                                   (args.window && extent.token(place + 31) >= args.sinks &&
+                                    extent.token(place) <= extent.length - 1 - args.window);
+            const bool is_real = real >> lane & 1u;
             bool careful = false;  // some token that some row may not see has values that are not finite
 
             // ---- parameters as floats, lane = token, and the power of two that lets weight * scale fit fp16 whatever the
@@ -749,6 +754,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 load_words(pairs, value_params + lane * (kGroups * 4));
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g) {
+                    if (!is_real) pairs[g] = 0;
                     scales[g] = E::low(pairs[g]);
                     widest = fmaxf(widest, fabsf(scales[g]));
                 }
@@ -790,6 +796,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                     wide[g] = make_float2(scales[g] * fit, fmaf(8.0f, scales[g], E::high(pairs[g])));
                 store_floats(wide_values + lane * (kGroups * 8), wide);
                 load_words(pairs, key_params + lane * (kGroups * 4));
+                if (!is_real) {
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) pairs[g] = 0;
+                }
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g) wide[g] = make_float2(E::low(pairs[g]) * to_log2, E::high(pairs[g]) * to_log2);
                 store_floats(wide_keys + lane * (kGroups * 8), wide);
@@ -858,8 +868,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                             for (uint32_t h = 0; h < kSteps; ++h)
 #pragma unroll
                                 for (uint32_t half = 0; half < 2; ++half) {
-                                    const int32_t j = tokens[16 * (round * kSteps + h) + 8 * half + own_token];
-                                    const bool seen = j <= i && (!args.window || j > i - args.window || j < args.sinks);
+                                    const uint32_t k = 16 * (round * kSteps + h) + 8 * half + own_token;
+                                    const int32_t j = extent.token(place + static_cast<int32_t>(k));
+                                    const bool seen = (real >> k & 1u) && j <= i &&
+                                                      (!args.window || j > i - args.window || j < args.sinks);
                                     if (!seen) x[h][n][2 * half + e] = -INFINITY;
                                 }
                         }
@@ -992,12 +1004,12 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                         }
                 }
             }
-            use_stage ^= 1;
-            use_parity ^= use_stage == 0;
+            __syncwarp();  // every lane is done with the stage, which is filled next, and with the wide parameters
+            stage ^= 1;
+            parity ^= stage == 0;
         }
 
-        // ---- the next piece's first unit is sent for; then the warps' parts of this one meet in shared memory, where
-        // its last unit was (and for more than one row tile, whose rows are more than a stage holds, beside the ring).
+        // ---- the warps' parts of the piece meet in shared memory
         Cut piece{b, kv_head, first_row, from == 0 && to == units_of(cost) ? 0u : 1u, 0};
         uint32_t which = 0;
         if (piece.parts) {
@@ -1006,12 +1018,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             piece.parts = block_of(first_unit + units_of(cost) - 1) - piece.owner + 1;
             which = piece.owner == blockIdx.x;
         }
-        __syncwarp();
         more = next_piece();
         if (more) start_piece();
-        const uint32_t merge_at = Shape::kMergeInRing ? (use_stage ^ 1) * Shape::kStageBytes : Shape::kMergeAt;
         {
-            float* const merged = reinterpret_cast<float*>(own + merge_at);
+            float* const merged = reinterpret_cast<float*>(own + Shape::kMergeAt);
             float* const stats = merged + kRows * kPitch;
             const float unfit = power_of_two(254 - min(kFitBiased - top, 254));
 #pragma unroll
@@ -1048,7 +1058,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         }
         __syncthreads();
         const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
-        uint8_t* const rings = shared + Shape::kQueryBytes + merge_at;
+        uint8_t* const rings = memory_of(0) + Shape::kMergeAt;
         // A warp for each row: the warps' shares of it, left in the place of their references.
         for (uint32_t row = warp; row < rows_here; row += warps) {
             float2* const its = reinterpret_cast<float2*>(rings + min(lane, warps - 1) * Shape::kWarpBytes + kRows * kPitch * 4) + row;
@@ -1068,7 +1078,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         // their first. Parts are handed in together at the end.
         float* const part = args.partials + (2 * blockIdx.x + which) * static_cast<size_t>(kPartialFloats);
         if (piece.parts && threadIdx.x == 0) cuts[which] = piece;
-        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
+        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
             const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
@@ -1085,8 +1095,6 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
             }
         }
-        // Copies to where the merged rows lay come by another way than these reads.
-        fence_proxy_async_shared();
         __syncthreads();
     }
 
@@ -1116,7 +1124,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         const Cut piece = cuts[c];
         const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
         const float* const base = args.partials + 2 * piece.owner * static_cast<size_t>(kPartialFloats);
-        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += blockDim.x) {
+        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
             const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float2 all = make_float2(-INFINITY, 0.0f);
@@ -1152,8 +1160,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     }
     // After a wait that gave up, copies may still be on their way: give them a while before the block's memory goes.
     if (stop_flag)
-        for (uint32_t s = 0; s < kStages; ++s)
-            for (uint32_t i = 0; i < 1000 && !mbar_try_wait(barriers + 8 * s, use_parity ^ (s < use_stage)); ++i) {
+        for (uint32_t k = 0; k < 2 * kStages; ++k)
+            for (uint32_t i = 0; i < 100 && !mbar_try_wait(smem_u32(own + Shape::kBarriers + 16 * (k / 2)), k & 1); ++i) {
             }
 }
 
@@ -1298,9 +1306,10 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     if (admitted != FK_OK) return admitted;
     args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
-    const uint32_t small = 4;
-    const uint32_t warps = segments >= 2ull * facts.sm_count ? small : Shape::kMostWarps;
-    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (warps == small ? Shape::kMostWarps / small : 1);
+    const uint32_t half = Shape::kMostWarps / 2;
+    const bool whole = segments < 2ull * facts.sm_count;
+    const uint32_t warps = whole ? Shape::kMostWarps : half;
+    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (whole ? 1 : 2);
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
     args.least_units = 3;
     args.segment_cost = 1;
