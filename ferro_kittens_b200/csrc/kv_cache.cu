@@ -313,12 +313,13 @@ struct AttentionArguments {
     Divider page, ratio;
     uint32_t least_units;   // units a block takes before another block is put to work
     uint32_t segment_cost;  // what beginning and ending a segment takes, in units
+    uint32_t copying;       // warps that copy
     uint32_t* arrivals;    // workspace: a counter for each block, then the partial results
     float* partials;
 };
 
 constexpr uint32_t kWarpTokens = 32;
-constexpr uint32_t kStages = 2;
+constexpr uint32_t kStages = 3;
 constexpr uint32_t kMostBlocksPerSm = 4;
 constexpr uint32_t kMostRows = 32;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
@@ -329,7 +330,8 @@ constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
 constexpr float kSlack = 8.0f;
 constexpr int32_t kFit = 6;
 constexpr int32_t kFitBiased = 254 + kFit;  // less a scale's biased exponent: that of the power that brings it to 2^kFit
-constexpr uint32_t kStallCodes = 0x504;  // a warp waiting for a stage of tokens
+constexpr uint32_t kStallFull = 0x504;  // a computing warp waiting for a stage of tokens
+constexpr uint32_t kStallFree = 0x505;  // a copying warp waiting for a stage to be free
 
 template <int D, int G, int NT>
 struct AttentionShape {
@@ -338,28 +340,30 @@ struct AttentionShape {
     // One row tile's queries stay in registers; of more, the fragments and sums lie in shared memory.
     static constexpr bool kSharedQueries = NT > 1;
     static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 : 0;
-    // A warp's memory: a ring of stages; the unit's parameters as floats, and over them the merge of the warps' results; for
-    // each stage a barrier and a word that says which of its tokens are there.
+    // For each computing warp: its tokens in each stage, and the unit's parameters as floats. The merge of the warps' results
+    // lies over the piece's last stage, which is given back after it, or (where rows are more than fit there) beside.
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
     static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
     static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes;
     static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 8;
     static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
     static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
-    static constexpr uint32_t kMergeAt = kStages * kStageBytes;
-    static constexpr uint32_t kBarriers = kMergeAt + (2 * kWideBytes > kMergeBytes ? 2 * kWideBytes : kMergeBytes);
-    static constexpr uint32_t kWarpBytes = kBarriers + kStages * 16;
+    static constexpr bool kMergeInRing = kMergeBytes <= kStageBytes;
+    static constexpr uint32_t kScratchBytes = kMergeInRing || 2 * kWideBytes > kMergeBytes ? 2 * kWideBytes : kMergeBytes;
+    static constexpr uint32_t kWarpBytes = kStages * kStageBytes + kScratchBytes;
     // Registers a thread: 128, 168 or 255.
-    static constexpr uint32_t kMostByRegisters = NT == 1 ? (kGroups > 2 ? 12 : 16) : NT == 2 ? 12 : 8;
+    static constexpr uint32_t kMostThreads = 32 * (NT == 1 ? (kGroups > 2 ? 12 : 16) : NT == 2 ? 12 : 8);
     static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
-    static constexpr uint32_t kMostWarps = kMostByRegisters < kMostByMemory ? kMostByRegisters : kMostByMemory;
+    static constexpr uint32_t most_warps(uint32_t copying) {
+        return kMostThreads / 32 - copying < kMostByMemory ? kMostThreads / 32 - copying : kMostByMemory;
+    }
     static constexpr uint32_t shared_bytes(uint32_t warps) { return kQueryBytes + warps * kWarpBytes; }
 };
 
 /// What of a sequence is read: its tokens, less those between the sinks and the window that no query row sees.
 struct Extent {
     int32_t length, first;  // tokens; the first query's position (0 if it lies before the first token)
-    int32_t kept, skipped;  // tokens read before the gap, and the gap's length
+    int32_t kept, skipped;  // tokens read before the gap, and the gap's length, both multiples of 16: parameters are copied by 16 bytes
     __device__ __forceinline__ int32_t visible() const { return length - skipped; }
     __device__ __forceinline__ int32_t token(int32_t at) const { return at < kept ? at : at + skipped; }
 };
@@ -374,8 +378,8 @@ __device__ __forceinline__ Extent extent_of(const AttentionArguments& args, uint
     }
     e.first = max(e.length - static_cast<int32_t>(args.queries), 0);
     const int32_t start = args.window ? max(e.first + 1 - args.window, 0) : 0;
-    e.kept = min(args.sinks, start);
-    e.skipped = start - e.kept;
+    e.kept = min((min(args.sinks, start) + 15) & ~15, start & ~15);
+    e.skipped = (start & ~15) - e.kept;
     return e;
 }
 
@@ -397,6 +401,11 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+/// A rendezvous of the block's first `threads` threads, the warps that compute.
+__device__ __forceinline__ void sync_computing(uint32_t threads) {
+    asm volatile("bar.sync 1, %0;" ::"r"(threads) : "memory");
+}
+
 /// D[16, 8] += A[16, 16] . B[16, 8] in fp16 with fp32 sums.
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                             uint32_t b1) {
@@ -462,7 +471,7 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
 }
 
 template <int D, int G, int NT, bool BF16>
-__global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
+__global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     attention_kernel(const __grid_constant__ AttentionArguments args, uint32_t* status) {
     using E = Element<BF16>;
     using Shape = AttentionShape<D, G, NT>;
@@ -471,12 +480,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     constexpr uint32_t kSteps = NT == 4 ? 1 : 2;      // steps of 16 tokens between looks at the running maximum
     constexpr bool kEights = NT == 1;                 // see `eights` below
     extern __shared__ __align__(16) uint8_t shared[];
+    __shared__ uint64_t barriers[2 * kStages];  // of each stage: it is full; it is free again
+    __shared__ uint32_t bad_pages[kStages];     // whether a stage has places whose page lies outside the cache
     __shared__ uint32_t stop_flag, complete[2];
     __shared__ Cut cuts[2];              // the parts of segments that are cut over blocks: the one this share begins in, ends in
     __shared__ float2 row_stats[kRows];  // reference and sum of each row over the warps
-    const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // The first warps compute, the last one or two copy: keys and values, or one side each.
+    const uint32_t warps = blockDim.x / 32 - args.copying, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
-    const auto memory_of = [&](uint32_t w) { return shared + Shape::kQueryBytes + w * Shape::kWarpBytes; };
+    uint8_t* const ring = shared + Shape::kQueryBytes;
+    const uint32_t stage_bytes = warps * Shape::kStageBytes, value_codes = warps * Shape::kCodeBytes;
 
     // ---- this block's share: units of unit_tokens tokens, sequence by sequence, (kv head, row tile) by (kv head,
     // row tile), cut evenly over the blocks whatever the lengths are. A segment, one sequence's units of one (kv
@@ -519,10 +532,13 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
 
-    uint8_t* const own = memory_of(warp);
-    if (lane == 0)
-        for (uint32_t s = 0; s < kStages; ++s) mbar_init(smem_u32(own + Shape::kBarriers + 16 * s), 1);
-    if (threadIdx.x == 0) stop_flag = cuts[0].parts = cuts[1].parts = 0;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kStages; ++i) {
+            mbar_init(smem_u32(barriers + 2 * i), args.copying);
+            mbar_init(smem_u32(barriers + 2 * i + 1), warps);
+        }
+        stop_flag = cuts[0].parts = cuts[1].parts = 0;
+    }
     fence_mbarrier_init();
     __syncthreads();
     const StallSite site{status, &stop_flag, 0};
@@ -563,81 +579,77 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         return find_piece();
     };
 
-    // ---- copies. Each warp keeps a ring of its own, 32 tokens a stage: tokens that follow each other in a page are one
-    // run, copied in bulk by one thread, codes and parameters of both sides. (Parameters of runs that do not begin and end
-    // on 16 bytes go token by token.) The page of a unit's first run is asked for a unit before it is needed.
-    uint32_t fill_stage = 0, next_page = 0;
     const auto page_at = [&](int32_t place) {
         return args.table ? static_cast<uint32_t>(
                                 __ldg(args.table + b * args.table_stride + args.page.quotient(extent.token(place))))
                           : b;
     };
-    const auto place_of = [&](uint32_t unit) { return static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens); };
-    const auto ask = [&](uint32_t unit) {
-        if (place_of(unit) < extent.visible()) next_page = page_at(place_of(unit));
-    };
-    const auto issue = [&](uint32_t unit) {
-        const int32_t place = place_of(unit);
-        const uint32_t full = smem_u32(own + Shape::kBarriers + 16 * fill_stage);
-        const uint32_t memory_at = smem_u32(own + fill_stage * Shape::kStageBytes);
-        if (elect_one()) {
-            const int32_t count = min(extent.visible() - place, static_cast<int32_t>(kWarpTokens));
-            uint32_t real = 0, bytes = 0, page = next_page;
-            bool single = false;
-#pragma unroll 1
-            for (int32_t i = 0; i < count;) {
-                const uint32_t token = static_cast<uint32_t>(extent.token(place + i));
-                const uint32_t inside = token - args.page.quotient(token) * args.page_size;
-                uint32_t run = min(static_cast<uint32_t>(count - i), args.page_size - inside);
-                if (place + i < extent.kept) run = min(run, static_cast<uint32_t>(extent.kept - place - i));
-                const int32_t then = i + static_cast<int32_t>(run);
-                const uint32_t then_page = then < count ? page_at(place + then) : 0;
-                if (page < args.pages) {
-                    const uint64_t row = (page * args.kv_heads + kv_head) * args.page_size + inside;
-                    const uint32_t to_at = memory_at + i * (D / 2);
-                    bulk_load(to_at, args.codes[0] + row * (D / 2), run * (D / 2), full);
-                    bulk_load(to_at + Shape::kCodeBytes, args.codes[1] + row * (D / 2), run * (D / 2), full);
-                    bytes += run * D;
-                    const uint32_t params_at = memory_at + 2 * Shape::kCodeBytes + i * (kGroups * 4);
-                    const uint64_t params = row * (kGroups * 4);
-                    if (((static_cast<uint32_t>(params) | params_at | run * (kGroups * 4)) & 15u) == 0) {
-                        bulk_load(params_at, args.params[0] + params, run * (kGroups * 4), full);
-                        bulk_load(params_at + Shape::kParamBytes, args.params[1] + params, run * (kGroups * 4), full);
-                        bytes += run * (kGroups * 8);
-                    } else {
-                        single = true;
-#pragma unroll 1
-                        for (uint32_t r = 0; r < run; ++r) {
-                            copy_async<kGroups * 4>(params_at + r * (kGroups * 4), args.params[0] + params + r * (kGroups * 4));
-                            copy_async<kGroups * 4>(params_at + Shape::kParamBytes + r * (kGroups * 4),
-                                                    args.params[1] + params + r * (kGroups * 4));
-                        }
-                    }
-                    real |= (run == 32 ? 0xffffffffu : (1u << run) - 1) << i;
-                } else {
-                    note(status, kBadPage, b, page);
-                }
-                i = then;
-                page = then_page;
-            }
-            *reinterpret_cast<uint32_t*>(own + Shape::kBarriers + 16 * fill_stage + 8) = real;
-            if (single) copy_async_arrive(full);
-            mbar_arrive_expect_tx(full, bytes);
-        }
-        __syncwarp();
-        fill_stage ^= 1;
-    };
-    // A piece's first unit is on its way before the piece before it is merged.
-    const auto start_piece = [&]() {
-        ask(from);
-        issue(from);
-        ask(from + 1);
+    const auto next_stage = [&]() {
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+        parity ^= stage == 0;
     };
 
+    if (warp >= warps) {
+        // ---- copies, by one thread: tokens that follow each other in a page are one run, copied in bulk, codes and
+        // parameters. (Parameters of runs that do not begin and end on 16 bytes go token by token.) The page of the next
+        // run is asked for before the present one is copied.
+        if (!elect_one()) return;
+        const uint32_t side = warp - warps;
+        for (bool more = find_piece(); more; more = next_piece()) {
+            int32_t place = static_cast<int32_t>(from * unit_tokens);
+            uint32_t next_page = page_at(min(place, max(extent.visible() - 1, 0)));
+            for (uint32_t unit = from; unit < to; ++unit, place += unit_tokens) {
+                const uint32_t full = smem_u32(barriers + 2 * stage), memory = smem_u32(ring) + stage * stage_bytes;
+                if (!mbar_wait(full + 8, parity ^ 1, site, kStallFree, unit)) return;
+                const int32_t count = min(extent.visible() - place, static_cast<int32_t>(unit_tokens));
+                uint32_t bytes = 0, bad = 0;
+                bool single = false;
+#pragma unroll 1
+                for (int32_t i = 0; i < count;) {
+                    const uint32_t token = static_cast<uint32_t>(extent.token(place + i));
+                    const uint32_t inside = token - args.page.quotient(token) * args.page_size;
+                    uint32_t run = min(static_cast<uint32_t>(count - i), args.page_size - inside);
+                    if (place + i < extent.kept) run = min(run, static_cast<uint32_t>(extent.kept - place - i));
+                    const uint32_t page = next_page;
+                    const int32_t then = place + i + static_cast<int32_t>(run);
+                    if (then < extent.visible()) next_page = page_at(then);
+                    if (page < args.pages) {
+                        const uint64_t row = (page * args.kv_heads + kv_head) * args.page_size + inside;
+                        const uint32_t param_bytes = run * (kGroups * 4);
+#pragma unroll
+                        for (uint32_t which = 0; which < 2; ++which) {
+                            if (args.copying == 2 && which != side) continue;
+                            bulk_load(memory + which * value_codes + i * (D / 2), args.codes[which] + row * (D / 2), run * (D / 2), full);
+                            bytes += run * (D / 2);
+                            const uint8_t* const params = args.params[which] + row * (kGroups * 4);
+                            const uint32_t params_at = memory + 2 * value_codes + which * warps * Shape::kParamBytes + i * (kGroups * 4);
+                            if (((static_cast<uint32_t>(row * (kGroups * 4)) | params_at | param_bytes) & 15u) == 0) {
+                                bulk_load(params_at, params, param_bytes, full);
+                                bytes += param_bytes;
+                            } else {
+                                single = true;
+#pragma unroll 1
+                                for (uint32_t r = 0; r < param_bytes; r += kGroups * 4)
+                                    copy_async<kGroups * 4>(params_at + r, params + r);
+                            }
+                        }
+                    } else {
+                        bad = 1;
+                        if (side == 0) note(status, kBadPage, b, page);
+                    }
+                    i += static_cast<int32_t>(run);
+                }
+                if (side == 0) bad_pages[stage] = bad;
+                if (single) copy_async_arrive(full);
+                mbar_arrive_expect_tx(full, bytes);
+                next_stage();
+            }
+        }
+        return;
+    }
+
     const uint32_t l4 = lane / 4, c4 = lane % 4;
-    bool more = find_piece();
-    if (more) start_piece();
-    while (more) {
+    for (bool more = find_piece(); more; more = next_piece()) {
         // ---- queries as the second operand of the scores' product: lane (l4, c4) holds row l4 of each 8, in the
         // channel order of the key codes. The tile is scaled by a power of two so that its largest value lies in
         // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second register of each pair carries 1/16 for
@@ -710,7 +722,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 }
             }
         }
-        if constexpr (Shape::kSharedQueries) __syncthreads();
+        if constexpr (Shape::kSharedQueries) sync_computing(warps * 32);
 
         float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {}, lows[kGroups][NT][2] = {};
         float peak[NT][2], sum[NT][2] = {};
@@ -722,24 +734,22 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
         // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
         // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
         const uint32_t own_token = (l4 >> 1) + 4 * (l4 & 1);
-        uint8_t* const wide_keys = own + Shape::kMergeAt;  // (scale, low) * to_log2 of each token and group
+        uint8_t* const wide_keys = ring + kStages * stage_bytes + warp * Shape::kScratchBytes;  // (scale, low) * to_log2 of each token and group
         uint8_t* const wide_values = wide_keys + Shape::kWideBytes;     // (scale * fit, low + 8 * scale)
 
 #pragma unroll 1
         for (uint32_t unit = from; unit < to; ++unit) {
-            if (unit + 1 < to) {
-                issue(unit + 1);
-                ask(unit + 2);
-            }
-            const uint32_t full = smem_u32(own + Shape::kBarriers + 16 * stage);
-            if (live) live = mbar_wait(full, parity, site, kStallCodes, unit);
-            const uint8_t* const keys = own + stage * Shape::kStageBytes;
-            const uint8_t* const values = keys + Shape::kCodeBytes;
-            const uint8_t* const key_params = keys + 2 * Shape::kCodeBytes;
-            const uint8_t* const value_params = key_params + Shape::kParamBytes;
+            const uint32_t full = smem_u32(barriers + 2 * stage);
+            if (live) live = mbar_wait(full, parity, site, kStallFull, unit);
+            const uint8_t* const keys = ring + stage * stage_bytes + warp * Shape::kCodeBytes;
+            const uint8_t* const values = keys + value_codes;
+            const uint8_t* const key_params = ring + stage * stage_bytes + 2 * value_codes + warp * Shape::kParamBytes;
+            const uint8_t* const value_params = key_params + warps * Shape::kParamBytes;
             // Which of the 32 tokens are there, and whether some row may not see some token (they rise from place to place).
-            const uint32_t real = *reinterpret_cast<const uint32_t*>(own + Shape::kBarriers + 16 * stage + 8);
-            const int32_t place = place_of(unit);
+            const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens), here = extent.visible() - place;
+            uint32_t real = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1;
+            if (bad_pages[stage])
+                real &= __ballot_sync(0xffffffffu, static_cast<int32_t>(lane) < here && page_at(place + lane) < args.pages);
             const bool is_masked = real != 0xffffffffu || extent.token(place + 31) > extent.first ||
                                    (args.window && extent.token(place + 31) >= args.sinks &&
                                     extent.token(place) <= extent.length - 1 - args.window);
@@ -1004,12 +1014,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                         }
                 }
             }
-            __syncwarp();  // every lane is done with the stage, which is filled next, and with the wide parameters
-            stage ^= 1;
-            parity ^= stage == 0;
+            __syncwarp();  // every lane is done with the stage and with the wide parameters
+            if (unit + 1 == to) break;  // the last stage is given back when the merge is done with it
+            if (lane == 0) mbar_arrive(full + 8);
+            next_stage();
         }
 
         // ---- the warps' parts of the piece meet in shared memory
+        uint8_t* const merge_memory = Shape::kMergeInRing ? ring + stage * stage_bytes : ring + kStages * stage_bytes;
+        constexpr uint32_t merge_pitch = Shape::kMergeInRing ? Shape::kStageBytes : Shape::kScratchBytes;
+        sync_computing(warps * 32);  // the stage is every warp's
         Cut piece{b, kv_head, first_row, from == 0 && to == units_of(cost) ? 0u : 1u, 0};
         uint32_t which = 0;
         if (piece.parts) {
@@ -1018,10 +1032,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             piece.parts = block_of(first_unit + units_of(cost) - 1) - piece.owner + 1;
             which = piece.owner == blockIdx.x;
         }
-        more = next_piece();
-        if (more) start_piece();
         {
-            float* const merged = reinterpret_cast<float*>(own + Shape::kMergeAt);
+            float* const merged = reinterpret_cast<float*>(merge_memory + warp * merge_pitch);
             float* const stats = merged + kRows * kPitch;
             const float unfit = power_of_two(254 - min(kFitBiased - top, 254));
 #pragma unroll
@@ -1056,12 +1068,11 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                     }
                 }
         }
-        __syncthreads();
+        sync_computing(warps * 32);
         const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
-        uint8_t* const rings = memory_of(0) + Shape::kMergeAt;
         // A warp for each row: the warps' shares of it, left in the place of their references.
         for (uint32_t row = warp; row < rows_here; row += warps) {
-            float2* const its = reinterpret_cast<float2*>(rings + min(lane, warps - 1) * Shape::kWarpBytes + kRows * kPitch * 4) + row;
+            float2* const its = reinterpret_cast<float2*>(merge_memory + min(lane, warps - 1) * merge_pitch + kRows * kPitch * 4) + row;
             const float2 stat = lane < warps ? *its : make_float2(-INFINITY, 0.0f);
             float m = stat.x;
 #pragma unroll
@@ -1073,7 +1084,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             if (lane < warps) its->x = factor;
             if (lane == 0) row_stats[row] = make_float2(m, s);
         }
-        __syncthreads();
+        sync_computing(warps * 32);
         // A part of a segment that is cut over blocks: the block its first unit lies in keeps it in its second place, the others in
         // their first. Parts are handed in together at the end.
         float* const part = args.partials + (2 * blockIdx.x + which) * static_cast<size_t>(kPartialFloats);
@@ -1083,7 +1094,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
             for (uint32_t w = 0; w < warps; ++w) {
-                const float* const its = reinterpret_cast<const float*>(rings + w * Shape::kWarpBytes);
+                const float* const its = reinterpret_cast<const float*>(merge_memory + w * merge_pitch);
                 const float factor = its[kRows * kPitch + 2 * row];
                 const float4 z = *reinterpret_cast<const float4*>(its + row * kPitch + d);
                 y = make_float4(fmaf(z.x, factor, y.x), fmaf(z.y, factor, y.y), fmaf(z.z, factor, y.z), fmaf(z.w, factor, y.w));
@@ -1095,12 +1106,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
                 if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
             }
         }
-        __syncthreads();
+        // Copies to where the merged rows lay come by another way than these reads.
+        fence_proxy_async_shared();
+        sync_computing(warps * 32);
+        if (lane == 0) mbar_arrive(smem_u32(barriers + 2 * stage + 1));
+        next_stage();
     }
 
     // ---- the parts of segments that are cut over blocks: the block that comes last to one adds them up, always in the same
     // order, and leaves the counter at zero.
-    __syncthreads();
+    sync_computing(warps * 32);
     if (threadIdx.x == 0) {
         complete[0] = complete[1] = 0;
         if (cuts[0].parts || cuts[1].parts) {
@@ -1118,7 +1133,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
             __threadfence();
         }
     }
-    __syncthreads();
+    sync_computing(warps * 32);
     for (uint32_t c = 0; c < 2; ++c) {
         if (!complete[c]) continue;
         const Cut piece = cuts[c];
@@ -1161,7 +1176,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostWarps * 32, 1)
     // After a wait that gave up, copies may still be on their way: give them a while before the block's memory goes.
     if (stop_flag)
         for (uint32_t k = 0; k < 2 * kStages; ++k)
-            for (uint32_t i = 0; i < 100 && !mbar_try_wait(smem_u32(own + Shape::kBarriers + 16 * (k / 2)), k & 1); ++i) {
+            for (uint32_t i = 0; i < 100 && !mbar_try_wait(smem_u32(barriers + k / 2 * 2), k & 1); ++i) {
             }
 }
 
@@ -1302,14 +1317,15 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     using Shape = cache::AttentionShape<D, G, NT>;
     const auto kernel = cache::attention_kernel<D, G, NT, BF16>;
     uint32_t limit = 0;
-    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(Shape::kMostWarps), &limit);
+    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(Shape::most_warps(1)), &limit);
     if (admitted != FK_OK) return admitted;
     args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
-    const uint32_t half = Shape::kMostWarps / 2;
-    const bool whole = segments < 2ull * facts.sm_count;
-    const uint32_t warps = whole ? Shape::kMostWarps : half;
-    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (whole ? 1 : 2);
+    const bool alone = segments < 2ull * facts.sm_count;
+    args.copying = alone ? 2 : 1;
+    const uint32_t half = Shape::kMostThreads / 64 - 1;
+    const uint32_t warps = alone ? Shape::most_warps(2) : half < Shape::kMostByMemory / 2 ? half : Shape::kMostByMemory / 2;
+    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (alone ? 1 : 2);
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
     args.least_units = 3;
     args.segment_cost = 1;
@@ -1318,7 +1334,7 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
         return fk_fail(FK_ERR_SHAPE, "%u sequences of up to %llu tokens on %u heads are more than a launch counts", args.batch,
                        static_cast<unsigned long long>(args.table_pages) * args.page_size, args.kv_heads);
     const uint32_t grid = most_units < resident ? static_cast<uint32_t>(most_units) : resident;
-    kernel<<<grid, warps * 32, Shape::shared_bytes(warps), static_cast<cudaStream_t>(stream)>>>(args, device_status);
+    kernel<<<grid, (warps + args.copying) * 32, Shape::shared_bytes(warps), static_cast<cudaStream_t>(stream)>>>(args, device_status);
     FK_CUDA(cudaGetLastError());
     return FK_OK;
 }
@@ -1350,7 +1366,7 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
     if (table && table_pages == 0) return fk_fail(FK_ERR_SHAPE, "the page table has no columns");
     const uint32_t columns = table ? table_pages : 1;
     const uint64_t capacity = static_cast<uint64_t>(columns) * cache->page_size;
-    if (capacity >= (1ull << 31))
+    if (capacity >= 0x7ffff000ull)
         return fk_fail(FK_ERR_SHAPE, "%u pages of %u tokens are more than 2^31 - 1 tokens a sequence", columns,
                        cache->page_size);
     DeviceFacts facts;
