@@ -162,93 +162,128 @@ __device__ __forceinline__ uint32_t value_word(uint32_t block) {
     return (block & 7u) * (D / 64) + (block >> 3);
 }
 
-// One lane holds 8 channels (16 bytes) of a row, D / 8 lanes a row; a group's smallest and largest value are
-// found together, as the minimum of packed pairs (x, -x) over its G / 8 lanes.
+/// Codes and parameters of 8 channels (`words`, 16 bytes of a row) whose group lies in G / 8 neighbouring lanes. All lanes of a warp
+/// take part; where `kept` is false the result is not used.
+template <int G, bool BF16>
+struct Quantised {
+    uint32_t word, params;
+};
+
+template <int G, bool BF16>
+__device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
+    using E = Element<BF16>;
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+    // {smallest, -largest} of the group together, NaN if it holds one.
+    uint32_t least = words[0], most = words[0] ^ 0x80008000u;
+#pragma unroll
+    for (uint32_t i = 1; i < 4; ++i) {
+        least = E::min_nan(least, words[i]);
+        most = E::min_nan(most, words[i] ^ 0x80008000u);
+    }
+    uint32_t ends = E::min_nan(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
+#pragma unroll
+    for (uint32_t mask = 1; mask < G / 8; mask *= 2) ends = E::min_nan(ends, __shfl_xor_sync(0xffffffffu, ends, mask));
+    const float low = E::low(ends), high = -E::high(ends);
+    // Half the span (the span itself may pass fp32's range), and what its rounding left out, exactly (the error of a sum is
+    // a float).
+    const float a = 0.5f * high, b = 0.5f * low;
+    const float half_span = a - b;
+    const float b_part = half_span - a;
+    const float lost = (a - (half_span - b_part)) - (b + b_part);
+    const bool finite = half_span < __uint_as_float(0x7f800000u);  // false for NaN as well
+    // The scale: near half_span / 7.5, then made exact, since 7.5 times a value of the type is.
+    const auto fits = [&](uint32_t bits) {
+        const float product = 7.5f * E::low(bits);
+        return product < half_span || (product == half_span && lost >= 0.0f);
+    };
+    uint32_t scale_bits = finite ? E::truncate(half_span * (1.0f / 7.5f)) : 0u;
+    if (finite) {
+        if (fits(scale_bits + 1)) ++scale_bits;
+        else if (scale_bits && !fits(scale_bits)) --scale_bits;
+    }
+    const float scale = E::low(scale_bits);
+    // Tiny spans are lifted by 2^100 so that 1 / scale stays finite, huge ones halved so that x - low does (the products are
+    // exact). Nothing is coded where the scale is zero: step and reach are then such that every code is 0.
+    const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f && scale > 0.0f ? 0x1p100f : 1.0f;
+    const bool coded = scale > 0.0f;
+    const float step = coded ? scale * lift : 1.0f, origin = -low * lift;
+    // A guess that is never above the code and at most one below: the quotient's error is under 16 * 2^-22. The remainder t -
+    // guess * step is exact, and a half step or more of it is one more.
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+    const float2 lift2 = make_float2(lift, lift), origin2 = make_float2(origin, origin);
+    const float inverse = coded ? __frcp_rn(step) : 0.0f, half_step = 0.5f * step;
+    const float2 inverse2 = make_float2(inverse, inverse), under2 = make_float2(kMagic, kMagic);
+    const float2 bias2 = make_float2(-0x1p-17f, -0x1p-17f), minus_magic2 = make_float2(-kMagic, -kMagic);
+    const float2 minus_step2 = make_float2(-step, -step);
+    float2 code[4];
+    float nearest = -1.0f;  // the largest remainder
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const float2 value = make_float2(E::low(words[i]), E::high(words[i]));
+        const float2 t = __ffma2_rn(value, lift2, origin2);
+        const float2 guess = __fadd2_rn(__fadd2_rn(__ffma2_rn(t, inverse2, bias2), under2), minus_magic2);
+        const float2 rest = __ffma2_rn(guess, minus_step2, t);
+        nearest = fmaxf(nearest, fmaxf(rest.x, rest.y));
+        code[i] = __fadd2_rn(guess, make_float2(rest.x >= half_step ? 1.0f : 0.0f, rest.y >= half_step ? 1.0f : 0.0f));
+    }
+    // Where a remainder is a half step to the bit, t's own rounding may have made it one (of a value that vanishes beside
+    // the group's smallest), and where the scale was cut short (of a span of a few subnormals) codes pass 15.
+    if (coded && (nearest == half_step || half_span > 7.75f * scale)) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const float lifted = ((i & 1u) ? E::high(words[i / 2]) : E::low(words[i / 2])) * lift;
+            const float t = lifted + origin, o_part = t - lifted;
+            const float t_lost = (lifted - (t - o_part)) + (origin - o_part);
+            float& c = (i & 1u) ? code[i / 2].y : code[i / 2].x;
+            const float guess = fminf(rintf(t * inverse), 15.0f);
+            const float rest = __fmaf_rn(guess, -step, t);
+            if ((rest - half_step) + t_lost >= 0.0f) c = guess + 1.0f;
+            else if ((rest + half_step) + t_lost < 0.0f) c = guess - 1.0f;
+            else c = guess;
+            c = fminf(c, 15.0f);
+        }
+    }
+    // Four codes make a whole number under 2^16, which a sum with 2^23 leaves in the low bits.
+    const float2 shift2 = make_float2(256.0f, 256.0f);
+    const float2 front = __ffma2_rn(code[1], shift2, code[0]), back = __ffma2_rn(code[3], shift2, code[2]);
+    const uint32_t first = __float_as_uint(__fmaf_rn(front.y, 16.0f, front.x) + 8388608.0f);
+    const uint32_t last = __float_as_uint(__fmaf_rn(back.y, 16.0f, back.x) + 8388608.0f);
+    Quantised<G, BF16> result;
+    result.word = coded ? __byte_perm(first, last, 0x5410) : 0u;
+    result.params = scale_bits | ((finite ? ends & 0xffffu : E::kNaN) << 16);
+    return result;
+}
+
+// One lane holds 8 channels (16 bytes) of a row's key and of its value, D / 8 lanes a row.
 template <int D, int G, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constant__ RowArguments args,
                                                             uint32_t* status) {
-    using E = Element<BF16>;
     constexpr uint32_t kLanes = D / 8;
-    const uint32_t which = blockIdx.y;
     const uint32_t lane = threadIdx.x & 31u, block = threadIdx.x % kLanes;
     const uint32_t step = gridDim.x * (kRowThreads / kLanes);
     for (uint32_t first = blockIdx.x * (kRowThreads / kLanes); first < args.rows; first += step) {
         const uint32_t index = first + threadIdx.x / kLanes;
-        uint4 x = make_uint4(0, 0, 0, 0);
+        uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         uint64_t row = 0;
         bool kept = index < args.rows;
         if (kept) {
             const uint32_t token = args.heads.quotient(index), head = index - token * args.heads.divisor;
+#pragma unroll
+            for (uint32_t which = 0; which < 2; ++which)
+                x[which] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(args.tensor[which]) +
+                                                                 token * args.token_stride[which] +
+                                                                 head * args.head_stride[which]) +
+                                  block);
             kept = cache_row(args, token, head, row, status);
-            if (kept)
-                x = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(args.tensor[which]) +
-                                                          token * args.token_stride[which] +
-                                                          head * args.head_stride[which]) +
-                           block);
         }
-        const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-        // {smallest, -largest} of the group, NaN if it holds one.
-        uint32_t least = words[0], most = words[0] ^ 0x80008000u;
 #pragma unroll
-        for (uint32_t i = 1; i < 4; ++i) {
-            least = E::min_nan(least, words[i]);
-            most = E::min_nan(most, words[i] ^ 0x80008000u);
-        }
-        uint32_t ends = E::min_nan(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
-#pragma unroll
-        for (uint32_t mask = 1; mask < G / 8; mask *= 2)
-            ends = E::min_nan(ends, __shfl_xor_sync(0xffffffffu, ends, mask));
-        const float low = E::low(ends), high = -E::high(ends);
-        // Half the span: the span itself may pass fp32's range. `lost` is what its rounding left out, exactly
-        // (the error of a sum is a float).
-        const float a = 0.5f * high, b = 0.5f * low;
-        const float half_span = a - b;
-        const float b_part = half_span - a;
-        const float lost = (a - (half_span - b_part)) - (b + b_part);
-        const bool finite = half_span < __uint_as_float(0x7f800000u);  // false for NaN as well
-        uint32_t scale_bits = finite ? E::truncate(__fdiv_rn(half_span, 7.5f)) : 0u;
-        float scale = E::low(scale_bits);
-        // The quotient's rounding may have carried it over a value of the type: 7.5 * scale is exact.
-        if (finite && (7.5f * scale > half_span || (7.5f * scale == half_span && lost < 0.0f))) {
-            --scale_bits;
-            scale = E::low(scale_bits);
-        }
-        const uint32_t low_bits = finite ? (ends & 0xffffu) : E::kNaN;
-        // Tiny spans are lifted by 2^100 so that 1 / scale stays finite, huge ones halved so that x - low does
-        // (the products are exact).
-        const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f && scale > 0.0f ? 0x1p100f : 1.0f;
-        const float step_size = scale * lift, origin = -low * lift;
-        const bool coded = finite && scale > 0.0f;
-        const float inverse = coded ? __fdiv_rn(1.0f, step_size) : 0.0f;
-        const float half_step = coded ? 0.5f * step_size : __uint_as_float(0x7f800000u);
-        uint32_t word = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            const float value = (i & 1u) ? E::high(words[i / 2]) : E::low(words[i / 2]);
-            const float lifted = value * lift;
-            const float t = coded ? lifted + origin : 0.0f;
-            // What rounding left out of t, exactly.
-            const float o_part = t - lifted;
-            const float t_lost = coded ? (lifted - (t - o_part)) + (origin - o_part) : 0.0f;
-            const float guess = fminf(rintf(t * inverse), 15.0f);
-            // Where t stands against the guess's borders: the remainder is exact.
-            const float r = __fmaf_rn(-guess, step_size, t);
-            int code = static_cast<int>(guess);
-            if ((r - half_step) + t_lost >= 0.0f) ++code;
-            else if ((r + half_step) + t_lost < 0.0f) --code;
-            code = min(max(code, 0), 15);
-            word |= static_cast<uint32_t>(code) << (4 * i);
-        }
-        uint32_t at;
-        if (which == 0) {
-            at = key_word<D>(block);
-        } else {
-            word = transpose_nibbles(word, lane);
-            at = value_word<D>(block);
-        }
-        if (kept) {
-            args.codes[which][row * (D / 8) + at] = word;
-            if (block % (G / 8) == 0) args.params[which][row * (D / G) + block / (G / 8)] = scale_bits | (low_bits << 16);
+        for (uint32_t which = 0; which < 2; ++which) {
+            Quantised<G, BF16> q = quantise<G, BF16>(x[which]);
+            if (which == 1) q.word = transpose_nibbles(q.word, lane);
+            if (kept) {
+                args.codes[which][row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))] = q.word;
+                if (block % (G / 8) == 0) args.params[which][row * (D / G) + block / (G / 8)] = q.params;
+            }
         }
     }
 }
@@ -260,36 +295,43 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant
                                                            uint32_t* status) {
     using E = Element<BF16>;
     constexpr uint32_t kLanes = D / 8;
-    const uint32_t which = blockIdx.y;
     const uint32_t lane = threadIdx.x & 31u, block = threadIdx.x % kLanes;
     const uint32_t step = gridDim.x * (kRowThreads / kLanes);
     for (uint32_t first = blockIdx.x * (kRowThreads / kLanes); first < args.rows; first += step) {
         const uint32_t index = first + threadIdx.x / kLanes;
         const bool inside = index < args.rows;
-        uint32_t word = 0, pair = 0;
-        uint4* destination = nullptr;
+        uint32_t word[2] = {}, pair[2] = {}, token = 0, head = 0;
         bool kept = false;
         if (inside) {
-            const uint32_t token = args.heads.quotient(index), head = index - token * args.heads.divisor;
+            token = args.heads.quotient(index);
+            head = index - token * args.heads.divisor;
             uint64_t row = 0;
             kept = cache_row(args, token, head, row, status);
             if (kept) {
-                word = args.codes[which][row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))];
-                pair = args.params[which][row * (D / G) + block / (G / 8)];
-            }
-            destination = reinterpret_cast<uint4*>(static_cast<uint8_t*>(const_cast<void*>(args.tensor[which])) +
-                                                   token * args.token_stride[which] + head * args.head_stride[which]) +
-                          block;
-        }
-        if (which == 1) word = transpose_nibbles(word, lane);
-        const uint32_t scale = __byte_perm(pair, 0, 0x1010), low = __byte_perm(pair, 0, 0x3232);
-        uint32_t y[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t codes = ((word >> (8 * i)) & 0xfu) | ((word >> (8 * i) << 12) & 0xf0000u);
-            y[i] = E::fma(E::minus_magic(codes | E::kMagic), scale, low);
+                for (uint32_t which = 0; which < 2; ++which) {
+                    word[which] = __ldcs(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
+                    pair[which] = __ldcs(args.params[which] + row * (D / G) + block / (G / 8));
+                }
+            }
         }
-        if (inside && (kept || args.clear_skipped)) *destination = kept ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(0, 0, 0, 0);
+        word[1] = transpose_nibbles(word[1], lane);
+#pragma unroll
+        for (uint32_t which = 0; which < 2; ++which) {
+            const uint32_t scale = __byte_perm(pair[which], 0, 0x1010), low = __byte_perm(pair[which], 0, 0x3232);
+            uint32_t y[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t codes = ((word[which] >> (8 * i)) & 0xfu) | ((word[which] >> (8 * i) << 12) & 0xf0000u);
+                y[i] = E::fma(E::minus_magic(codes | E::kMagic), scale, low);
+            }
+            uint4* const destination =
+                reinterpret_cast<uint4*>(static_cast<uint8_t*>(const_cast<void*>(args.tensor[which])) +
+                                         token * args.token_stride[which] + head * args.head_stride[which]) +
+                block;
+            if (inside && (kept || args.clear_skipped))
+                *destination = kept ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(0, 0, 0, 0);
+        }
     }
 }
 
@@ -1277,8 +1319,8 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
     return for_cache(cache, [&](auto dim, auto group, auto bf16) {
         const uint32_t rows_a_block = cache::kRowThreads / (dim / 8);
         const uint32_t blocks = (args.rows + rows_a_block - 1) / rows_a_block;
-        const uint32_t most = static_cast<uint32_t>(facts.sm_count) * 4;  // half of what fits; k and v are grid rows
-        const dim3 grid(blocks < most ? blocks : most, 2);
+        const uint32_t most = static_cast<uint32_t>(facts.sm_count) * 32;  // some rounds of what is resident at a time
+        const uint32_t grid = blocks < most ? blocks : most;
         if (write)
             cache::write_kernel<dim, group, bf16>
                 <<<grid, cache::kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(args, device_status);
