@@ -2,6 +2,8 @@
 // attention of a sequence's newest tokens over its rows. No counterpart in the reference, whose attention
 // reads whole bf16 planes (examples/src/flash_forward.rs:151-158); the format is stated in the header.
 
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -162,6 +164,17 @@ __device__ __forceinline__ uint32_t value_word(uint32_t block) {
     return (block & 7u) * (D / 64) + (block >> 3);
 }
 
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float one_if_ge(float a, float b) {
+    float y;
+    asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 /// Codes and parameters of 8 channels (`words`, 16 bytes of a row) whose group lies in G / 8 neighbouring lanes. All lanes of a warp
 /// take part; where `kept` is false the result is not used.
 template <int G, bool BF16>
@@ -191,27 +204,22 @@ __device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
     const float b_part = half_span - a;
     const float lost = (a - (half_span - b_part)) - (b + b_part);
     const bool finite = half_span < __uint_as_float(0x7f800000u);  // false for NaN as well
-    // The scale: near half_span / 7.5, then made exact, since 7.5 times a value of the type is.
-    const auto fits = [&](uint32_t bits) {
-        const float product = 7.5f * E::low(bits);
-        return product < half_span || (product == half_span && lost >= 0.0f);
-    };
-    uint32_t scale_bits = finite ? E::truncate(half_span * (1.0f / 7.5f)) : 0u;
-    if (finite) {
-        if (fits(scale_bits + 1)) ++scale_bits;
-        else if (scale_bits && !fits(scale_bits)) --scale_bits;
-    }
+    // The scale: half_span / 7.5 with a little added, cut to the type, is right or one too large, which 7.5 times it, exact,
+    // tells.
+    uint32_t scale_bits = finite ? E::truncate(half_span * (0x1.111112p-3f * (1.0f + 0x1p-21f))) : 0u;
+    const float product = 7.5f * E::low(scale_bits);
+    if (product > half_span || (product == half_span && lost < 0.0f)) --scale_bits;
     const float scale = E::low(scale_bits);
     // Tiny spans are lifted by 2^100 so that 1 / scale stays finite, huge ones halved so that x - low does (the products are
     // exact). Nothing is coded where the scale is zero: step and reach are then such that every code is 0.
     const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f && scale > 0.0f ? 0x1p100f : 1.0f;
     const bool coded = scale > 0.0f;
     const float step = coded ? scale * lift : 1.0f, origin = -low * lift;
-    // A guess that is never above the code and at most one below: the quotient's error is under 16 * 2^-22. The remainder t -
+    // A guess that is never above the code and at most one below: the quotient's error is under 2^-18. The remainder t -
     // guess * step is exact, and a half step or more of it is one more.
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
     const float2 lift2 = make_float2(lift, lift), origin2 = make_float2(origin, origin);
-    const float inverse = coded ? __frcp_rn(step) : 0.0f, half_step = 0.5f * step;
+    const float inverse = coded ? rcp_approx(step) : 0.0f, half_step = 0.5f * step;
     const float2 inverse2 = make_float2(inverse, inverse), under2 = make_float2(kMagic, kMagic);
     const float2 bias2 = make_float2(-0x1p-17f, -0x1p-17f), minus_magic2 = make_float2(-kMagic, -kMagic);
     const float2 minus_step2 = make_float2(-step, -step);
@@ -224,23 +232,33 @@ __device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
         const float2 guess = __fadd2_rn(__fadd2_rn(__ffma2_rn(t, inverse2, bias2), under2), minus_magic2);
         const float2 rest = __ffma2_rn(guess, minus_step2, t);
         nearest = fmaxf(nearest, fmaxf(rest.x, rest.y));
-        code[i] = __fadd2_rn(guess, make_float2(rest.x >= half_step ? 1.0f : 0.0f, rest.y >= half_step ? 1.0f : 0.0f));
+        code[i] = __fadd2_rn(guess, make_float2(one_if_ge(rest.x, half_step), one_if_ge(rest.y, half_step)));
     }
-    // Where a remainder is a half step to the bit, t's own rounding may have made it one (of a value that vanishes beside
-    // the group's smallest), and where the scale was cut short (of a span of a few subnormals) codes pass 15.
-    if (coded && (nearest == half_step || half_span > 7.75f * scale)) {
+    // Where a remainder is a half step to the bit, t's own rounding may have made it one. That takes a value (or a smallest
+    // value) that is not zero and under 2^-9 of the span: others' lowest bits lie above t's. And where the scale was cut short (of
+    // a span of a few subnormals) codes pass 15.
+    if (coded && (nearest == half_step || half_span >= 7.75f * scale)) {
+        const float tiny = half_span * 0x1p-8f;
+        bool doubtful = half_span >= 7.75f * scale || (fabsf(low) < tiny && low != 0.0f);
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            const float lifted = ((i & 1u) ? E::high(words[i / 2]) : E::low(words[i / 2])) * lift;
+        for (uint32_t i = 0; i < 4; ++i) {
+            const float u = fabsf(E::low(words[i])), v = fabsf(E::high(words[i]));
+            doubtful |= (u < tiny && u != 0.0f) || (v < tiny && v != 0.0f);
+        }
+#pragma unroll 1
+        for (uint32_t i = 0; doubtful && i < 8; ++i) {
+            const uint32_t pair = i < 4 ? (i < 2 ? words[0] : words[1]) : (i < 6 ? words[2] : words[3]);
+            const float lifted = ((i & 1u) ? E::high(pair) : E::low(pair)) * lift;
             const float t = lifted + origin, o_part = t - lifted;
             const float t_lost = (lifted - (t - o_part)) + (origin - o_part);
-            float& c = (i & 1u) ? code[i / 2].y : code[i / 2].x;
-            const float guess = fminf(rintf(t * inverse), 15.0f);
-            const float rest = __fmaf_rn(guess, -step, t);
-            if ((rest - half_step) + t_lost >= 0.0f) c = guess + 1.0f;
-            else if ((rest + half_step) + t_lost < 0.0f) c = guess - 1.0f;
-            else c = guess;
+            float c = fminf(rintf(t * inverse), 15.0f);
+            const float rest = __fmaf_rn(c, -step, t);
+            if ((rest - half_step) + t_lost >= 0.0f) c += 1.0f;
+            else if ((rest + half_step) + t_lost < 0.0f) c -= 1.0f;
             c = fminf(c, 15.0f);
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (k == i) ((k & 1u) ? code[k / 2].y : code[k / 2].x) = c;
         }
     }
     // Four codes make a whole number under 2^16, which a sum with 2^23 leaves in the low bits.
@@ -254,83 +272,85 @@ __device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
     return result;
 }
 
-// One lane holds 8 channels (16 bytes) of a row's key and of its value, D / 8 lanes a row.
-template <int D, int G, bool BF16>
+// One lane holds 8 channels (16 bytes) of a row's key and of its value, D / 8 lanes a row, ROWS rows of its own at a time: slots,
+// then rows, of all of them are on their way before the first is worked on.
+template <int D, int G, int ROWS, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constant__ RowArguments args,
                                                             uint32_t* status) {
-    constexpr uint32_t kLanes = D / 8;
+    constexpr uint32_t kLanes = D / 8, kAtATime = kRowThreads / kLanes;
     const uint32_t lane = threadIdx.x & 31u, block = threadIdx.x % kLanes;
-    const uint32_t step = gridDim.x * (kRowThreads / kLanes);
-    for (uint32_t first = blockIdx.x * (kRowThreads / kLanes); first < args.rows; first += step) {
-        const uint32_t index = first + threadIdx.x / kLanes;
-        uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-        uint64_t row = 0;
-        bool kept = index < args.rows;
-        if (kept) {
-            const uint32_t token = args.heads.quotient(index), head = index - token * args.heads.divisor;
+    const uint32_t first = blockIdx.x * (kAtATime * ROWS) + threadIdx.x / kLanes;
+    uint4 x[ROWS][2];
+    uint64_t row[ROWS];
+    bool kept[ROWS];
 #pragma unroll
-            for (uint32_t which = 0; which < 2; ++which)
-                x[which] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(args.tensor[which]) +
-                                                                 token * args.token_stride[which] +
-                                                                 head * args.head_stride[which]) +
-                                  block);
-            kept = cache_row(args, token, head, row, status);
-        }
+    for (uint32_t r = 0; r < ROWS; ++r) {
+        const uint32_t index = min(first + r * kAtATime, args.rows - 1);
+        const uint32_t token = args.heads.quotient(index), head = index - token * args.heads.divisor;
+#pragma unroll
+        for (uint32_t which = 0; which < 2; ++which)
+            x[r][which] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(args.tensor[which]) +
+                                                                token * args.token_stride[which] +
+                                                                head * args.head_stride[which]) +
+                                 block);
+        kept[r] = first + r * kAtATime < args.rows && cache_row(args, token, head, row[r], status);
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < ROWS; ++r)
 #pragma unroll
         for (uint32_t which = 0; which < 2; ++which) {
-            Quantised<G, BF16> q = quantise<G, BF16>(x[which]);
+            Quantised<G, BF16> q = quantise<G, BF16>(x[r][which]);
             if (which == 1) q.word = transpose_nibbles(q.word, lane);
-            if (kept) {
-                args.codes[which][row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))] = q.word;
-                if (block % (G / 8) == 0) args.params[which][row * (D / G) + block / (G / 8)] = q.params;
+            if (kept[r]) {
+                args.codes[which][row[r] * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))] = q.word;
+                if (block % (G / 8) == 0) args.params[which][row[r] * (D / G) + block / (G / 8)] = q.params;
             }
         }
-    }
 }
 
 // The same lanes the other way: a code in the low mantissa bits of a power of two, less that power, is exact,
 // and one fused multiply-add in the cache's type rounds low + code * scale once.
-template <int D, int G, bool BF16>
+template <int D, int G, int ROWS, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant__ RowArguments args,
                                                            uint32_t* status) {
     using E = Element<BF16>;
-    constexpr uint32_t kLanes = D / 8;
+    constexpr uint32_t kLanes = D / 8, kAtATime = kRowThreads / kLanes;
     const uint32_t lane = threadIdx.x & 31u, block = threadIdx.x % kLanes;
-    const uint32_t step = gridDim.x * (kRowThreads / kLanes);
-    for (uint32_t first = blockIdx.x * (kRowThreads / kLanes); first < args.rows; first += step) {
-        const uint32_t index = first + threadIdx.x / kLanes;
-        const bool inside = index < args.rows;
-        uint32_t word[2] = {}, pair[2] = {}, token = 0, head = 0;
-        bool kept = false;
-        if (inside) {
-            token = args.heads.quotient(index);
-            head = index - token * args.heads.divisor;
-            uint64_t row = 0;
-            kept = cache_row(args, token, head, row, status);
-            if (kept) {
+    const uint32_t first = blockIdx.x * (kAtATime * ROWS) + threadIdx.x / kLanes;
+    uint32_t word[ROWS][2], pair[ROWS][2];
+    bool kept[ROWS];
 #pragma unroll
-                for (uint32_t which = 0; which < 2; ++which) {
-                    word[which] = __ldcs(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
-                    pair[which] = __ldcs(args.params[which] + row * (D / G) + block / (G / 8));
-                }
-            }
-        }
-        word[1] = transpose_nibbles(word[1], lane);
+    for (uint32_t r = 0; r < ROWS; ++r) {
+        const uint32_t index = min(first + r * kAtATime, args.rows - 1);
+        const uint32_t token = args.heads.quotient(index), head = index - token * args.heads.divisor;
+        uint64_t row = 0;
+        kept[r] = cache_row(args, token, head, row, status);
+        if (!kept[r]) row = 0;
 #pragma unroll
         for (uint32_t which = 0; which < 2; ++which) {
-            const uint32_t scale = __byte_perm(pair[which], 0, 0x1010), low = __byte_perm(pair[which], 0, 0x3232);
+            word[r][which] = __ldcs(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
+            pair[r][which] = __ldcs(args.params[which] + row * (D / G) + block / (G / 8));
+        }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < ROWS; ++r) {
+        const uint32_t index = first + r * kAtATime;
+        const uint32_t token = args.heads.quotient(index), head = index - token * args.heads.divisor;
+        word[r][1] = transpose_nibbles(word[r][1], lane);
+#pragma unroll
+        for (uint32_t which = 0; which < 2; ++which) {
+            const uint32_t scale = __byte_perm(pair[r][which], 0, 0x1010), low = __byte_perm(pair[r][which], 0, 0x3232);
             uint32_t y[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t codes = ((word[which] >> (8 * i)) & 0xfu) | ((word[which] >> (8 * i) << 12) & 0xf0000u);
-                y[i] = E::fma(E::minus_magic(codes | E::kMagic), scale, low);
+                const uint32_t codes = ((word[r][which] >> (8 * i)) & 0xfu) | ((word[r][which] >> (8 * i) << 12) & 0xf0000u);
+                y[i] = kept[r] ? E::fma(E::minus_magic(codes | E::kMagic), scale, low) : 0u;
             }
-            uint4* const destination =
-                reinterpret_cast<uint4*>(static_cast<uint8_t*>(const_cast<void*>(args.tensor[which])) +
-                                         token * args.token_stride[which] + head * args.head_stride[which]) +
-                block;
-            if (inside && (kept || args.clear_skipped))
-                *destination = kept ? make_uint4(y[0], y[1], y[2], y[3]) : make_uint4(0, 0, 0, 0);
+            if (index < args.rows && (kept[r] || args.clear_skipped))
+                __stcs(reinterpret_cast<uint4*>(static_cast<uint8_t*>(const_cast<void*>(args.tensor[which])) +
+                                                token * args.token_stride[which] + head * args.head_stride[which]) +
+                           block,
+                       make_uint4(y[0], y[1], y[2], y[3]));
         }
     }
 }
@@ -1317,16 +1337,24 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
     args.page = cache::Divider(cache->page_size);
     args.clear_skipped = clear_skipped != 0;
     return for_cache(cache, [&](auto dim, auto group, auto bf16) {
-        const uint32_t rows_a_block = cache::kRowThreads / (dim / 8);
-        const uint32_t blocks = (args.rows + rows_a_block - 1) / rows_a_block;
-        const uint32_t most = static_cast<uint32_t>(facts.sm_count) * 32;  // some rounds of what is resident at a time
-        const uint32_t grid = blocks < most ? blocks : most;
-        if (write)
-            cache::write_kernel<dim, group, bf16>
-                <<<grid, cache::kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(args, device_status);
+        const auto launch = [&](auto rows_a_thread) {
+            const uint32_t rows_a_block = cache::kRowThreads / (dim / 8) * rows_a_thread;
+            const uint32_t blocks = (args.rows + rows_a_block - 1) / rows_a_block;
+            if (write)
+                cache::write_kernel<dim, group, rows_a_thread, bf16>
+                    <<<blocks, cache::kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(args, device_status);
+            else
+                cache::read_kernel<dim, group, rows_a_thread, bf16>
+                    <<<blocks, cache::kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(args, device_status);
+        };
+        // A few rows take one a thread, and so more threads.
+        const uint32_t few = static_cast<uint32_t>(facts.sm_count) * 4 * (cache::kRowThreads / (dim / 8));
+        if (args.rows <= few)
+            launch(std::integral_constant<int, 1>{});
+        else if (write)
+            launch(std::integral_constant<int, 2>{});
         else
-            cache::read_kernel<dim, group, bf16>
-                <<<grid, cache::kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(args, device_status);
+            launch(std::integral_constant<int, 4>{});
         FK_CUDA(cudaGetLastError());
         return static_cast<int>(FK_OK);
     });
