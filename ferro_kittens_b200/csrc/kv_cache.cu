@@ -58,6 +58,14 @@ struct Element<true> {
         asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
         return d;
     }
+    /// The smaller magnitude of each pair (the signs mean nothing).
+    static __device__ __forceinline__ uint32_t min_magnitude(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    /// What of a sum's size a value must have, not to lie below its last bit: 2^-15 (8 significant bits of 24), made 2^-14.
+    static constexpr float kVanishes = 0x1p-14f;
     /// The bits of the largest value of the type not above x >= 0.
     static __device__ __forceinline__ uint32_t truncate(float x) { return __float_as_uint(x) >> 16; }
     static __device__ __forceinline__ uint32_t minus_magic(uint32_t x) {
@@ -88,6 +96,12 @@ struct Element<false> {
         asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
         return d;
     }
+    static __device__ __forceinline__ uint32_t min_magnitude(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static constexpr float kVanishes = 0x1p-11f;
     static __device__ __forceinline__ uint32_t truncate(float x) {
         return __half_as_ushort(__float2half_rz(x));
     }
@@ -175,27 +189,23 @@ __device__ __forceinline__ float one_if_ge(float a, float b) {
     return y;
 }
 
-/// Codes and parameters of 8 channels (`words`, 16 bytes of a row) whose group lies in G / 8 neighbouring lanes. All lanes of a warp
-/// take part; where `kept` is false the result is not used.
+/// {smallest, -largest} of a group together, NaN if it holds one: 8 channels (`x`) in each of G / 8 neighbouring lanes.
 template <int G, bool BF16>
-struct Quantised {
-    uint32_t word, params;
-};
-
-template <int G, bool BF16>
-__device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
+__device__ __forceinline__ uint32_t group_ends(const uint4 x) {
     using E = Element<BF16>;
-    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-    // {smallest, -largest} of the group together, NaN if it holds one.
-    uint32_t least = words[0], most = words[0] ^ 0x80008000u;
-#pragma unroll
-    for (uint32_t i = 1; i < 4; ++i) {
-        least = E::min_nan(least, words[i]);
-        most = E::min_nan(most, words[i] ^ 0x80008000u);
-    }
+    const uint32_t least = E::min_nan(E::min_nan(x.x, x.y), E::min_nan(x.z, x.w));
+    const uint32_t most = E::min_nan(E::min_nan(x.x ^ 0x80008000u, x.y ^ 0x80008000u),
+                                     E::min_nan(x.z ^ 0x80008000u, x.w ^ 0x80008000u));
     uint32_t ends = E::min_nan(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
 #pragma unroll
     for (uint32_t mask = 1; mask < G / 8; mask *= 2) ends = E::min_nan(ends, __shfl_xor_sync(0xffffffffu, ends, mask));
+    return ends;
+}
+
+/// The group's scale in the low half and its smallest value in the high one, of its ends.
+template <bool BF16>
+__device__ __forceinline__ uint32_t group_params(uint32_t ends) {
+    using E = Element<BF16>;
     const float low = E::low(ends), high = -E::high(ends);
     // Half the span (the span itself may pass fp32's range), and what its rounding left out, exactly (the error of a sum is
     // a float).
@@ -206,47 +216,47 @@ __device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
     const bool finite = half_span < __uint_as_float(0x7f800000u);  // false for NaN as well
     // The scale: half_span / 7.5 with a little added, cut to the type, is right or one too large, which 7.5 times it, exact,
     // tells.
-    uint32_t scale_bits = finite ? E::truncate(half_span * (0x1.111112p-3f * (1.0f + 0x1p-21f))) : 0u;
+    uint32_t scale_bits = E::truncate(half_span * (0x1.111112p-3f * (1.0f + 0x1p-21f)));
     const float product = 7.5f * E::low(scale_bits);
     if (product > half_span || (product == half_span && lost < 0.0f)) --scale_bits;
-    const float scale = E::low(scale_bits);
+    return finite ? scale_bits | (ends << 16) : E::kNaN << 16;
+}
+
+/// The codes of 8 channels whose group has the parameters `params` and the largest value `high`.
+template <bool BF16>
+__device__ __forceinline__ uint32_t group_codes(const uint4 x, uint32_t params, float high) {
+    using E = Element<BF16>;
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+    const float scale = E::low(params), low = E::high(params);
     // Tiny spans are lifted by 2^100 so that 1 / scale stays finite, huge ones halved so that x - low does (the products are
-    // exact). Nothing is coded where the scale is zero: step and reach are then such that every code is 0.
-    const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f && scale > 0.0f ? 0x1p100f : 1.0f;
-    const bool coded = scale > 0.0f;
-    const float step = coded ? scale * lift : 1.0f, origin = -low * lift;
+    // exact).
+    const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f ? 0x1p100f : 1.0f;
+    const float step = scale * lift, origin = -low * lift, half_step = 0.5f * step, span = __fmaf_rn(high, lift, origin);
     // A guess that is never above the code and at most one below: the quotient's error is under 2^-18. The remainder t -
     // guess * step is exact, and a half step or more of it is one more.
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-    const float2 lift2 = make_float2(lift, lift), origin2 = make_float2(origin, origin);
-    const float inverse = coded ? rcp_approx(step) : 0.0f, half_step = 0.5f * step;
-    const float2 inverse2 = make_float2(inverse, inverse), under2 = make_float2(kMagic, kMagic);
-    const float2 bias2 = make_float2(-0x1p-17f, -0x1p-17f), minus_magic2 = make_float2(-kMagic, -kMagic);
-    const float2 minus_step2 = make_float2(-step, -step);
+    const float inverse = rcp_approx(step);
+    const float2 lift2 = make_float2(lift, lift), origin2 = make_float2(origin, origin), inverse2 = make_float2(inverse, inverse);
+    const float2 bias2 = make_float2(-0x1p-17f, -0x1p-17f), magic2 = make_float2(kMagic, kMagic);
+    const float2 minus_magic2 = make_float2(-kMagic, -kMagic), minus_step2 = make_float2(-step, -step);
     float2 code[4];
-    float nearest = -1.0f;  // the largest remainder
+    float nearest = 0.0f;  // the largest remainder
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
-        const float2 value = make_float2(E::low(words[i]), E::high(words[i]));
-        const float2 t = __ffma2_rn(value, lift2, origin2);
-        const float2 guess = __fadd2_rn(__fadd2_rn(__ffma2_rn(t, inverse2, bias2), under2), minus_magic2);
+        const float2 t = __ffma2_rn(make_float2(E::low(words[i]), E::high(words[i])), lift2, origin2);
+        const float2 guess = __fadd2_rn(__fadd2_rn(__ffma2_rn(t, inverse2, bias2), magic2), minus_magic2);
         const float2 rest = __ffma2_rn(guess, minus_step2, t);
-        nearest = fmaxf(nearest, fmaxf(rest.x, rest.y));
         code[i] = __fadd2_rn(guess, make_float2(one_if_ge(rest.x, half_step), one_if_ge(rest.y, half_step)));
+        nearest = fmaxf(nearest, fmaxf(rest.x, rest.y));
     }
-    // Where a remainder is a half step to the bit, t's own rounding may have made it one. That takes a value (or a smallest
-    // value) that is not zero and under 2^-9 of the span: others' lowest bits lie above t's. And where the scale was cut short (of
-    // a span of a few subnormals) codes pass 15.
-    if (coded && (nearest == half_step || half_span >= 7.75f * scale)) {
-        const float tiny = half_span * 0x1p-8f;
-        bool doubtful = half_span >= 7.75f * scale || (fabsf(low) < tiny && low != 0.0f);
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const float u = fabsf(E::low(words[i])), v = fabsf(E::high(words[i]));
-            doubtful |= (u < tiny && u != 0.0f) || (v < tiny && v != 0.0f);
-        }
+    // t is exact but where a value or the smallest one all but vanishes in it: there its rounding may have made a half step of the
+    // remainder. And where the scale was cut short (of a span of a few subnormals) codes pass 15. Both go the long way.
+    uint32_t small = E::min_magnitude(E::min_magnitude(words[0], words[1]), E::min_magnitude(words[2], words[3]));
+    small = E::min_magnitude(small, __byte_perm(small, params, 0x7632));  // with its other half, and the smallest value
+    const float vanishing = fminf(fabsf(E::low(small)), fabsf(E::high(small))) * lift;
+    if ((nearest == half_step && vanishing < span * E::kVanishes) || span >= 15.5f * step) {
 #pragma unroll 1
-        for (uint32_t i = 0; doubtful && i < 8; ++i) {
+        for (uint32_t i = 0; i < 8; ++i) {
             const uint32_t pair = i < 4 ? (i < 2 ? words[0] : words[1]) : (i < 6 ? words[2] : words[3]);
             const float lifted = ((i & 1u) ? E::high(pair) : E::low(pair)) * lift;
             const float t = lifted + origin, o_part = t - lifted;
@@ -266,10 +276,7 @@ __device__ __forceinline__ Quantised<G, BF16> quantise(const uint4 x) {
     const float2 front = __ffma2_rn(code[1], shift2, code[0]), back = __ffma2_rn(code[3], shift2, code[2]);
     const uint32_t first = __float_as_uint(__fmaf_rn(front.y, 16.0f, front.x) + 8388608.0f);
     const uint32_t last = __float_as_uint(__fmaf_rn(back.y, 16.0f, back.x) + 8388608.0f);
-    Quantised<G, BF16> result;
-    result.word = coded ? __byte_perm(first, last, 0x5410) : 0u;
-    result.params = scale_bits | ((finite ? ends & 0xffffu : E::kNaN) << 16);
-    return result;
+    return scale > 0.0f ? __byte_perm(first, last, 0x5410) : 0u;  // no span, or NaN: every code is 0
 }
 
 // One lane holds 8 channels (16 bytes) of a row's key and of its value, D / 8 lanes a row, ROWS rows of its own at a time: slots,
@@ -296,16 +303,22 @@ __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constan
         kept[r] = first + r * kAtATime < args.rows && cache_row(args, token, head, row[r], status);
     }
 #pragma unroll
-    for (uint32_t r = 0; r < ROWS; ++r)
+    for (uint32_t r = 0; r < ROWS; ++r) {
+        // Even lanes work out the key group's parameters, odd ones the value group's.
+        const uint32_t ends[2] = {group_ends<G, BF16>(x[r][0]), group_ends<G, BF16>(x[r][1])};
+        const uint32_t own = group_params<BF16>((lane & 1u) ? ends[1] : ends[0]);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+        const uint32_t params[2] = {(lane & 1u) ? other : own, (lane & 1u) ? own : other};
 #pragma unroll
         for (uint32_t which = 0; which < 2; ++which) {
-            Quantised<G, BF16> q = quantise<G, BF16>(x[r][which]);
-            if (which == 1) q.word = transpose_nibbles(q.word, lane);
+            uint32_t word = group_codes<BF16>(x[r][which], params[which], -Element<BF16>::high(ends[which]));
+            if (which == 1) word = transpose_nibbles(word, lane);
             if (kept[r]) {
-                args.codes[which][row[r] * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))] = q.word;
-                if (block % (G / 8) == 0) args.params[which][row[r] * (D / G) + block / (G / 8)] = q.params;
+                args.codes[which][row[r] * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))] = word;
+                if (block % (G / 8) == 0) args.params[which][row[r] * (D / G) + block / (G / 8)] = params[which];
             }
         }
+    }
 }
 
 // The same lanes the other way: a code in the low mantissa bits of a power of two, less that power, is exact,
@@ -330,6 +343,7 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant
         for (uint32_t which = 0; which < 2; ++which) {
             word[r][which] = __ldcs(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
             pair[r][which] = __ldcs(args.params[which] + row * (D / G) + block / (G / 8));
+            if (!kept[r]) word[r][which] = pair[r][which] = 0;  // reads as zeros
         }
     }
 #pragma unroll
@@ -340,17 +354,16 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant
 #pragma unroll
         for (uint32_t which = 0; which < 2; ++which) {
             const uint32_t scale = __byte_perm(pair[r][which], 0, 0x1010), low = __byte_perm(pair[r][which], 0, 0x3232);
-            uint32_t y[4];
+            uint32_t y[4];  // channels (i, i + 4)
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t codes = ((word[r][which] >> (8 * i)) & 0xfu) | ((word[r][which] >> (8 * i) << 12) & 0xf0000u);
-                y[i] = kept[r] ? E::fma(E::minus_magic(codes | E::kMagic), scale, low) : 0u;
-            }
+            for (uint32_t i = 0; i < 4; ++i)
+                y[i] = E::fma(E::minus_magic(((word[r][which] >> (4 * i)) & 0x000f000fu) | E::kMagic), scale, low);
             if (index < args.rows && (kept[r] || args.clear_skipped))
                 __stcs(reinterpret_cast<uint4*>(static_cast<uint8_t*>(const_cast<void*>(args.tensor[which])) +
                                                 token * args.token_stride[which] + head * args.head_stride[which]) +
                            block,
-                       make_uint4(y[0], y[1], y[2], y[3]));
+                       make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410),
+                                  __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632)));
         }
     }
 }
