@@ -58,6 +58,11 @@ struct Element<true> {
         asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
         return d;
     }
+    static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
     /// The smaller magnitude of each pair (the signs mean nothing).
     static __device__ __forceinline__ uint32_t min_magnitude(uint32_t a, uint32_t b) {
         uint32_t d;
@@ -94,6 +99,11 @@ struct Element<false> {
     static __device__ __forceinline__ uint32_t min_nan(uint32_t a, uint32_t b) {
         uint32_t d;
         asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
         return d;
     }
     static __device__ __forceinline__ uint32_t min_magnitude(uint32_t a, uint32_t b) {
@@ -135,7 +145,7 @@ __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t x, uint32_t lane)
 
 // ---------------------------------------------------------------- writing and reading
 
-constexpr uint32_t kRowThreads = 256;
+constexpr uint32_t kRowThreads = 128;
 
 struct RowArguments {
     const void* tensor[2];  // k, v (the source of a write, the destination of a read)
@@ -194,8 +204,7 @@ template <int G, bool BF16>
 __device__ __forceinline__ uint32_t group_ends(const uint4 x) {
     using E = Element<BF16>;
     const uint32_t least = E::min_nan(E::min_nan(x.x, x.y), E::min_nan(x.z, x.w));
-    const uint32_t most = E::min_nan(E::min_nan(x.x ^ 0x80008000u, x.y ^ 0x80008000u),
-                                     E::min_nan(x.z ^ 0x80008000u, x.w ^ 0x80008000u));
+    const uint32_t most = E::max_nan(E::max_nan(x.x, x.y), E::max_nan(x.z, x.w)) ^ 0x80008000u;
     uint32_t ends = E::min_nan(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
 #pragma unroll
     for (uint32_t mask = 1; mask < G / 8; mask *= 2) ends = E::min_nan(ends, __shfl_xor_sync(0xffffffffu, ends, mask));
@@ -228,43 +237,45 @@ __device__ __forceinline__ uint32_t group_codes(const uint4 x, uint32_t params, 
     using E = Element<BF16>;
     const uint32_t words[4] = {x.x, x.y, x.z, x.w};
     const float scale = E::low(params), low = E::high(params);
-    // Tiny spans are lifted by 2^100 so that 1 / scale stays finite, huge ones halved so that x - low does (the products are
-    // exact).
-    const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float step = scale * lift, origin = -low * lift, half_step = 0.5f * step, span = __fmaf_rn(high, lift, origin);
+    const float half_step = 0.5f * scale, span = high - low;
     // A guess that is never above the code and at most one below: the quotient's error is under 2^-18. The remainder t -
-    // guess * step is exact, and a half step or more of it is one more.
+    // guess * scale is exact, and a half step or more of it is one more.
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
-    const float inverse = rcp_approx(step);
-    const float2 lift2 = make_float2(lift, lift), origin2 = make_float2(origin, origin), inverse2 = make_float2(inverse, inverse);
+    const float inverse = rcp_approx(scale);
+    const float2 origin2 = make_float2(-low, -low), inverse2 = make_float2(inverse, inverse);
     const float2 bias2 = make_float2(-0x1p-17f, -0x1p-17f), magic2 = make_float2(kMagic, kMagic);
-    const float2 minus_magic2 = make_float2(-kMagic, -kMagic), minus_step2 = make_float2(-step, -step);
+    const float2 minus_magic2 = make_float2(-kMagic, -kMagic), minus_scale2 = make_float2(-scale, -scale);
     float2 code[4];
     float nearest = 0.0f;  // the largest remainder
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
-        const float2 t = __ffma2_rn(make_float2(E::low(words[i]), E::high(words[i])), lift2, origin2);
+        const float2 t = __fadd2_rn(make_float2(E::low(words[i]), E::high(words[i])), origin2);
         const float2 guess = __fadd2_rn(__fadd2_rn(__ffma2_rn(t, inverse2, bias2), magic2), minus_magic2);
-        const float2 rest = __ffma2_rn(guess, minus_step2, t);
+        const float2 rest = __ffma2_rn(guess, minus_scale2, t);
         code[i] = __fadd2_rn(guess, make_float2(one_if_ge(rest.x, half_step), one_if_ge(rest.y, half_step)));
         nearest = fmaxf(nearest, fmaxf(rest.x, rest.y));
     }
     // t is exact but where a value or the smallest one all but vanishes in it: there its rounding may have made a half step of the
-    // remainder. And where the scale was cut short (of a span of a few subnormals) codes pass 15. Both go the long way.
+    // remainder. Where the scale was cut short (of a span of a few subnormals) codes pass 15, and far scales leave fp32's range
+    // in t or in 1 / scale. All these go the long way, far scales lifted by 2^100 or halved (exactly).
     uint32_t small = E::min_magnitude(E::min_magnitude(words[0], words[1]), E::min_magnitude(words[2], words[3]));
     small = E::min_magnitude(small, __byte_perm(small, params, 0x7632));  // with its other half, and the smallest value
-    const float vanishing = fminf(fabsf(E::low(small)), fabsf(E::high(small))) * lift;
-    if ((nearest == half_step && vanishing < span * E::kVanishes) || span >= 15.5f * step) {
+    const float vanishing = fminf(fabsf(E::low(small)), fabsf(E::high(small)));
+    const bool far = scale < 0x1p-100f || scale > 0x1p100f;
+    if (scale > 0.0f && ((nearest == half_step && vanishing < span * E::kVanishes) || span >= 15.5f * scale || far)) {
+        const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f ? 0x1p100f : 1.0f;
+        const float step = scale * lift, origin = -low * lift, lifted_half = 0.5f * step;
+        const float lifted_inverse = __frcp_rn(step);
 #pragma unroll 1
         for (uint32_t i = 0; i < 8; ++i) {
             const uint32_t pair = i < 4 ? (i < 2 ? words[0] : words[1]) : (i < 6 ? words[2] : words[3]);
             const float lifted = ((i & 1u) ? E::high(pair) : E::low(pair)) * lift;
             const float t = lifted + origin, o_part = t - lifted;
             const float t_lost = (lifted - (t - o_part)) + (origin - o_part);
-            float c = fminf(rintf(t * inverse), 15.0f);
+            float c = fminf(rintf(t * lifted_inverse), 15.0f);
             const float rest = __fmaf_rn(c, -step, t);
-            if ((rest - half_step) + t_lost >= 0.0f) c += 1.0f;
-            else if ((rest + half_step) + t_lost < 0.0f) c -= 1.0f;
+            if ((rest - lifted_half) + t_lost >= 0.0f) c += 1.0f;
+            else if ((rest + lifted_half) + t_lost < 0.0f) c -= 1.0f;
             c = fminf(c, 15.0f);
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k)
@@ -341,8 +352,8 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant
         if (!kept[r]) row = 0;
 #pragma unroll
         for (uint32_t which = 0; which < 2; ++which) {
-            word[r][which] = __ldcs(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
-            pair[r][which] = __ldcs(args.params[which] + row * (D / G) + block / (G / 8));
+            word[r][which] = __ldg(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
+            pair[r][which] = __ldg(args.params[which] + row * (D / G) + block / (G / 8));
             if (!kept[r]) word[r][which] = pair[r][which] = 0;  // reads as zeros
         }
     }
@@ -1364,10 +1375,8 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
         const uint32_t few = static_cast<uint32_t>(facts.sm_count) * 4 * (cache::kRowThreads / (dim / 8));
         if (args.rows <= few)
             launch(std::integral_constant<int, 1>{});
-        else if (write)
-            launch(std::integral_constant<int, 2>{});
         else
-            launch(std::integral_constant<int, 4>{});
+            launch(std::integral_constant<int, 2>{});
         FK_CUDA(cudaGetLastError());
         return static_cast<int>(FK_OK);
     });
