@@ -570,6 +570,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     __shared__ uint32_t bad_pages[kStages];     // whether a stage has places whose page lies outside the cache
     __shared__ uint32_t stop_flag, complete[2];
     __shared__ Cut cuts[2];              // the parts of segments that are cut over blocks: the one this share begins in, ends in
+    __shared__ uint32_t tile_most[NT];   // largest magnitudes of the tile's queries
     __shared__ float2 row_stats[kRows];  // reference and sum of each row over the warps
     // The first warps compute, the last one or two copy: keys and values, or one side each.
     const uint32_t warps = blockDim.x / 32 - args.copying, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -745,38 +746,27 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         float q_sum[Shape::kSharedQueries ? 1 : kGroups][2];
         uint4* const shared_q = reinterpret_cast<uint4*>(shared);
         float* const shared_sums = reinterpret_cast<float*>(shared + kRows * D * 2);
-        const auto row_of = [&](uint32_t n) {
-            const uint32_t r = min(first_row + 8 * n + l4, args.rows - 1), t = args.ratio.quotient(r);
-            return args.q + b * args.q_batch_stride + t * args.q_token_stride +
-                   (kv_head * args.ratio.divisor + (r - t * args.ratio.divisor)) * args.q_head_stride;
-        };
-        uint4 raw[NT][kKeyWords];
-        float most = 0.0f;
-#pragma unroll
-        for (uint32_t n = 0; n < NT; ++n) {
-            const uint8_t* const q = row_of(n);
-            float row_most = 0.0f;
+        const auto load_row = [&](uint32_t n, uint4 (&raw)[kKeyWords]) {
+            const uint32_t r = first_row + 8 * n + l4, t = args.ratio.quotient(min(r, args.rows - 1));
+            const uint8_t* const q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
+                                     (kv_head * args.ratio.divisor + (r - t * args.ratio.divisor)) * args.q_head_stride;
+            float most = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kKeyWords; ++w) {
-                raw[n][w] = make_uint4(0, 0, 0, 0);
-                if (first_row + 8 * n + l4 < args.rows) raw[n][w] = __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4);
-                const uint32_t words[4] = {raw[n][w].x, raw[n][w].y, raw[n][w].z, raw[n][w].w};
+                raw[w] = r < args.rows ? __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4) : make_uint4(0, 0, 0, 0);
+                const uint32_t words[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i)
-                    row_most = fmaxf(row_most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
+                for (uint32_t i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
             }
-            if (row_most < INFINITY) most = fmaxf(most, row_most);  // a row that holds an infinity says nothing about others
-        }
-        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-        const int32_t biased = most == 0.0f ? 127 : min(268 - static_cast<int32_t>(__float_as_uint(most) >> 23), 254);
-        const float up = power_of_two(biased);
-        const float to_log2 = args.scale * 1.4426950408889634f * 0x1p24f * power_of_two(254 - biased);
-#pragma unroll
-        for (uint32_t n = 0; n < NT; ++n) {
-            float sums[kGroups] = {};
+            return most < INFINITY ? most : 0.0f;  // a row that holds an infinity says nothing about others
+        };
+        const auto power_for = [](float most) {
+            return most == 0.0f ? 127 : min(268 - static_cast<int32_t>(__float_as_uint(most) >> 23), 254);
+        };
+        const auto convert_row = [&](const uint4 (&raw)[kKeyWords], float up, uint4 (&f)[kKeyWords], float (&sums)[kGroups]) {
 #pragma unroll
             for (uint32_t w = 0; w < kKeyWords; ++w) {
-                const uint32_t words[4] = {raw[n][w].x, raw[n][w].y, raw[n][w].z, raw[n][w].w};
+                const uint32_t words[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
                 float v[8];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
@@ -784,38 +774,63 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     v[2 * i + 1] = E::high(words[i]) * up;
                     sums[w * 32 / G] += v[2 * i] + v[2 * i + 1];
                 }
-                uint4 f;
-                f.x = Element<false>::pack(v[0], v[4]);
-                f.y = Element<false>::pack(v[1] * 0.0625f, v[5] * 0.0625f);
-                f.z = Element<false>::pack(v[2], v[6]);
-                f.w = Element<false>::pack(v[3] * 0.0625f, v[7] * 0.0625f);
-                if constexpr (Shape::kSharedQueries) {
-                    if (warp == n % warps) shared_q[(n * kKeyWords + w) * 32 + lane] = f;
-                } else {
-                    qf[2 * w][0] = f.x, qf[2 * w][1] = f.y, qf[2 * w + 1][0] = f.z, qf[2 * w + 1][1] = f.w;
-                }
+                f[w].x = Element<false>::pack(v[0], v[4]);
+                f[w].y = Element<false>::pack(v[1] * 0.0625f, v[5] * 0.0625f);
+                f[w].z = Element<false>::pack(v[2], v[6]);
+                f[w].w = Element<false>::pack(v[3] * 0.0625f, v[7] * 0.0625f);
             }
 #pragma unroll
             for (uint32_t g = 0; g < kGroups; ++g) {
                 sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 1);
                 sums[g] += __shfl_xor_sync(0xffffffffu, sums[g], 2);
                 sums[g] *= 0x1p-24f;
-                if constexpr (Shape::kSharedQueries) {
-                    if (warp == n % warps && c4 == 0) shared_sums[g * kRows + 8 * n + l4] = sums[g];
-                } else {
+            }
+        };
+        int32_t power;
+        {
+            uint4 raw[kKeyWords], f[kKeyWords];
+            if constexpr (Shape::kSharedQueries) {
+                for (uint32_t n = warp; n < NT; n += warps) {
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(load_row(n, raw)));
+                    if (lane == 0) tile_most[n] = most;
+                }
+                sync_computing(warps * 32);
+                uint32_t most = 0;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) most = max(most, tile_most[n]);
+                power = power_for(__uint_as_float(most));
+                for (uint32_t n = warp; n < NT; n += warps) {
+                    float sums[kGroups] = {};
+                    load_row(n, raw);
+                    convert_row(raw, power_of_two(power), f, sums);
+#pragma unroll
+                    for (uint32_t w = 0; w < kKeyWords; ++w) shared_q[(n * kKeyWords + w) * 32 + lane] = f[w];
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g)
+                        if (c4 == 0) shared_sums[g * kRows + 8 * n + l4] = sums[g];
+                }
+                sync_computing(warps * 32);
+            } else {
+                power = power_for(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(load_row(0, raw)))));
+                float sums[kGroups] = {};
+                convert_row(raw, power_of_two(power), f, sums);
+#pragma unroll
+                for (uint32_t w = 0; w < kKeyWords; ++w)
+                    qf[2 * w][0] = f[w].x, qf[2 * w][1] = f[w].y, qf[2 * w + 1][0] = f[w].z, qf[2 * w + 1][1] = f[w].w;
+#pragma unroll
+                for (uint32_t g = 0; g < kGroups; ++g)
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) q_sum[g][e] = __shfl_sync(0xffffffffu, sums[g], 8 * c4 + 4 * e);
-                }
             }
         }
-        if constexpr (Shape::kSharedQueries) sync_computing(warps * 32);
+        const float to_log2 = args.scale * 1.4426950408889634f * 0x1p24f * power_of_two(254 - power);
 
         float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {}, lows[kGroups][NT][2] = {};
-        float peak[NT][2], sum[NT][2] = {};
+        float peak[NT][2], minus_peak[NT][2] = {}, sum[NT][2] = {};  // minus_peak: 0 while peak is -inf
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) peak[n][0] = peak[n][1] = -INFINITY;
         int32_t top = 0;  // biased exponent of the largest value scale so far
-        float fit = power_of_two(254);
+        float fit = power_of_two(254), limit = 0x1p-126f;  // limit: the least scale that would raise top
 
         // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
         // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
@@ -839,65 +854,64 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             const bool is_masked = real != 0xffffffffu || extent.token(place + 31) > extent.first ||
                                    (args.window && extent.token(place + 31) >= args.sinks &&
                                     extent.token(place) <= extent.length - 1 - args.window);
-            const bool is_real = real >> lane & 1u;
             bool careful = false;  // some token that some row may not see has values that are not finite
 
             // ---- parameters as floats, lane = token, and the power of two that lets weight * scale fit fp16 whatever the
             // scales' size; what was summed so far follows when it changes.
             {
-                uint32_t pairs[kGroups];
+                uint32_t key_pairs[kGroups], pairs[kGroups];
                 float scales[kGroups], widest = 0.0f;
+                load_words(key_pairs, key_params + lane * (kGroups * 4));
                 load_words(pairs, value_params + lane * (kGroups * 4));
-#pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g) {
-                    if (!is_real) pairs[g] = 0;
-                    scales[g] = E::low(pairs[g]);
-                    widest = fmaxf(widest, fabsf(scales[g]));
-                }
                 if (is_masked) {
                     bool finite = true;
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g)
-                        finite = finite && fabsf(scales[g]) < INFINITY && fabsf(E::high(pairs[g])) < INFINITY;
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        if (!(real >> lane & 1u)) key_pairs[g] = pairs[g] = 0;
+                        finite = finite && fabsf(E::low(pairs[g])) < INFINITY && fabsf(E::high(pairs[g])) < INFINITY;
+                    }
                     careful = !__all_sync(0xffffffffu, finite);
                 }
-                uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(widest));
-                if (bits >= 0x7f800000u) {  // an infinity says nothing about the others
-                    widest = 0.0f;
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g)
-                        if (fabsf(scales[g]) < INFINITY) widest = fmaxf(widest, fabsf(scales[g]));
-                    bits = __reduce_max_sync(0xffffffffu, __float_as_uint(widest));
+                for (uint32_t g = 0; g < kGroups; ++g) {
+                    scales[g] = E::low(pairs[g]);
+                    widest = fmaxf(widest, fabsf(scales[g]));
                 }
-                const int32_t unit_top = static_cast<int32_t>(bits >> 23);
-                if (unit_top > top) {
-                    const float shrink = power_of_two(max(127 + min(kFitBiased - unit_top, 254) - min(kFitBiased - top, 254), 0));
-                    top = unit_top;
-                    fit = power_of_two(min(kFitBiased - top, 254));
+                if (__any_sync(0xffffffffu, widest >= limit)) {
+                    if (!(widest < INFINITY)) {  // an infinity says nothing about the others
+                        widest = 0.0f;
 #pragma unroll
-                    for (uint32_t n = 0; n < NT; ++n)
+                        for (uint32_t g = 0; g < kGroups; ++g)
+                            if (fabsf(scales[g]) < INFINITY) widest = fmaxf(widest, fabsf(scales[g]));
+                    }
+                    const int32_t unit_top =
+                        static_cast<int32_t>(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23);
+                    if (unit_top > top) {
+                        const float shrink = power_of_two(max(127 + min(kFitBiased - unit_top, 254) - min(kFitBiased - top, 254), 0));
+                        top = unit_top;
+                        fit = power_of_two(min(kFitBiased - top, 254));
+                        limit = power_of_two(top + 1);
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
+                        for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
-                            for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= shrink;
-                            if constexpr (kEights) {
+                            for (uint32_t i = 0; i < 4; ++i) {
 #pragma unroll
-                                for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= shrink;
+                                for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= shrink;
+                                if constexpr (kEights) {
+#pragma unroll
+                                    for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= shrink;
+                                }
                             }
-                        }
+                    }
                 }
                 float2 wide[kGroups];
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g)
                     wide[g] = make_float2(scales[g] * fit, fmaf(8.0f, scales[g], E::high(pairs[g])));
                 store_floats(wide_values + lane * (kGroups * 8), wide);
-                load_words(pairs, key_params + lane * (kGroups * 4));
-                if (!is_real) {
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) pairs[g] = 0;
-                }
-#pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g) wide[g] = make_float2(E::low(pairs[g]) * to_log2, E::high(pairs[g]) * to_log2);
+                for (uint32_t g = 0; g < kGroups; ++g)
+                    wide[g] = make_float2(E::low(key_pairs[g]) * to_log2, E::high(key_pairs[g]) * to_log2);
                 store_floats(wide_keys + lane * (kGroups * 8), wide);
             }
             __syncwarp();
@@ -924,15 +938,15 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n) {
-                                uint4 f;
-                                if constexpr (Shape::kSharedQueries)
-                                    f = shared_q[(n * kKeyWords + w) * 32 + lane];
+                                uint32_t f[4];
+                                if constexpr (Shape::kSharedQueries)  // each time anew: registers are full
+                                    ld_shared_v4(smem_u32(shared_q + (n * kKeyWords + w) * 32 + lane), f);
                                 else
-                                    f = make_uint4(qf[2 * w][0], qf[2 * w][1], qf[2 * w + 1][0], qf[2 * w + 1][1]);
+                                    f[0] = qf[2 * w][0], f[1] = qf[2 * w][1], f[2] = qf[2 * w + 1][0], f[3] = qf[2 * w + 1][1];
                                 mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
-                                            a[1][w] & 0x00f000f0u, f.x, f.y);
+                                            a[1][w] & 0x00f000f0u, f[0], f[1]);
                                 mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u,
-                                            y1 & 0x00f000f0u, f.z, f.w);
+                                            y1 & 0x00f000f0u, f[2], f[3]);
                             }
                         }
 #pragma unroll
@@ -1000,6 +1014,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             if (m > peak[n][e]) {
                                 keep[e] = ex2_approx(peak[n][e] - m);
                                 peak[n][e] = m;
+                                minus_peak[n][e] = -m;
                             }
                             sum[n][e] *= keep[e];
 #pragma unroll
@@ -1032,8 +1047,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             float p[4];
 #pragma unroll
                             for (uint32_t i = 0; i < 4; ++i) {
-                                // A row that has seen nothing has a peak of -inf, and so have its scores.
-                                p[i] = ex2_approx(x[h][n][i] - (peak[n][i % 2] == -INFINITY ? 0.0f : peak[n][i % 2]));
+                                p[i] = ex2_approx(x[h][n][i] + minus_peak[n][i % 2]);
                                 sum[n][i % 2] += p[i];
                             }
 #pragma unroll
