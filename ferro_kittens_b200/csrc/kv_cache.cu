@@ -71,6 +71,9 @@ struct Element<true> {
     }
     /// What of a sum's size a value must have, not to lie below its last bit: 2^-15 (8 significant bits of 24), made 2^-14.
     static constexpr float kVanishes = 0x1p-14f;
+    static __device__ __forceinline__ bool finite(uint32_t pair) {
+        return (pair & 0x7f80u) != 0x7f80u && (pair & 0x7f800000u) != 0x7f800000u;
+    }
     /// The bits of the largest value of the type not above x >= 0.
     static __device__ __forceinline__ uint32_t truncate(float x) { return __float_as_uint(x) >> 16; }
     static __device__ __forceinline__ uint32_t minus_magic(uint32_t x) {
@@ -112,6 +115,9 @@ struct Element<false> {
         return d;
     }
     static constexpr float kVanishes = 0x1p-11f;
+    static __device__ __forceinline__ bool finite(uint32_t pair) {
+        return (pair & 0x7c00u) != 0x7c00u && (pair & 0x7c000000u) != 0x7c000000u;
+    }
     static __device__ __forceinline__ uint32_t truncate(float x) {
         return __half_as_ushort(__float2half_rz(x));
     }
@@ -407,7 +413,7 @@ struct AttentionArguments {
 constexpr uint32_t kWarpTokens = 32;
 constexpr uint32_t kStages = 3;
 constexpr uint32_t kMostBlocksPerSm = 4;
-constexpr uint32_t kMostRows = 32;
+constexpr uint32_t kMostRows = 16;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
 constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
 /// How far (in powers of two) a score may lie above its row's reference before the reference is moved. Weights reach
@@ -431,14 +437,14 @@ struct AttentionShape {
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
     static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
     static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes;
-    static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 8;
+    static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 16;
     static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
     static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
     static constexpr bool kMergeInRing = kMergeBytes <= kStageBytes;
     static constexpr uint32_t kScratchBytes = kMergeInRing || 2 * kWideBytes > kMergeBytes ? 2 * kWideBytes : kMergeBytes;
     static constexpr uint32_t kWarpBytes = kStages * kStageBytes + kScratchBytes;
-    // Registers a thread: 128, 168 or 255.
-    static constexpr uint32_t kMostThreads = 32 * (NT == 1 ? (kGroups > 2 ? 12 : 16) : NT == 2 ? 12 : 8);
+    // Registers a thread: 128, or 168 for more than one row tile or two groups.
+    static constexpr uint32_t kMostThreads = 32 * (NT == 1 && kGroups <= 2 ? 16 : 12);
     static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
     static constexpr uint32_t most_warps(uint32_t copying) {
         return kMostThreads / 32 - copying < kMostByMemory ? kMostThreads / 32 - copying : kMostByMemory;
@@ -528,13 +534,6 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const void* fro
     }
 }
 
-template <int PAIRS>
-__device__ __forceinline__ void store_floats(void* to, const float2 (&x)[PAIRS]) {
-    if constexpr (PAIRS == 1) *static_cast<float2*>(to) = x[0];
-#pragma unroll
-    for (int i = 0; i + 1 < PAIRS; i += 2) static_cast<float4*>(to)[i / 2] = make_float4(x[i].x, x[i].y, x[i + 1].x, x[i + 1].y);
-}
-
 /// A piece of a segment (of its first row's tile), and if blocks share the segment, in how many parts and which block keeps count.
 struct Cut {
     uint32_t b, kv_head, first_row, parts, owner;
@@ -563,8 +562,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     using Shape = AttentionShape<D, G, NT>;
     constexpr uint32_t kGroups = Shape::kGroups, kRows = Shape::kRows, kPitch = Shape::kPitch;
     constexpr uint32_t kKeyWords = D / 32, kValueWords = D / 64, kTiles = D / 16;
-    constexpr uint32_t kSteps = NT == 4 ? 1 : 2;      // steps of 16 tokens between looks at the running maximum
-    constexpr bool kEights = NT == 1;                 // see `eights` below
+    constexpr bool kEights = NT == 1;  // see `eights` below
     extern __shared__ __align__(16) uint8_t shared[];
     __shared__ uint64_t barriers[2 * kStages];  // of each stage: it is full; it is free again
     __shared__ uint32_t bad_pages[kStages];     // whether a stage has places whose page lies outside the cache
@@ -825,18 +823,20 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         }
         const float to_log2 = args.scale * 1.4426950408889634f * 0x1p24f * power_of_two(254 - power);
 
-        float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {}, lows[kGroups][NT][2] = {};
-        float peak[NT][2], minus_peak[NT][2] = {}, sum[NT][2] = {};  // minus_peak: 0 while peak is -inf
+        // Pairs are a fragment's two rows.
+        float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {};
+        float2 lows[kGroups][NT] = {}, peak[NT], minus_peak[NT] = {}, sum[NT] = {};  // minus_peak: 0 while peak is -inf
 #pragma unroll
-        for (uint32_t n = 0; n < NT; ++n) peak[n][0] = peak[n][1] = -INFINITY;
+        for (uint32_t n = 0; n < NT; ++n) peak[n] = make_float2(-INFINITY, -INFINITY);
         int32_t top = 0;  // biased exponent of the largest value scale so far
         float fit = power_of_two(254), limit = 0x1p-126f;  // limit: the least scale that would raise top
 
         // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
         // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
         const uint32_t own_token = (l4 >> 1) + 4 * (l4 & 1);
-        uint8_t* const wide_keys = ring + kStages * stage_bytes + warp * Shape::kScratchBytes;  // (scale, low) * to_log2 of each token and group
-        uint8_t* const wide_values = wide_keys + Shape::kWideBytes;     // (scale * fit, low + 8 * scale)
+        // Of each token and group: (scale, scale, low, low), the keys' times to_log2; the values' scale * fit and low + 8 * scale.
+        float4* const wide_keys = reinterpret_cast<float4*>(ring + kStages * stage_bytes + warp * Shape::kScratchBytes);
+        float4* const wide_values = wide_keys + kWarpTokens * kGroups;
 
 #pragma unroll 1
         for (uint32_t unit = from; unit < to; ++unit) {
@@ -846,128 +846,115 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             const uint8_t* const values = keys + value_codes;
             const uint8_t* const key_params = ring + stage * stage_bytes + 2 * value_codes + warp * Shape::kParamBytes;
             const uint8_t* const value_params = key_params + warps * Shape::kParamBytes;
-            // Which of the 32 tokens are there, and whether some row may not see some token (they rise from place to place).
+            // Whether some row may not see some of the 32 tokens (they rise from place to place), or some are not there.
             const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens), here = extent.visible() - place;
-            uint32_t real = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1;
-            if (bad_pages[stage])
-                real &= __ballot_sync(0xffffffffu, static_cast<int32_t>(lane) < here && page_at(place + lane) < args.pages);
-            const bool is_masked = real != 0xffffffffu || extent.token(place + 31) > extent.first ||
+            const bool is_masked = here < 32 || bad_pages[stage] || extent.token(place + 31) > extent.first ||
                                    (args.window && extent.token(place + 31) >= args.sinks &&
                                     extent.token(place) <= extent.length - 1 - args.window);
-            bool careful = false;  // some token that some row may not see has values that are not finite
 
-            // ---- parameters as floats, lane = token, and the power of two that lets weight * scale fit fp16 whatever the
-            // scales' size; what was summed so far follows when it changes.
-            {
-                uint32_t key_pairs[kGroups], pairs[kGroups];
-                float scales[kGroups], widest = 0.0f;
-                load_words(key_pairs, key_params + lane * (kGroups * 4));
-                load_words(pairs, value_params + lane * (kGroups * 4));
-                if (is_masked) {
-                    bool finite = true;
+            // ---- parameters as floats, each twice, lane = token, for packed arithmetic on a fragment's two rows.
+            uint32_t key_pairs[kGroups], value_pairs[kGroups];
+            float widest = 0.0f;
+            load_words(key_pairs, key_params + lane * (kGroups * 4));
+            load_words(value_pairs, value_params + lane * (kGroups * 4));
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) {
-                        if (!(real >> lane & 1u)) key_pairs[g] = pairs[g] = 0;
-                        finite = finite && fabsf(E::low(pairs[g])) < INFINITY && fabsf(E::high(pairs[g])) < INFINITY;
-                    }
-                    careful = !__all_sync(0xffffffffu, finite);
-                }
-#pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g) {
-                    scales[g] = E::low(pairs[g]);
-                    widest = fmaxf(widest, fabsf(scales[g]));
-                }
-                if (__any_sync(0xffffffffu, widest >= limit)) {
-                    if (!(widest < INFINITY)) {  // an infinity says nothing about the others
-                        widest = 0.0f;
-#pragma unroll
-                        for (uint32_t g = 0; g < kGroups; ++g)
-                            if (fabsf(scales[g]) < INFINITY) widest = fmaxf(widest, fabsf(scales[g]));
-                    }
-                    const int32_t unit_top =
-                        static_cast<int32_t>(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23);
-                    if (unit_top > top) {
-                        const float shrink = power_of_two(max(127 + min(kFitBiased - unit_top, 254) - min(kFitBiased - top, 254), 0));
-                        top = unit_top;
-                        fit = power_of_two(min(kFitBiased - top, 254));
-                        limit = power_of_two(top + 1);
-#pragma unroll
-                        for (uint32_t n = 0; n < NT; ++n)
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) {
-#pragma unroll
-                                for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= shrink;
-                                if constexpr (kEights) {
-#pragma unroll
-                                    for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= shrink;
-                                }
-                            }
-                    }
-                }
-                float2 wide[kGroups];
-#pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g)
-                    wide[g] = make_float2(scales[g] * fit, fmaf(8.0f, scales[g], E::high(pairs[g])));
-                store_floats(wide_values + lane * (kGroups * 8), wide);
-#pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g)
-                    wide[g] = make_float2(E::low(key_pairs[g]) * to_log2, E::high(key_pairs[g]) * to_log2);
-                store_floats(wide_keys + lane * (kGroups * 8), wide);
+            for (uint32_t g = 0; g < kGroups; ++g) {
+                const float scale = E::low(key_pairs[g]) * to_log2, low = E::high(key_pairs[g]) * to_log2;
+                wide_keys[lane * kGroups + g] = make_float4(scale, scale, low, low);
+                widest = fmaxf(widest, fabsf(E::low(value_pairs[g])));
             }
-            __syncwarp();
 
+            // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
+            // subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
+            float2 x[2][NT][2];  // [step of 16 tokens][row tile][token of the fragment's upper or lower half] (two rows)
+            const auto products = [&](uint32_t h, uint32_t g, const uint32_t (&a)[2][kKeyWords], float (&part)[NT][4]) {
 #pragma unroll
-            for (uint32_t round = 0; round < 2 / kSteps; ++round) {
-                // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
-                // subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
-                float x[kSteps][NT][4];
+                for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w) {
+                    const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
 #pragma unroll
-                for (uint32_t h = 0; h < kSteps; ++h) {
-                    uint32_t a[2][kKeyWords], wide[2][2 * kGroups];
-#pragma unroll
-                    for (uint32_t half = 0; half < 2; ++half) {
-                        const uint32_t row = 16 * (round * kSteps + h) + 8 * half + own_token;
-                        load_words(a[half], keys + row * (D / 2) + c4 * (D / 8));
-                        load_words(wide[half], wide_keys + row * (kGroups * 8));
+                    for (uint32_t n = 0; n < NT; ++n) {
+                        uint32_t f[4];
+                        if constexpr (Shape::kSharedQueries)  // each time anew: registers are full
+                            ld_shared_v4(smem_u32(shared_q + (n * kKeyWords + w) * 32 + lane), f);
+                        else
+                            f[0] = qf[2 * w][0], f[1] = qf[2 * w][1], f[2] = qf[2 * w + 1][0], f[3] = qf[2 * w + 1][1];
+                        mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
+                                    a[1][w] & 0x00f000f0u, f[0], f[1]);
+                        mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, f[2], f[3]);
                     }
+                }
+            };
+            const auto load_keys = [&](uint32_t h, uint32_t (&a)[2][kKeyWords]) {
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half)
+                    load_words(a[half], keys + (16 * h + 8 * half + own_token) * (D / 2) + c4 * (D / 8));
+            };
+            const auto add_up = [&](uint32_t h, uint32_t g, const float (&part)[NT][4]) {
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    const float4 wide = wide_keys[(16 * h + 8 * half + own_token) * kGroups + g];
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n) {
+                        float2 sums;
+                        if constexpr (Shape::kSharedQueries)
+                            sums = *reinterpret_cast<const float2*>(shared_sums + g * kRows + 8 * n + 2 * c4);
+                        else
+                            sums = make_float2(q_sum[g][0], q_sum[g][1]);
+                        const float2 low = make_float2(wide.z, wide.w);
+                        const float2 rest = g == 0 ? __fmul2_rn(low, sums) : __ffma2_rn(low, sums, x[h][n][half]);
+                        x[h][n][half] = __ffma2_rn(make_float2(wide.x, wide.y),
+                                                   make_float2(part[n][2 * half], part[n][2 * half + 1]), rest);
+                    }
+                }
+            };
+            if constexpr (NT == 1) {  // all products first: the parameters' way through shared memory hides behind them
+                float part[2][kGroups][NT][4] = {};
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    uint32_t a[2][kKeyWords];
+                    load_keys(h, a);
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) products(h, g, a, part[h][g]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) add_up(h, g, part[h][g]);
+            } else {
+                __syncwarp();
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    uint32_t a[2][kKeyWords];
+                    load_keys(h, a);
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; ++g) {
                         float part[NT][4] = {};
-#pragma unroll
-                        for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w) {
-                            const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
-#pragma unroll
-                            for (uint32_t n = 0; n < NT; ++n) {
-                                uint32_t f[4];
-                                if constexpr (Shape::kSharedQueries)  // each time anew: registers are full
-                                    ld_shared_v4(smem_u32(shared_q + (n * kKeyWords + w) * 32 + lane), f);
-                                else
-                                    f[0] = qf[2 * w][0], f[1] = qf[2 * w][1], f[2] = qf[2 * w + 1][0], f[3] = qf[2 * w + 1][1];
-                                mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
-                                            a[1][w] & 0x00f000f0u, f[0], f[1]);
-                                mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u,
-                                            y1 & 0x00f000f0u, f[2], f[3]);
-                            }
-                        }
-#pragma unroll
-                        for (uint32_t n = 0; n < NT; ++n) {
-                            float2 sums;
-                            if constexpr (Shape::kSharedQueries)
-                                sums = *reinterpret_cast<const float2*>(shared_sums + g * kRows + 8 * n + 2 * c4);
-                            else
-                                sums = make_float2(q_sum[g][0], q_sum[g][1]);
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) {
-                                const float scale = __uint_as_float(wide[i / 2][2 * g]);
-                                const float low = __uint_as_float(wide[i / 2][2 * g + 1]);
-                                const float s = i % 2 ? sums.y : sums.x;
-                                const float rest = g == 0 ? low * s : fmaf(low, s, x[h][n][i]);
-                                x[h][n][i] = fmaf(scale, part[n][i], rest);
-                            }
-                        }
+                        products(h, g, a, part);
+                        add_up(h, g, part);
                     }
                 }
+            }
+
+            // ---- what rarely happens, all in one place: tokens that some row may not see; a score more than kSlack above its
+            // row's reference, the score that its exponentials are taken from (so that weights stay under 2^kSlack); a
+            // value scale over the largest so far, which fixes the power of two that lets weight * scale fit fp16.
+            float2 largest[NT];
+            bool grows = widest >= limit;
+            const auto look = [&]() {
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n)
+                    largest[n] = make_float2(fmaxf(fmaxf(x[0][n][0].x, x[0][n][1].x), fmaxf(x[1][n][0].x, x[1][n][1].x)),
+                                             fmaxf(fmaxf(x[0][n][0].y, x[0][n][1].y), fmaxf(x[1][n][0].y, x[1][n][1].y)));
+            };
+            look();
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n) grows |= largest[n].x > peak[n].x + kSlack || largest[n].y > peak[n].y + kSlack;
+            if (is_masked || __any_sync(0xffffffffu, grows)) {
                 if (is_masked) {
+                    uint32_t real = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1;
+                    if (bad_pages[stage])
+                        real &= __ballot_sync(0xffffffffu, static_cast<int32_t>(lane) < here && page_at(place + lane) < args.pages);
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
@@ -975,144 +962,158 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             const uint32_t t = args.ratio.quotient(min(first_row + 8 * n + 2 * c4 + e, args.rows - 1));
                             const int32_t i = extent.length - static_cast<int32_t>(args.queries) + static_cast<int32_t>(t);
 #pragma unroll
-                            for (uint32_t h = 0; h < kSteps; ++h)
-#pragma unroll
-                                for (uint32_t half = 0; half < 2; ++half) {
-                                    const uint32_t k = 16 * (round * kSteps + h) + 8 * half + own_token;
-                                    const int32_t j = extent.token(place + static_cast<int32_t>(k));
-                                    const bool seen = (real >> k & 1u) && j <= i &&
-                                                      (!args.window || j > i - args.window || j < args.sinks);
-                                    if (!seen) x[h][n][2 * half + e] = -INFINITY;
-                                }
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                const uint32_t its = 8 * k + own_token;
+                                const int32_t j = extent.token(place + static_cast<int32_t>(its));
+                                if (!(real >> its & 1u) || j > i || (args.window && j <= i - args.window && j >= args.sinks))
+                                    (e ? x[k / 2][n][k % 2].y : x[k / 2][n][k % 2].x) = -INFINITY;
+                            }
                         }
-                }
-
-                // ---- the reference of each row's exponentials: its largest score when it was last set, and set again only
-                // when some score lies more than kSlack above it, so that a weight stays under 2^kSlack.
-                float largest[NT][2];
-                bool grows = false;
+                    // Values that are not finite make NaN of the groups of the rows that see them, and of no others: a
+                    // weight of zero would make NaN of them too.
+                    bool finite = true;
 #pragma unroll
-                for (uint32_t n = 0; n < NT; ++n)
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        if (!(real >> lane & 1u)) value_pairs[g] = 0;
+                        finite = finite && E::finite(value_pairs[g]);
+                    }
+                    const uint32_t sound = __ballot_sync(0xffffffffu, finite);
+                    if (sound != 0xffffffffu) {
+#pragma unroll
+                        for (uint32_t g = 0; g < kGroups; ++g) {
+#pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                const uint32_t its = 8 * k + own_token;
+                                const uint32_t pair = reinterpret_cast<const uint32_t*>(value_params)[its * kGroups + g];
+                                if ((real >> its & 1u) && !E::finite(pair))
+#pragma unroll
+                                    for (uint32_t n = 0; n < NT; ++n) {
+                                        if (x[k / 2][n][k % 2].x != -INFINITY) lows[g][n].x = __uint_as_float(0x7fffffffu);
+                                        if (x[k / 2][n][k % 2].y != -INFINITY) lows[g][n].y = __uint_as_float(0x7fffffffu);
+                                    }
+                            }
+                            if (!E::finite(value_pairs[g])) value_pairs[g] = 0;
+                        }
+                    }
+                    widest = 0.0f;
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) widest = fmaxf(widest, fabsf(E::low(value_pairs[g])));
+                    look();
+                }
+                if (!(widest < INFINITY)) {  // an infinity says nothing about the others
+                    widest = 0.0f;
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g)
+                        if (E::finite(value_pairs[g])) widest = fmaxf(widest, fabsf(E::low(value_pairs[g])));
+                }
+                const int32_t unit_top = static_cast<int32_t>(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23);
+                float shrink = 1.0f;
+                if (unit_top > top) {
+                    shrink = power_of_two(max(127 + min(kFitBiased - unit_top, 254) - min(kFitBiased - top, 254), 0));
+                    top = unit_top;
+                    fit = power_of_two(min(kFitBiased - top, 254));
+                    limit = power_of_two(top + 1);
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) {
+                    float keep[2], m[2] = {largest[n].x, largest[n].y}, was[2] = {peak[n].x, peak[n].y};
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) {
-                        float m = fmaxf(x[0][n][e], x[0][n][2 + e]);
-                        if constexpr (kSteps == 2) m = fmaxf(m, fmaxf(x[1][n][e], x[1][n][2 + e]));
-                        largest[n][e] = m;
-                        grows |= m > peak[n][e] + kSlack;
+                        m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 4));
+                        m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 8));
+                        m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 16));
+                        keep[e] = m[e] > was[e] ? ex2_approx(was[e] - m[e]) : 1.0f;
+                        m[e] = fmaxf(m[e], was[e]);
                     }
-                if (__any_sync(0xffffffffu, grows)) {
+                    peak[n] = make_float2(m[0], m[1]);
+                    // While a row has seen nothing its scores are -inf: so are its exponents, with nothing taken off.
+                    minus_peak[n] = make_float2(m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]);
+                    const float2 keep2 = make_float2(keep[0], keep[1]);
+                    sum[n] = __fmul2_rn(sum[n], keep2);
 #pragma unroll
-                    for (uint32_t n = 0; n < NT; ++n) {
-                        float keep[2];
+                    for (uint32_t g = 0; g < kGroups; ++g) lows[g][n] = __fmul2_rn(lows[g][n], keep2);
 #pragma unroll
-                        for (uint32_t e = 0; e < 2; ++e) {
-                            float m = largest[n][e];
-                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                            keep[e] = 1.0f;
-                            if (m > peak[n][e]) {
-                                keep[e] = ex2_approx(peak[n][e] - m);
-                                peak[n][e] = m;
-                                minus_peak[n][e] = -m;
-                            }
-                            sum[n][e] *= keep[e];
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const float factor = keep[i % 2] * shrink;
 #pragma unroll
-                            for (uint32_t g = 0; g < kGroups; ++g) lows[g][n][e] *= keep[e];
-                        }
+                        for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= factor;
+                        if constexpr (kEights) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-#pragma unroll
-                            for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= keep[i % 2];
-                            if constexpr (kEights) {
-#pragma unroll
-                                for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= keep[i % 2];
-                            }
+                            for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= factor;
                         }
                     }
                 }
+            }
 
 #pragma unroll
-                for (uint32_t h = 0; h < kSteps; ++h) {
-                    // ---- weights, their sums, and weight * scale in fp16, turned to be the values' second operand.
-                    const uint32_t first_token = 16 * (round * kSteps + h);
-                    uint32_t wide[2][2 * kGroups];
+            for (uint32_t g = 0; g < kGroups; ++g) {
+                const float scale = E::low(value_pairs[g]), low = fmaf(8.0f, scale, E::high(value_pairs[g]));
+                wide_values[lane * kGroups + g] = make_float4(scale * fit, scale * fit, low, low);
+            }
+            __syncwarp();
 #pragma unroll
-                    for (uint32_t half = 0; half < 2; ++half)
-                        load_words(wide[half], wide_values + (first_token + 8 * half + own_token) * (kGroups * 8));
-                    uint32_t weights[kGroups][NT][2];
-                    const auto weigh = [&](auto guarded) {
+            for (uint32_t h = 0; h < 2; ++h) {
+                // ---- weights, their sums, and weight * scale in fp16, turned to be the values' second operand.
+                uint32_t weights[kGroups][NT][2];
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    float2 p[NT];
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n) {
+                        const float2 power = __fadd2_rn(x[h][n][half], minus_peak[n]);
+                        p[n] = make_float2(ex2_approx(power.x), ex2_approx(power.y));
+                        sum[n] = __fadd2_rn(sum[n], p[n]);
+                    }
+#pragma unroll
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        const float4 wide = wide_values[(16 * h + 8 * half + own_token) * kGroups + g];
 #pragma unroll
                         for (uint32_t n = 0; n < NT; ++n) {
-                            float p[4];
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) {
-                                p[i] = ex2_approx(x[h][n][i] + minus_peak[n][i % 2]);
-                                sum[n][i % 2] += p[i];
-                            }
-#pragma unroll
-                            for (uint32_t g = 0; g < kGroups; ++g) {
-                                float weight[4];
-#pragma unroll
-                                for (uint32_t i = 0; i < 4; ++i) {
-                                    const float scale = __uint_as_float(wide[i / 2][2 * g]);
-                                    const float low = __uint_as_float(wide[i / 2][2 * g + 1]);
-                                    const bool seen = !decltype(guarded)::value || x[h][n][i] != -INFINITY;
-                                    lows[g][n][i % 2] = fmaf(p[i], seen ? low : 0.0f, lows[g][n][i % 2]);
-                                    weight[i] = p[i] * (seen ? scale : 0.0f);
-                                }
-                                const uint32_t packed[2] = {Element<false>::pack(weight[0], weight[1]),
-                                                            Element<false>::pack(weight[2], weight[3])};
-                                weights[g][n][0] = transpose_8x8(packed[0]);
-                                weights[g][n][1] = transpose_8x8(packed[1]);
-                            }
+                            lows[g][n] = __ffma2_rn(p[n], make_float2(wide.z, wide.w), lows[g][n]);
+                            const float2 weight = __fmul2_rn(p[n], make_float2(wide.x, wide.y));
+                            weights[g][n][half] = transpose_8x8(Element<false>::pack(weight.x, weight.y));
                         }
-                    };
-                    if (careful)
-                        weigh(std::true_type{});
-                    else
-                        weigh(std::false_type{});
-                    // ---- O^T += V^T . (P scale)^T. Two tokens' nibbles of a channel side by side are a pair of the first
-                    // operand; the odd fragment rows' channels come 16 times too large. Codes count from their middle, 8,
-                    // with 8 * weight in fp32 in `lows`. For one row tile `eights`, a product with a constant, sums 8 * weight
-                    // as rounded, to be taken off at the end; for more, whose registers are full, the codes are made normal
-                    // numbers and 8 is subtracted from them.
-                    if constexpr (kEights) {
+                    }
+                }
+                // ---- O^T += V^T . (P scale)^T. Two tokens' nibbles of a channel side by side are a pair of the first
+                // operand; the odd fragment rows' channels come 16 times too large. Codes count from their middle, 8,
+                // with 8 * weight in fp32 in `lows`. For one row tile `eights`, a product with a constant, sums 8 * weight
+                // as rounded, to be taken off at the end; for more, whose registers are full, the codes are made normal
+                // numbers and 8 is subtracted from them.
+                if constexpr (kEights) {
 #pragma unroll
-                        for (uint32_t g = 0; g < kGroups; ++g)
+                    for (uint32_t g = 0; g < kGroups; ++g)
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n)
+                            mma_16x8x16(eights[g][n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u,
+                                        weights[g][n][0], weights[g][n][1]);
+                }
+                uint32_t v[4][kValueWords];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) load_words(v[i], values + (16 * h + 4 * i + c4) * (D / 2) + l4 * (D / 16));
+#pragma unroll
+                for (uint32_t w = 0; w < kValueWords; ++w)
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; ++half) {
+                        uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
+                        uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (uint32_t byte = 0; byte < 2; ++byte) {
+                            const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
+                            uint32_t codes[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
+                            if constexpr (!kEights) {
+                                codes[0] = add_f16x2(codes[0] | 0x64006400u, 0xe408e408u);  // 1024 + code - 1032
+                                codes[1] = add_f16x2(codes[1] | 0x64006400u, 0xe480e480u);  // 1024 + 16 code - 1152
+                                codes[2] = add_f16x2(codes[2] | 0x64006400u, 0xe408e408u);
+                                codes[3] = add_f16x2(codes[3] | 0x64006400u, 0xe480e480u);
+                            }
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n)
-                                mma_16x8x16(eights[g][n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u,
-                                            weights[g][n][0], weights[g][n][1]);
-                    }
-                    uint32_t v[4][kValueWords];
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i)
-                        load_words(v[i], values + (first_token + 4 * i + c4) * (D / 2) + l4 * (D / 16));
-#pragma unroll
-                    for (uint32_t w = 0; w < kValueWords; ++w)
-#pragma unroll
-                        for (uint32_t half = 0; half < 2; ++half) {
-                            uint32_t lo = __byte_perm(v[0][w], v[1][w], half ? 0x7632 : 0x5410);
-                            uint32_t hi = __byte_perm(v[2][w], v[3][w], half ? 0x7632 : 0x5410);
-#pragma unroll
-                            for (uint32_t byte = 0; byte < 2; ++byte) {
-                                const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
-                                uint32_t codes[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
-                                if constexpr (!kEights) {
-                                    codes[0] = add_f16x2(codes[0] | 0x64006400u, 0xe408e408u);  // 1024 + code - 1032
-                                    codes[1] = add_f16x2(codes[1] | 0x64006400u, 0xe480e480u);  // 1024 + 16 code - 1152
-                                    codes[2] = add_f16x2(codes[2] | 0x64006400u, 0xe408e408u);
-                                    codes[3] = add_f16x2(codes[3] | 0x64006400u, 0xe480e480u);
-                                }
-#pragma unroll
-                                for (uint32_t n = 0; n < NT; ++n)
-                                    mma_16x8x16(out[j][n], codes[0], codes[1], codes[2], codes[3], weights[g][n][0], weights[g][n][1]);
-                                lo >>= 8;
-                                hi >>= 8;
-                            }
+                                mma_16x8x16(out[j][n], codes[0], codes[1], codes[2], codes[3], weights[g][n][0], weights[g][n][1]);
+                            lo >>= 8;
+                            hi >>= 8;
                         }
-                }
+                    }
             }
             __syncwarp();  // every lane is done with the stage and with the wide parameters
             if (unit + 1 == to) break;  // the last stage is given back when the merge is done with it
@@ -1140,10 +1141,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
                 for (uint32_t e = 0; e < 2; ++e) {
-                    float s = sum[n][e];
+                    float s = e ? sum[n].y : sum[n].x;
                     float low[kGroups];
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) low[g] = lows[g][n][e];
+                    for (uint32_t g = 0; g < kGroups; ++g) low[g] = e ? lows[g][n].y : lows[g][n].x;
 #pragma unroll
                     for (uint32_t mask = 4; mask < 32; mask *= 2) {
                         s += __shfl_xor_sync(0xffffffffu, s, mask);
@@ -1163,7 +1164,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         merged[row * kPitch + 16 * j + 8 + l4] = fmaf(odd_y, unfit, low[g]);
                     }
                     if (l4 == 0) {
-                        stats[2 * row] = peak[n][e];
+                        stats[2 * row] = e ? peak[n].y : peak[n].x;
                         stats[2 * row + 1] = s;
                     }
                 }
@@ -1517,7 +1518,6 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
     args.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + counters);
     return for_cache(cache, [&](auto dim, auto group, auto bf16) {
         if (rows <= 8) return launch_attention<dim, group, 1, bf16>(args, facts, stream, device_status);
-        if (rows <= 16) return launch_attention<dim, group, 2, bf16>(args, facts, stream, device_status);
-        return launch_attention<dim, group, 4, bf16>(args, facts, stream, device_status);
+        return launch_attention<dim, group, 2, bf16>(args, facts, stream, device_status);
     });
 }
