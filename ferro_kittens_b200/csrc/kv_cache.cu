@@ -675,58 +675,103 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     };
 
     if (warp >= warps) {
-        // ---- copies, by one thread: tokens that follow each other in a page are one run, copied in bulk, codes and
-        // parameters. (Parameters of runs that do not begin and end on 16 bytes go token by token.) The page of the next
-        // run is asked for before the present one is copied.
-        if (!elect_one()) return;
+        // ---- copies: tokens that follow each other in a page are one run, copied in bulk, codes and parameters. (Parameters
+        // of runs that do not begin and end on 16 bytes go token by token.) Lane r works out run r of a unit; the pages of the
+        // next unit's runs are asked for before the present one's are copied, by one thread after another's numbers.
         const uint32_t side = warp - warps;
-        for (bool more = find_piece(); more; more = next_piece()) {
-            int32_t place = static_cast<int32_t>(from * unit_tokens);
-            uint32_t next_page = page_at(min(place, max(extent.visible() - 1, 0)));
-            for (uint32_t unit = from; unit < to; ++unit, place += unit_tokens) {
-                const uint32_t full = smem_u32(barriers + 2 * stage), memory = smem_u32(ring) + stage * stage_bytes;
-                if (!mbar_wait(full + 8, parity ^ 1, site, kStallFree, unit)) return;
-                const int32_t count = min(extent.visible() - place, static_cast<int32_t>(unit_tokens));
-                uint32_t bytes = 0, bad = 0;
-                bool single = false;
-#pragma unroll 1
-                for (int32_t i = 0; i < count;) {
-                    const uint32_t token = static_cast<uint32_t>(extent.token(place + i));
-                    const uint32_t inside = token - args.page.quotient(token) * args.page_size;
-                    uint32_t run = min(static_cast<uint32_t>(count - i), args.page_size - inside);
-                    if (place + i < extent.kept) run = min(run, static_cast<uint32_t>(extent.kept - place - i));
-                    const uint32_t page = next_page;
-                    const int32_t then = place + i + static_cast<int32_t>(run);
-                    if (then < extent.visible()) next_page = page_at(then);
-                    if (page < args.pages) {
-                        const uint64_t row = (page * args.kv_heads + kv_head) * args.page_size + inside;
-                        const uint32_t param_bytes = run * (kGroups * 4);
+        struct Run {
+            uint32_t entry, inside, at, length;  // page of the sequence, place in it, place in the unit, tokens
+        };
+        const auto run_of = [&](uint32_t unit, uint32_t r, Run& run) {
+            const int32_t place = static_cast<int32_t>(unit * unit_tokens);
+            const int32_t count = min(extent.visible() - place, static_cast<int32_t>(unit_tokens));
+            // Before the gap between sinks and window, and behind it, tokens follow each other.
+            const int32_t front = max(min(extent.kept - place, count), 0);
+            uint32_t base = 0;
 #pragma unroll
-                        for (uint32_t which = 0; which < 2; ++which) {
-                            if (args.copying == 2 && which != side) continue;
-                            bulk_load(memory + which * value_codes + i * (D / 2), args.codes[which] + row * (D / 2), run * (D / 2), full);
-                            bytes += run * (D / 2);
-                            const uint8_t* const params = args.params[which] + row * (kGroups * 4);
-                            const uint32_t params_at = memory + 2 * value_codes + which * warps * Shape::kParamBytes + i * (kGroups * 4);
-                            if (((static_cast<uint32_t>(row * (kGroups * 4)) | params_at | param_bytes) & 15u) == 0) {
-                                bulk_load(params_at, params, param_bytes, full);
-                                bytes += param_bytes;
-                            } else {
-                                single = true;
-#pragma unroll 1
-                                for (uint32_t r = 0; r < param_bytes; r += kGroups * 4)
-                                    copy_async<kGroups * 4>(params_at + r, params + r);
-                            }
-                        }
-                    } else {
-                        bad = 1;
+            for (uint32_t part = 0; part < 2; ++part) {
+                const uint32_t tokens = static_cast<uint32_t>(part ? max(count - front, 0) : front);
+                if (tokens == 0) continue;
+                const uint32_t begin = static_cast<uint32_t>(part ? place + front + extent.skipped : place);
+                const uint32_t first = args.page.quotient(begin), runs = args.page.quotient(begin + tokens - 1) - first + 1;
+                if (r < base + runs) {
+                    run.entry = first + (r - base);
+                    const uint32_t page_begin = run.entry * args.page_size, start = max(begin, page_begin);
+                    run.inside = start - page_begin;
+                    run.length = min(begin + tokens - start, args.page_size - run.inside);
+                    run.at = start - begin + (part ? front : 0);
+                    return true;
+                }
+                base += runs;
+            }
+            return false;
+        };
+        const auto page_of = [&](const Run& run) {
+            return args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + run.entry)) : b;
+        };
+        for (bool more = find_piece(); more; more = next_piece()) {
+            Run run;
+            bool there = run_of(from, lane, run);
+            uint32_t page = there ? page_of(run) : 0;
+            for (uint32_t unit = from; unit < to; ++unit) {
+                const uint32_t full = smem_u32(barriers + 2 * stage), memory = smem_u32(ring) + stage * stage_bytes;
+                Run then;
+                const bool then_there = unit + 1 < to && run_of(unit + 1, lane, then);
+                const uint32_t then_page = then_there ? page_of(then) : 0;
+                if (!mbar_wait(full + 8, parity ^ 1, site, kStallFree, unit)) return;
+                uint32_t bytes = 0;
+                bool bad = false, single = false;
+                for (uint32_t chunk = 32;; chunk += 32) {
+                    const bool sound = there && page < args.pages;
+                    if (there && !sound) {
+                        bad = true;
                         if (side == 0) note(status, kBadPage, b, page);
                     }
-                    i += static_cast<int32_t>(run);
+                    const uint32_t row = (page * args.kv_heads + kv_head) * args.page_size + run.inside;
+                    for (uint32_t left = __ballot_sync(0xffffffffu, sound); left; left &= left - 1) {
+                        const uint32_t lane_of = __ffs(left) - 1;
+                        const uint64_t its_row = __shfl_sync(0xffffffffu, row, lane_of);
+                        const uint32_t at = __shfl_sync(0xffffffffu, run.at, lane_of);
+                        const uint32_t length = __shfl_sync(0xffffffffu, run.length, lane_of);
+                        const uint32_t param_bytes = length * (kGroups * 4);
+                        const bool aligned = ((static_cast<uint32_t>(its_row * (kGroups * 4)) | at * (kGroups * 4) | param_bytes) & 15u) == 0;
+                        const uint32_t moved = length * (D / 2) + (aligned ? param_bytes : 0);
+                        bytes += args.copying == 2 ? moved : 2 * moved;
+                        single |= !aligned;
+                        if (elect_one()) {
+#pragma unroll
+                            for (uint32_t which = 0; which < 2; ++which) {
+                                if (args.copying == 2 && which != side) continue;
+                                bulk_load(memory + which * value_codes + at * (D / 2), args.codes[which] + its_row * (D / 2),
+                                          length * (D / 2), full);
+                                const uint8_t* const params = args.params[which] + its_row * (kGroups * 4);
+                                const uint32_t params_at =
+                                    memory + 2 * value_codes + which * warps * Shape::kParamBytes + at * (kGroups * 4);
+                                if (aligned) {
+                                    bulk_load(params_at, params, param_bytes, full);
+                                } else {
+#pragma unroll 1
+                                    for (uint32_t i = 0; i < param_bytes; i += kGroups * 4)
+                                        copy_async<kGroups * 4>(params_at + i, params + i);
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    there = run_of(unit, chunk + lane, run);
+                    if (!__any_sync(0xffffffffu, there)) break;
+                    page = there ? page_of(run) : 0;
                 }
-                if (side == 0) bad_pages[stage] = bad;
-                if (single) copy_async_arrive(full);
-                mbar_arrive_expect_tx(full, bytes);
+                bad = __any_sync(0xffffffffu, bad);
+                if (elect_one()) {
+                    if (side == 0) bad_pages[stage] = bad;
+                    if (single) copy_async_arrive(full);
+                    mbar_arrive_expect_tx(full, bytes);
+                }
+                __syncwarp();
+                run = then;
+                there = then_there;
+                page = then_page;
                 next_stage();
             }
         }
