@@ -432,16 +432,15 @@ struct AttentionShape {
     // One row tile's queries stay in registers; of more, the fragments and sums lie in shared memory.
     static constexpr bool kSharedQueries = NT > 1;
     static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 : 0;
-    // For each computing warp: its tokens in each stage, and the unit's parameters as floats. The merge of the warps' results
-    // lies over the piece's last stage, which is given back after it, or (where rows are more than fit there) beside.
+    // For each computing warp: its tokens in each stage. The merge of the warps' results lies over the piece's last stage, which
+    // is given back after it, or (where rows are more than fit there) beside.
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
     static constexpr uint32_t kParamBytes = kWarpTokens * kGroups * 4;
     static constexpr uint32_t kStageBytes = 2 * kCodeBytes + 2 * kParamBytes;
-    static constexpr uint32_t kWideBytes = kWarpTokens * kGroups * 16;
     static constexpr uint32_t kPitch = D + 4;  // floats of a merged row: the four columns of a fragment fall in other banks
     static constexpr uint32_t kMergeBytes = kRows * kPitch * 4 + kRows * 8;
     static constexpr bool kMergeInRing = kMergeBytes <= kStageBytes;
-    static constexpr uint32_t kScratchBytes = kMergeInRing || 2 * kWideBytes > kMergeBytes ? 2 * kWideBytes : kMergeBytes;
+    static constexpr uint32_t kScratchBytes = kMergeInRing ? 0 : kMergeBytes;
     static constexpr uint32_t kWarpBytes = kStages * kStageBytes + kScratchBytes;
     // Registers a thread: 128, or 168 for more than one row tile or two groups.
     static constexpr uint32_t kMostThreads = 32 * (NT == 1 && kGroups <= 2 ? 16 : 12);
@@ -845,7 +844,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 for (uint32_t n = warp; n < NT; n += warps) {
                     float sums[kGroups] = {};
                     load_row(n, raw);
-                    convert_row(raw, power_of_two(power), f, sums);
+                    convert_row(raw, args.scale < 0.0f ? -power_of_two(power) : power_of_two(power), f, sums);
 #pragma unroll
                     for (uint32_t w = 0; w < kKeyWords; ++w) shared_q[(n * kKeyWords + w) * 32 + lane] = f[w];
 #pragma unroll
@@ -856,7 +855,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             } else {
                 power = power_for(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(load_row(0, raw)))));
                 float sums[kGroups] = {};
-                convert_row(raw, power_of_two(power), f, sums);
+                convert_row(raw, args.scale < 0.0f ? -power_of_two(power) : power_of_two(power), f, sums);
 #pragma unroll
                 for (uint32_t w = 0; w < kKeyWords; ++w)
                     qf[2 * w][0] = f[w].x, qf[2 * w][1] = f[w].y, qf[2 * w + 1][0] = f[w].z, qf[2 * w + 1][1] = f[w].w;
@@ -866,22 +865,22 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     for (uint32_t e = 0; e < 2; ++e) q_sum[g][e] = __shfl_sync(0xffffffffu, sums[g], 8 * c4 + 4 * e);
             }
         }
-        const float to_log2 = args.scale * 1.4426950408889634f * 0x1p24f * power_of_two(254 - power);
+        // (Zero would make NaN of a hidden token's -inf.)
+        const float to_log2 = fmaxf(fabsf(args.scale) * 1.4426950408889634f * 0x1p24f * power_of_two(254 - power), 1e-37f);
+        const float slack = __fdividef(kSlack, to_log2);
 
-        // Pairs are a fragment's two rows.
+        // Pairs are a fragment's two rows. Scores and peaks are the products' sums; times to_log2 they are powers of two, and
+        // minus_peak is -peak in powers of two, 0 while peak is -inf.
         float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {};
-        float2 lows[kGroups][NT] = {}, peak[NT], minus_peak[NT] = {}, sum[NT] = {};  // minus_peak: 0 while peak is -inf
+        float2 lows[kGroups][NT] = {}, peak[NT], minus_peak[NT] = {}, sum[NT] = {};
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) peak[n] = make_float2(-INFINITY, -INFINITY);
         int32_t top = 0;  // biased exponent of the largest value scale so far
         float fit = power_of_two(254), limit = 0x1p-126f;  // limit: the least scale that would raise top
 
-        // Rows of S^T: the token of fragment row i is i/2 for even i < 8, 4 + i/2 for odd, and 8 further for the rest,
-        // so that the values' loads (tokens c4, 4 + c4, 8 + c4, 12 + c4) touch four neighbouring rows at a time.
-        const uint32_t own_token = (l4 >> 1) + 4 * (l4 & 1);
-        // Of each token and group: (scale, scale, low, low), the keys' times to_log2; the values' scale * fit and low + 8 * scale.
-        float4* const wide_keys = reinterpret_cast<float4*>(ring + kStages * stage_bytes + warp * Shape::kScratchBytes);
-        float4* const wide_values = wide_keys + kWarpTokens * kGroups;
+        // Rows of S^T: the tokens of fragment rows 2c and 2c + 1 are 2c and 2c + 1, in this order for c < 2 and in the other
+        // for the rest, so that neither the keys' loads (both rows at once) nor the values' (one of each c) crowd the same banks.
+        const uint32_t own_token = l4 ^ (l4 >> 2);
 
 #pragma unroll 1
         for (uint32_t unit = from; unit < to; ++unit) {
@@ -890,23 +889,19 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             const uint8_t* const keys = ring + stage * stage_bytes + warp * Shape::kCodeBytes;
             const uint8_t* const values = keys + value_codes;
             const uint8_t* const key_params = ring + stage * stage_bytes + 2 * value_codes + warp * Shape::kParamBytes;
-            const uint8_t* const value_params = key_params + warps * Shape::kParamBytes;
+            uint8_t* const value_params = const_cast<uint8_t*>(key_params) + warps * Shape::kParamBytes;
             // Whether some row may not see some of the 32 tokens (they rise from place to place), or some are not there.
             const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens), here = extent.visible() - place;
             const bool is_masked = here < 32 || bad_pages[stage] || extent.token(place + 31) > extent.first ||
                                    (args.window && extent.token(place + 31) >= args.sinks &&
                                     extent.token(place) <= extent.length - 1 - args.window);
 
-            // ---- parameters as floats, each twice, lane = token, for packed arithmetic on a fragment's two rows.
-            uint32_t key_pairs[kGroups], value_pairs[kGroups];
-            float widest = 0.0f;
-            load_words(key_pairs, key_params + lane * (kGroups * 4));
-            load_words(value_pairs, value_params + lane * (kGroups * 4));
+            float widest = 0.0f;  // of the value scales, lane = token
+            {
+                uint32_t pairs[kGroups];
+                load_words(pairs, value_params + lane * (kGroups * 4));
 #pragma unroll
-            for (uint32_t g = 0; g < kGroups; ++g) {
-                const float scale = E::low(key_pairs[g]) * to_log2, low = E::high(key_pairs[g]) * to_log2;
-                wide_keys[lane * kGroups + g] = make_float4(scale, scale, low, low);
-                widest = fmaxf(widest, fabsf(E::low(value_pairs[g])));
+                for (uint32_t g = 0; g < kGroups; ++g) widest = fmaxf(widest, fabsf(E::low(pairs[g])));
             }
 
             // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
@@ -934,10 +929,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 for (uint32_t half = 0; half < 2; ++half)
                     load_words(a[half], keys + (16 * h + 8 * half + own_token) * (D / 2) + c4 * (D / 8));
             };
-            const auto add_up = [&](uint32_t h, uint32_t g, const float (&part)[NT][4]) {
+            const auto add_up = [&](uint32_t h, uint32_t g, const uint32_t (&pairs)[2][kGroups], const float (&part)[NT][4]) {
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
-                    const float4 wide = wide_keys[(16 * h + 8 * half + own_token) * kGroups + g];
+                    const float scale = E::low(pairs[half][g]), low = E::high(pairs[half][g]);
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n) {
                         float2 sums;
@@ -945,39 +940,24 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             sums = *reinterpret_cast<const float2*>(shared_sums + g * kRows + 8 * n + 2 * c4);
                         else
                             sums = make_float2(q_sum[g][0], q_sum[g][1]);
-                        const float2 low = make_float2(wide.z, wide.w);
-                        const float2 rest = g == 0 ? __fmul2_rn(low, sums) : __ffma2_rn(low, sums, x[h][n][half]);
-                        x[h][n][half] = __ffma2_rn(make_float2(wide.x, wide.y),
-                                                   make_float2(part[n][2 * half], part[n][2 * half + 1]), rest);
+                        float2& y = x[h][n][half];
+                        y.x = fmaf(scale, part[n][2 * half], g == 0 ? low * sums.x : fmaf(low, sums.x, y.x));
+                        y.y = fmaf(scale, part[n][2 * half + 1], g == 0 ? low * sums.y : fmaf(low, sums.y, y.y));
                     }
                 }
             };
-            if constexpr (NT == 1) {  // all products first: the parameters' way through shared memory hides behind them
-                float part[2][kGroups][NT][4] = {};
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    uint32_t a[2][kKeyWords];
-                    load_keys(h, a);
+            for (uint32_t h = 0; h < 2; ++h) {
+                uint32_t a[2][kKeyWords], pairs[2][kGroups];
+                load_keys(h, a);
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) products(h, g, a, part[h][g]);
-                }
-                __syncwarp();
+                for (uint32_t half = 0; half < 2; ++half)
+                    load_words(pairs[half], key_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) add_up(h, g, part[h][g]);
-            } else {
-                __syncwarp();
-#pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    uint32_t a[2][kKeyWords];
-                    load_keys(h, a);
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) {
-                        float part[NT][4] = {};
-                        products(h, g, a, part);
-                        add_up(h, g, part);
-                    }
+                for (uint32_t g = 0; g < kGroups; ++g) {
+                    float part[NT][4] = {};
+                    products(h, g, a, part);
+                    add_up(h, g, pairs, part);
                 }
             }
 
@@ -994,7 +974,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             };
             look();
 #pragma unroll
-            for (uint32_t n = 0; n < NT; ++n) grows |= largest[n].x > peak[n].x + kSlack || largest[n].y > peak[n].y + kSlack;
+            for (uint32_t n = 0; n < NT; ++n) grows |= largest[n].x > peak[n].x + slack || largest[n].y > peak[n].y + slack;
             if (is_masked || __any_sync(0xffffffffu, grows)) {
                 if (is_masked) {
                     uint32_t real = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1;
@@ -1016,14 +996,15 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         }
                     // Values that are not finite make NaN of the groups of the rows that see them, and of no others: a
                     // weight of zero would make NaN of them too.
+                    uint32_t pairs[kGroups];
+                    load_words(pairs, value_params + lane * (kGroups * 4));
                     bool finite = true;
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; ++g) {
-                        if (!(real >> lane & 1u)) value_pairs[g] = 0;
-                        finite = finite && E::finite(value_pairs[g]);
+                        if (!(real >> lane & 1u)) pairs[g] = 0;
+                        finite = finite && E::finite(pairs[g]);
                     }
-                    const uint32_t sound = __ballot_sync(0xffffffffu, finite);
-                    if (sound != 0xffffffffu) {
+                    if (!__all_sync(0xffffffffu, finite)) {
 #pragma unroll
                         for (uint32_t g = 0; g < kGroups; ++g) {
 #pragma unroll
@@ -1037,19 +1018,27 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                                         if (x[k / 2][n][k % 2].y != -INFINITY) lows[g][n].y = __uint_as_float(0x7fffffffu);
                                     }
                             }
-                            if (!E::finite(value_pairs[g])) value_pairs[g] = 0;
+                            if (!E::finite(pairs[g])) pairs[g] = 0;
                         }
                     }
+                    __syncwarp();
                     widest = 0.0f;
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) widest = fmaxf(widest, fabsf(E::low(value_pairs[g])));
+                    for (uint32_t g = 0; g < kGroups; ++g) {
+                        reinterpret_cast<uint32_t*>(value_params)[lane * kGroups + g] = pairs[g];
+                        widest = fmaxf(widest, fabsf(E::low(pairs[g])));
+                    }
+                    fence_proxy_async_shared();  // what is copied there next comes by another way than these stores
+                    __syncwarp();
                     look();
                 }
                 if (!(widest < INFINITY)) {  // an infinity says nothing about the others
+                    uint32_t pairs[kGroups];
+                    load_words(pairs, value_params + lane * (kGroups * 4));
                     widest = 0.0f;
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; ++g)
-                        if (E::finite(value_pairs[g])) widest = fmaxf(widest, fabsf(E::low(value_pairs[g])));
+                        if (E::finite(pairs[g])) widest = fmaxf(widest, fabsf(E::low(pairs[g])));
                 }
                 const int32_t unit_top = static_cast<int32_t>(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23);
                 float shrink = 1.0f;
@@ -1067,12 +1056,12 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 4));
                         m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 8));
                         m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 16));
-                        keep[e] = m[e] > was[e] ? ex2_approx(was[e] - m[e]) : 1.0f;
+                        keep[e] = m[e] > was[e] ? ex2_approx((was[e] - m[e]) * to_log2) : 1.0f;
                         m[e] = fmaxf(m[e], was[e]);
                     }
                     peak[n] = make_float2(m[0], m[1]);
                     // While a row has seen nothing its scores are -inf: so are its exponents, with nothing taken off.
-                    minus_peak[n] = make_float2(m[0] == -INFINITY ? 0.0f : -m[0], m[1] == -INFINITY ? 0.0f : -m[1]);
+                    minus_peak[n] = make_float2(m[0] == -INFINITY ? 0.0f : -m[0] * to_log2, m[1] == -INFINITY ? 0.0f : -m[1] * to_log2);
                     const float2 keep2 = make_float2(keep[0], keep[1]);
                     sum[n] = __fmul2_rn(sum[n], keep2);
 #pragma unroll
@@ -1091,32 +1080,28 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             }
 
 #pragma unroll
-            for (uint32_t g = 0; g < kGroups; ++g) {
-                const float scale = E::low(value_pairs[g]), low = fmaf(8.0f, scale, E::high(value_pairs[g]));
-                wide_values[lane * kGroups + g] = make_float4(scale * fit, scale * fit, low, low);
-            }
-            __syncwarp();
-#pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
                 // ---- weights, their sums, and weight * scale in fp16, turned to be the values' second operand.
                 uint32_t weights[kGroups][NT][2];
 #pragma unroll
                 for (uint32_t half = 0; half < 2; ++half) {
                     float2 p[NT];
+                    uint32_t pairs[kGroups];
+                    load_words(pairs, value_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n) {
-                        const float2 power = __fadd2_rn(x[h][n][half], minus_peak[n]);
+                        const float2 power = __ffma2_rn(x[h][n][half], make_float2(to_log2, to_log2), minus_peak[n]);
                         p[n] = make_float2(ex2_approx(power.x), ex2_approx(power.y));
                         sum[n] = __fadd2_rn(sum[n], p[n]);
                     }
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; ++g) {
-                        const float4 wide = wide_values[(16 * h + 8 * half + own_token) * kGroups + g];
+                        const float scale = E::low(pairs[g]), fitted = scale * fit, low = fmaf(8.0f, scale, E::high(pairs[g]));
 #pragma unroll
                         for (uint32_t n = 0; n < NT; ++n) {
-                            lows[g][n] = __ffma2_rn(p[n], make_float2(wide.z, wide.w), lows[g][n]);
-                            const float2 weight = __fmul2_rn(p[n], make_float2(wide.x, wide.y));
-                            weights[g][n][half] = transpose_8x8(Element<false>::pack(weight.x, weight.y));
+                            lows[g][n].x = fmaf(p[n].x, low, lows[g][n].x);
+                            lows[g][n].y = fmaf(p[n].y, low, lows[g][n].y);
+                            weights[g][n][half] = transpose_8x8(Element<false>::pack(p[n].x * fitted, p[n].y * fitted));
                         }
                     }
                 }
@@ -1135,7 +1120,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 }
                 uint32_t v[4][kValueWords];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) load_words(v[i], values + (16 * h + 4 * i + c4) * (D / 2) + l4 * (D / 16));
+                for (uint32_t i = 0; i < 4; ++i) load_words(v[i], values + (16 * h + 8 * (i / 2) + 2 * c4 + ((i ^ (c4 >> 1)) & 1u)) * (D / 2) + l4 * (D / 16));
 #pragma unroll
                 for (uint32_t w = 0; w < kValueWords; ++w)
 #pragma unroll
@@ -1160,7 +1145,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         }
                     }
             }
-            __syncwarp();  // every lane is done with the stage and with the wide parameters
+            __syncwarp();  // every lane is done with the stage
             if (unit + 1 == to) break;  // the last stage is given back when the merge is done with it
             if (lane == 0) mbar_arrive(full + 8);
             next_stage();
@@ -1209,7 +1194,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         merged[row * kPitch + 16 * j + 8 + l4] = fmaf(odd_y, unfit, low[g]);
                     }
                     if (l4 == 0) {
-                        stats[2 * row] = e ? peak[n].y : peak[n].x;
+                        stats[2 * row] = (e ? peak[n].y : peak[n].x) * to_log2;
                         stats[2 * row + 1] = s;
                     }
                 }
