@@ -778,7 +778,60 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     }
 
     const uint32_t l4 = lane / 4, c4 = lane % 4;
-    for (bool more = find_piece(); more; more = next_piece()) {
+    const auto load_row = [&](uint32_t n, uint4 (&raw)[kKeyWords]) {
+        const uint32_t r = first_row + 8 * n + l4, t = args.ratio.quotient(min(r, args.rows - 1));
+        const uint8_t* const q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
+                                 (kv_head * args.ratio.divisor + (r - t * args.ratio.divisor)) * args.q_head_stride;
+        float most = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kKeyWords; ++w) {
+            raw[w] = r < args.rows ? __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4) : make_uint4(0, 0, 0, 0);
+            const uint32_t words[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
+        }
+        return most < INFINITY ? most : 0.0f;  // a row that holds an infinity says nothing about others
+    };
+    // The parts of a piece's rows (`parts` of them, `pitch` bytes apart, rows of kPitch floats, then each row's reference and sum)
+    // put together: by each block its warps' parts, and by the block that comes last to a segment the blocks'.
+    const auto put_together = [&](uint8_t* memory, uint32_t pitch, const Cut& piece, float* part) {
+        const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
+        // A warp for each row: the parts' shares of it, left in the place of their references.
+        for (uint32_t row = warp; row < rows_here; row += warps) {
+            float2* const its = reinterpret_cast<float2*>(memory + min(lane, warps - 1) * pitch + kRows * kPitch * 4) + row;
+            const float2 stat = lane < warps ? *its : make_float2(-INFINITY, 0.0f);
+            float m = stat.x;
+#pragma unroll
+            for (uint32_t mask = 16; mask > 0; mask >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, mask));
+            const float factor = stat.x == -INFINITY ? 0.0f : ex2_approx(stat.x - m);
+            float total = stat.y * factor;
+#pragma unroll
+            for (uint32_t mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
+            if (lane < warps) its->x = factor;
+            if (lane == 0) row_stats[row] = make_float2(m, total);
+        }
+        sync_computing(warps * 32);
+        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
+            const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (uint32_t w = 0; w < warps; ++w) {
+                const float* const its = reinterpret_cast<const float*>(memory + w * pitch);
+                const float factor = its[kRows * kPitch + 2 * row];
+                const float4 z = *reinterpret_cast<const float4*>(its + row * kPitch + d);
+                y = make_float4(fmaf(z.x, factor, y.x), fmaf(z.y, factor, y.y), fmaf(z.z, factor, y.z), fmaf(z.w, factor, y.w));
+            }
+            if (!part) {
+                finish_row<D, BF16>(args, piece, row, d, y, row_stats[row]);
+            } else {
+                *reinterpret_cast<float4*>(part + row * D + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
+            }
+        }
+    };
+
+    bool more = find_piece();
+    while (more) {
         // ---- queries as the second operand of the scores' product: lane (l4, c4) holds row l4 of each 8, in the
         // channel order of the key codes. The tile is scaled by a power of two so that its largest value lies in
         // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second register of each pair carries 1/16 for
@@ -788,20 +841,6 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         float q_sum[Shape::kSharedQueries ? 1 : kGroups][2];
         uint4* const shared_q = reinterpret_cast<uint4*>(shared);
         float* const shared_sums = reinterpret_cast<float*>(shared + kRows * D * 2);
-        const auto load_row = [&](uint32_t n, uint4 (&raw)[kKeyWords]) {
-            const uint32_t r = first_row + 8 * n + l4, t = args.ratio.quotient(min(r, args.rows - 1));
-            const uint8_t* const q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
-                                     (kv_head * args.ratio.divisor + (r - t * args.ratio.divisor)) * args.q_head_stride;
-            float most = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < kKeyWords; ++w) {
-                raw[w] = r < args.rows ? __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4) : make_uint4(0, 0, 0, 0);
-                const uint32_t words[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
-            }
-            return most < INFINITY ? most : 0.0f;  // a row that holds an infinity says nothing about others
-        };
         const auto power_for = [](float most) {
             return most == 0.0f ? 127 : min(268 - static_cast<int32_t>(__float_as_uint(most) >> 23), 254);
         };
@@ -892,6 +931,12 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             uint8_t* const value_params = const_cast<uint8_t*>(key_params) + warps * Shape::kParamBytes;
             // Whether some row may not see some of the 32 tokens (they rise from place to place), or some are not there.
             const int32_t place = static_cast<int32_t>(unit * unit_tokens + warp * kWarpTokens), here = extent.visible() - place;
+            if (here <= 0) {  // nothing of the unit is this warp's
+                if (unit + 1 == to) break;
+                if (lane == 0) mbar_arrive(full + 8);
+                next_stage();
+                continue;
+            }
             const bool is_masked = here < 32 || bad_pages[stage] || extent.token(place + 31) > extent.first ||
                                    (args.window && extent.token(place + 31) >= args.sinks &&
                                     extent.token(place) <= extent.length - 1 - args.window);
@@ -1199,44 +1244,13 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     }
                 }
         }
-        sync_computing(warps * 32);
-        const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
-        // A warp for each row: the warps' shares of it, left in the place of their references.
-        for (uint32_t row = warp; row < rows_here; row += warps) {
-            float2* const its = reinterpret_cast<float2*>(merge_memory + min(lane, warps - 1) * merge_pitch + kRows * kPitch * 4) + row;
-            const float2 stat = lane < warps ? *its : make_float2(-INFINITY, 0.0f);
-            float m = stat.x;
-#pragma unroll
-            for (uint32_t mask = 16; mask > 0; mask >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, mask));
-            const float factor = stat.x == -INFINITY ? 0.0f : ex2_approx(stat.x - m);
-            float s = stat.y * factor;
-#pragma unroll
-            for (uint32_t mask = 16; mask > 0; mask >>= 1) s += __shfl_xor_sync(0xffffffffu, s, mask);
-            if (lane < warps) its->x = factor;
-            if (lane == 0) row_stats[row] = make_float2(m, s);
-        }
+        more = next_piece();
         sync_computing(warps * 32);
         // A part of a segment that is cut over blocks: the block its first unit lies in keeps it in its second place, the others in
         // their first. Parts are handed in together at the end.
-        float* const part = args.partials + (2 * blockIdx.x + which) * static_cast<size_t>(kPartialFloats);
         if (piece.parts && threadIdx.x == 0) cuts[which] = piece;
-        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
-            const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (uint32_t w = 0; w < warps; ++w) {
-                const float* const its = reinterpret_cast<const float*>(merge_memory + w * merge_pitch);
-                const float factor = its[kRows * kPitch + 2 * row];
-                const float4 z = *reinterpret_cast<const float4*>(its + row * kPitch + d);
-                y = make_float4(fmaf(z.x, factor, y.x), fmaf(z.y, factor, y.y), fmaf(z.z, factor, y.z), fmaf(z.w, factor, y.w));
-            }
-            if (piece.parts == 0) {
-                finish_row<D, BF16>(args, piece, row, d, y, row_stats[row]);
-            } else {
-                *reinterpret_cast<float4*>(part + row * D + d) = y;
-                if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
-            }
-        }
+        put_together(merge_memory, merge_pitch, piece,
+                     piece.parts ? args.partials + (2 * blockIdx.x + which) * static_cast<size_t>(kPartialFloats) : nullptr);
         // Copies to where the merged rows lay come by another way than these reads.
         fence_proxy_async_shared();
         sync_computing(warps * 32);
@@ -1265,44 +1279,50 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         }
     }
     sync_computing(warps * 32);
+    uint8_t* const memory = Shape::kMergeInRing ? ring : ring + kStages * stage_bytes;
+    constexpr uint32_t kMergePitch = Shape::kMergeInRing ? Shape::kStageBytes : Shape::kScratchBytes;
     for (uint32_t c = 0; c < 2; ++c) {
         if (!complete[c]) continue;
         const Cut piece = cuts[c];
         const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
-        const float* const base = args.partials + 2 * piece.owner * static_cast<size_t>(kPartialFloats);
-        for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
-            const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float2 all = make_float2(-INFINITY, 0.0f);
-            constexpr uint32_t kBatch = 4;
-#pragma unroll 1
-            for (uint32_t p = 0; p < piece.parts; p += kBatch) {
-                float4 z[kBatch];
-                float2 stat[kBatch];
+        // Warp w puts parts w, w + warps, ... together; a lane's loads of a part are all on their way at once.
+        constexpr uint32_t kItems = kRows * D / 128;
+        float4 y[kItems] = {};
+        float2 all[kItems];
 #pragma unroll
-                for (uint32_t k = 0; k < kBatch; ++k) {
-                    const uint32_t q = min(p + k, piece.parts - 1);
-                    const float* const its = base + (2 * q + (q == 0)) * static_cast<size_t>(kPartialFloats);
+        for (uint32_t k = 0; k < kItems; ++k) all[k] = make_float2(-INFINITY, 0.0f);
+        for (uint32_t p = warp; p < piece.parts; p += warps) {
+            const float* const its = args.partials + (2 * (piece.owner + p) + (p == 0)) * static_cast<size_t>(kPartialFloats);
+            float4 z[kItems];
+            float2 stat[kItems];
+#pragma unroll
+            for (uint32_t k = 0; k < kItems; ++k) {
+                const uint32_t row = (lane + 32 * k) / (D / 4), d = (lane + 32 * k) % (D / 4) * 4;
+                stat[k] = make_float2(-INFINITY, 0.0f);
+                if (row < rows_here) {
                     stat[k] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
                     z[k] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
                 }
-                float m = all.x;
-#pragma unroll
-                for (uint32_t k = 0; k < kBatch; ++k) m = fmaxf(m, stat[k].x);
-                const float keep = all.x == -INFINITY ? 0.0f : ex2_approx(all.x - m);
-                y = make_float4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
-                all = make_float2(m, all.y * keep);
-#pragma unroll
-                for (uint32_t k = 0; k < kBatch; ++k) {
-                    if (p + k >= piece.parts || stat[k].x == -INFINITY) continue;
-                    const float factor = ex2_approx(stat[k].x - m);
-                    y = make_float4(fmaf(z[k].x, factor, y.x), fmaf(z[k].y, factor, y.y), fmaf(z[k].z, factor, y.z),
-                                    fmaf(z[k].w, factor, y.w));
-                    all.y = fmaf(stat[k].y, factor, all.y);
-                }
             }
-            finish_row<D, BF16>(args, piece, row, d, y, all);
+#pragma unroll
+            for (uint32_t k = 0; k < kItems; ++k) {
+                if (stat[k].x == -INFINITY) continue;
+                const float m = fmaxf(all[k].x, stat[k].x), keep = ex2_approx(all[k].x - m), factor = ex2_approx(stat[k].x - m);
+                y[k] = make_float4(fmaf(z[k].x, factor, y[k].x * keep), fmaf(z[k].y, factor, y[k].y * keep),
+                                   fmaf(z[k].z, factor, y[k].z * keep), fmaf(z[k].w, factor, y[k].w * keep));
+                all[k] = make_float2(m, fmaf(stat[k].y, factor, all[k].y * keep));
+            }
         }
+        float* const merged = reinterpret_cast<float*>(memory + warp * kMergePitch);
+#pragma unroll
+        for (uint32_t k = 0; k < kItems; ++k) {
+            const uint32_t row = (lane + 32 * k) / (D / 4), d = (lane + 32 * k) % (D / 4) * 4;
+            *reinterpret_cast<float4*>(merged + row * kPitch + d) = y[k];
+            if (d == 0) *reinterpret_cast<float2*>(merged + kRows * kPitch + 2 * row) = all[k];
+        }
+        sync_computing(warps * 32);
+        put_together(memory, kMergePitch, piece, nullptr);
+        sync_computing(warps * 32);
     }
     // After a wait that gave up, copies may still be on their way: give them a while before the block's memory goes.
     if (stop_flag)
