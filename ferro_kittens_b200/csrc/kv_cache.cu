@@ -402,8 +402,8 @@ struct AttentionArguments {
     uint32_t rows, row_tiles;  // query rows of a (sequence, kv head): queries * heads / kv_heads
     float scale;
     int32_t window, sinks;
-    Divider page, ratio;
-    uint32_t least_units;   // units a block takes before another block is put to work
+    Divider page, ratio, unit, tiles;  // by page_size, heads / kv_heads, a unit's tokens, row_tiles
+    uint32_t least_units;   // units a block takes before another block is put to work, as a power of two
     uint32_t segment_cost;  // what beginning and ending a segment takes, in units
     uint32_t copying;       // warps that copy
     uint32_t* arrivals;    // workspace: a counter for each block, then the partial results
@@ -568,7 +568,6 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     __shared__ uint32_t stop_flag, complete[2];
     __shared__ Cut cuts[2];              // the parts of segments that are cut over blocks: the one this share begins in, ends in
     __shared__ uint32_t tile_most[NT];   // largest magnitudes of the tile's queries
-    __shared__ float2 row_stats[kRows];  // reference and sum of each row over the warps
     // The first warps compute, the last one or two copy: keys and values, or one side each.
     const uint32_t warps = blockDim.x / 32 - args.copying, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
@@ -581,12 +580,12 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     // goes through the lengths by itself.
     const uint32_t segments = args.kv_heads * args.row_tiles;  // of one sequence
     const auto cost_of = [&](const Extent& e) {
-        return max((static_cast<uint32_t>(e.visible()) + unit_tokens - 1) / unit_tokens, 1u) + args.segment_cost;
+        return max(args.unit.quotient(static_cast<uint32_t>(e.visible()) + unit_tokens - 1), 1u) + args.segment_cost;
     };
     uint32_t mine = lane < args.batch ? cost_of(extent_of(args, lane, status)) : 0, total = mine;
     for (uint32_t i = lane + 32; i < args.batch; i += 32) total += cost_of(extent_of(args, i, status));
     total = __reduce_add_sync(0xffffffffu, total) * segments;
-    const uint32_t blocks = min(gridDim.x, max(total / args.least_units, 1u));
+    const uint32_t blocks = min(gridDim.x, max(total >> args.least_units, 1u));
     if (blockIdx.x >= blocks) return;
     // The first `longer` blocks take a unit more than the others.
     const uint32_t share = total / blocks, longer = total - share * blocks;
@@ -642,7 +641,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             from = offset > args.segment_cost ? offset - args.segment_cost : 0;
             to = offset + length > args.segment_cost ? offset + length - args.segment_cost : 0;
             if (from < to) {
-                kv_head = segment / args.row_tiles;
+                kv_head = args.tiles.quotient(segment);
                 first_row = (segment - kv_head * args.row_tiles) * kRows;
                 return true;
             }
@@ -792,40 +791,42 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         }
         return most < INFINITY ? most : 0.0f;  // a row that holds an infinity says nothing about others
     };
+    // A piece's queries, on their way to the nearest cache while the piece before is put together.
+    const auto fetch_rows = [&]() {
+        for (uint32_t r = first_row + warp; r < min(first_row + kRows, args.rows); r += warps) {
+            const uint32_t t = args.ratio.quotient(r);
+            const uint8_t* const q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
+                                     (kv_head * args.ratio.divisor + (r - t * args.ratio.divisor)) * args.q_head_stride;
+            if (lane < D / 64) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + lane * 128));
+        }
+    };
     // The parts of a piece's rows (`parts` of them, `pitch` bytes apart, rows of kPitch floats, then each row's reference and sum)
     // put together: by each block its warps' parts, and by the block that comes last to a segment the blocks'.
     const auto put_together = [&](uint8_t* memory, uint32_t pitch, const Cut& piece, float* part) {
         const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
-        // A warp for each row: the parts' shares of it, left in the place of their references.
-        for (uint32_t row = warp; row < rows_here; row += warps) {
-            float2* const its = reinterpret_cast<float2*>(memory + min(lane, warps - 1) * pitch + kRows * kPitch * 4) + row;
-            const float2 stat = lane < warps ? *its : make_float2(-INFINITY, 0.0f);
-            float m = stat.x;
-#pragma unroll
-            for (uint32_t mask = 16; mask > 0; mask >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, mask));
-            const float factor = stat.x == -INFINITY ? 0.0f : ex2_approx(stat.x - m);
-            float total = stat.y * factor;
-#pragma unroll
-            for (uint32_t mask = 16; mask > 0; mask >>= 1) total += __shfl_xor_sync(0xffffffffu, total, mask);
-            if (lane < warps) its->x = factor;
-            if (lane == 0) row_stats[row] = make_float2(m, total);
-        }
-        sync_computing(warps * 32);
         for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
             const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+            const auto stat_of = [&](uint32_t w) {
+                return reinterpret_cast<const float2*>(memory + w * pitch + kRows * kPitch * 4)[row];
+            };
+            float2 stat = make_float2(-INFINITY, 0.0f);
+#pragma unroll 4
+            for (uint32_t w = 0; w < warps; ++w) stat.x = fmaxf(stat.x, stat_of(w).x);
+            const float minus = stat.x == -INFINITY ? 0.0f : -stat.x;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
             for (uint32_t w = 0; w < warps; ++w) {
-                const float* const its = reinterpret_cast<const float*>(memory + w * pitch);
-                const float factor = its[kRows * kPitch + 2 * row];
-                const float4 z = *reinterpret_cast<const float4*>(its + row * kPitch + d);
+                const float2 its = stat_of(w);
+                const float factor = ex2_approx(its.x + minus);
+                const float4 z = *reinterpret_cast<const float4*>(memory + w * pitch + (row * kPitch + d) * 4);
                 y = make_float4(fmaf(z.x, factor, y.x), fmaf(z.y, factor, y.y), fmaf(z.z, factor, y.z), fmaf(z.w, factor, y.w));
+                stat.y = fmaf(its.y, factor, stat.y);
             }
             if (!part) {
-                finish_row<D, BF16>(args, piece, row, d, y, row_stats[row]);
+                finish_row<D, BF16>(args, piece, row, d, y, stat);
             } else {
                 *reinterpret_cast<float4*>(part + row * D + d) = y;
-                if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = row_stats[row];
+                if (d == 0) *reinterpret_cast<float2*>(part + kMostRows * 128 + 2 * row) = stat;
             }
         }
     };
@@ -1245,6 +1246,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 }
         }
         more = next_piece();
+        if (more) fetch_rows();
         sync_computing(warps * 32);
         // A part of a segment that is cut over blocks: the block its first unit lies in keeps it in its second place, the others in
         // their first. Parts are handed in together at the end.
@@ -1285,6 +1287,35 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         if (!complete[c]) continue;
         const Cut piece = cuts[c];
         const uint32_t rows_here = min(kRows, args.rows - piece.first_row);
+        constexpr uint32_t kFew = 4;
+        if (piece.parts <= kFew) {  // one thread for four channels, all parts on their way at once
+            for (uint32_t i = threadIdx.x; i < rows_here * (D / 4); i += warps * 32) {
+                const uint32_t row = i / (D / 4), d = i % (D / 4) * 4;
+                float4 z[kFew];
+                float2 stat[kFew], all = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (uint32_t p = 0; p < kFew; ++p) {
+                    const float* const its = args.partials + (2 * (piece.owner + min(p, piece.parts - 1)) + (p == 0)) *
+                                                                 static_cast<size_t>(kPartialFloats);
+                    stat[p] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
+                    z[p] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
+                    if (p >= piece.parts) stat[p] = make_float2(-INFINITY, 0.0f);
+                    all.x = fmaxf(all.x, stat[p].x);
+                }
+                const float minus = all.x == -INFINITY ? 0.0f : -all.x;
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (uint32_t p = 0; p < kFew; ++p) {
+                    if (p >= piece.parts) continue;
+                    const float factor = ex2_approx(stat[p].x + minus);
+                    y = make_float4(fmaf(z[p].x, factor, y.x), fmaf(z[p].y, factor, y.y), fmaf(z[p].z, factor, y.z),
+                                    fmaf(z[p].w, factor, y.w));
+                    all.y = fmaf(stat[p].y, factor, all.y);
+                }
+                finish_row<D, BF16>(args, piece, row, d, y, all);
+            }
+            continue;
+        }
         // Warp w puts parts w, w + warps, ... together; a lane's loads of a part are all on their way at once.
         constexpr uint32_t kItems = kRows * D / 128;
         float4 y[kItems] = {};
@@ -1484,7 +1515,9 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     const uint32_t warps = alone ? Shape::most_warps(2) : half < Shape::kMostByMemory / 2 ? half : Shape::kMostByMemory / 2;
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (alone ? 1 : 2);
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
-    args.least_units = 3;
+    args.least_units = 1;
+    args.unit = cache::Divider(static_cast<uint32_t>(unit_tokens));
+    args.tiles = cache::Divider(args.row_tiles);
     args.segment_cost = 1;
     const uint64_t most_units = segments * ((static_cast<uint64_t>(args.table_pages) * args.page_size + unit_tokens - 1) / unit_tokens + args.segment_cost);
     if (most_units >= (1ull << 31))
