@@ -412,7 +412,7 @@ struct AttentionArguments {
 
 constexpr uint32_t kWarpTokens = 32;
 constexpr uint32_t kStages = 3;
-constexpr uint32_t kMostBlocksPerSm = 4;
+constexpr uint32_t kMostBlocksPerSm = 3;
 constexpr uint32_t kMostRows = 16;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
 constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
@@ -531,6 +531,14 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[WORDS], const void* fro
     } else {
         w[0] = *static_cast<const uint32_t*>(from);
     }
+}
+
+/// One more at `counter`: what the block wrote before its last rendezvous comes first for whoever counts on, and what those that
+/// counted before wrote comes first for this block's next one.
+__device__ __forceinline__ uint32_t arrive(uint32_t* counter) {
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
 }
 
 /// A piece of a segment (of its first row's tile), and if blocks share the segment, in how many parts and which block keeps count.
@@ -1266,18 +1274,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     if (threadIdx.x == 0) {
         complete[0] = complete[1] = 0;
         if (cuts[0].parts || cuts[1].parts) {
-            __threadfence();
             uint32_t came[2] = {};
 #pragma unroll
             for (uint32_t c = 0; c < 2; ++c)
-                if (cuts[c].parts) came[c] = atomicAdd(args.arrivals + cuts[c].owner, 1u);
+                if (cuts[c].parts) came[c] = arrive(args.arrivals + cuts[c].owner);
 #pragma unroll
             for (uint32_t c = 0; c < 2; ++c)
                 if (cuts[c].parts && came[c] == cuts[c].parts - 1) {
                     args.arrivals[cuts[c].owner] = 0;
                     complete[c] = 1;
                 }
-            __threadfence();
         }
     }
     sync_computing(warps * 32);
@@ -1509,11 +1515,18 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     if (admitted != FK_OK) return admitted;
     args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
-    const bool alone = segments < 2ull * facts.sm_count;
-    args.copying = alone ? 2 : 1;
-    const uint32_t half = Shape::kMostThreads / 64 - 1;
-    const uint32_t warps = alone ? Shape::most_warps(2) : half < Shape::kMostByMemory / 2 ? half : Shape::kMostByMemory / 2;
-    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * (alone ? 1 : 2);
+    // How many warps share a piece. One block an SM, of all the warps it holds, leaves the fewest parts to put together: for
+    // segments fewer than the SMs, or than twice the SMs and long. Smaller blocks overlap one's beginnings and ends with others'
+    // units: two an SM while each can take a whole segment, three beyond. (128-wide heads, 8 rows, groups of 64: 256 segments of
+    // 15000 tokens 135 us against 143 with two blocks; 296 of 2000 27.6 us with two, 34.2 with three, 35.5 with one; 384 of
+    // 2000 39.6 with three, 42.0 with two; 1024 of 300 30.3 with three, 35.0 with two, 47.9 with one.)
+    const uint64_t sms = static_cast<uint64_t>(facts.sm_count);
+    const bool lengthy = static_cast<uint64_t>(args.table_pages) * args.page_size > 8192;
+    const uint32_t share = segments <= sms || (lengthy && segments < 2 * sms) ? 1 : segments <= 2 * sms ? 2 : 3;
+    args.copying = share == 1 ? 2 : 1;
+    const uint32_t by_threads = Shape::kMostThreads / 32 / share - args.copying, by_memory = Shape::kMostByMemory / share;
+    const uint32_t warps = by_threads < by_memory ? by_threads : by_memory;
+    const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * share;
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
     args.least_units = 1;
     args.unit = cache::Divider(static_cast<uint32_t>(unit_tokens));
