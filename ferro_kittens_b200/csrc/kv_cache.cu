@@ -405,7 +405,7 @@ struct AttentionArguments {
     Divider page, ratio, unit, tiles;  // by page_size, heads / kv_heads, a unit's tokens, row_tiles
     uint32_t least_units;   // units a block takes before another block is put to work, as a power of two
     uint32_t segment_cost;  // what beginning and ending a segment takes, in units
-    uint32_t copying;       // warps that copy
+    uint32_t copying;       // warps that copy: 1, 2 (a side each) or 4 (every other run of a side each)
     uint32_t* arrivals;    // workspace: a counter for each block, then the partial results
     float* partials;
 };
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     __shared__ uint32_t stop_flag, complete[2];
     __shared__ Cut cuts[2];              // the parts of segments that are cut over blocks: the one this share begins in, ends in
     __shared__ uint32_t tile_most[NT];   // largest magnitudes of the tile's queries
-    // The first warps compute, the last one or two copy: keys and values, or one side each.
+    // The first warps compute, the last ones copy.
     const uint32_t warps = blockDim.x / 32 - args.copying, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
     uint8_t* const ring = shared + Shape::kQueryBytes;
@@ -684,7 +684,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         // ---- copies: tokens that follow each other in a page are one run, copied in bulk, codes and parameters. (Parameters
         // of runs that do not begin and end on 16 bytes go token by token.) Lane r works out run r of a unit; the pages of the
         // next unit's runs are asked for before the present one's are copied, by one thread after another's numbers.
-        const uint32_t side = warp - warps;
+        const uint32_t side = (warp - warps) & 1u;
+        const bool first_copying = warp == warps;
+        const uint32_t own_runs = args.copying < 4 ? 0xffffffffu : warp - warps < 2 ? 0x55555555u : 0xaaaaaaaau;
         struct Run {
             uint32_t entry, inside, at, length;  // page of the sequence, place in it, place in the unit, tokens
         };
@@ -731,10 +733,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     const bool sound = there && page < args.pages;
                     if (there && !sound) {
                         bad = true;
-                        if (side == 0) note(status, kBadPage, b, page);
+                        if (first_copying) note(status, kBadPage, b, page);
                     }
                     const uint32_t row = (page * args.kv_heads + kv_head) * args.page_size + run.inside;
-                    for (uint32_t left = __ballot_sync(0xffffffffu, sound); left; left &= left - 1) {
+                    for (uint32_t left = __ballot_sync(0xffffffffu, sound) & own_runs; left; left &= left - 1) {
                         const uint32_t lane_of = __ffs(left) - 1;
                         const uint64_t its_row = __shfl_sync(0xffffffffu, row, lane_of);
                         const uint32_t at = __shfl_sync(0xffffffffu, run.at, lane_of);
@@ -742,12 +744,12 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         const uint32_t param_bytes = length * (kGroups * 4);
                         const bool aligned = ((static_cast<uint32_t>(its_row * (kGroups * 4)) | at * (kGroups * 4) | param_bytes) & 15u) == 0;
                         const uint32_t moved = length * (D / 2) + (aligned ? param_bytes : 0);
-                        bytes += args.copying == 2 ? moved : 2 * moved;
+                        bytes += args.copying > 1 ? moved : 2 * moved;
                         single |= !aligned;
                         if (elect_one()) {
 #pragma unroll
                             for (uint32_t which = 0; which < 2; ++which) {
-                                if (args.copying == 2 && which != side) continue;
+                                if (args.copying > 1 && which != side) continue;
                                 bulk_load(memory + which * value_codes + at * (D / 2), args.codes[which] + its_row * (D / 2),
                                           length * (D / 2), full);
                                 const uint8_t* const params = args.params[which] + its_row * (kGroups * 4);
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 }
                 bad = __any_sync(0xffffffffu, bad);
                 if (elect_one()) {
-                    if (side == 0) bad_pages[stage] = bad;
+                    if (first_copying) bad_pages[stage] = bad;
                     if (single) copy_async_arrive(full);
                     mbar_arrive_expect_tx(full, bytes);
                 }
@@ -1523,7 +1525,10 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     const uint64_t sms = static_cast<uint64_t>(facts.sm_count);
     const bool lengthy = static_cast<uint64_t>(args.table_pages) * args.page_size > 8192;
     const uint32_t share = segments <= sms || (lengthy && segments < 2 * sms) ? 1 : segments <= 2 * sms ? 2 : 3;
-    args.copying = share == 1 ? 2 : 1;
+    // A bulk copy takes its warp some 150 cycles, whatever its size, so four warps copy for a block that is alone on its SM (131072
+    // tokens of one sequence in pages of 16, 32, 64: 75, 53 and 48 us; with two 102, 66 and 49). Small blocks spare one (384
+    // segments of 2000 tokens in pages of 16 and 32: 54 and 43 us; with two 56 and 49).
+    args.copying = share == 1 ? 4 : 1;
     const uint32_t by_threads = Shape::kMostThreads / 32 / share - args.copying, by_memory = Shape::kMostByMemory / share;
     const uint32_t warps = by_threads < by_memory ? by_threads : by_memory;
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * share;
