@@ -87,44 +87,50 @@ def workspace(device="cuda") -> torch.Tensor:
 
 
 def _on(device: torch.device, call) -> None:
-    """``call(stream handle)`` with ``device`` current, on torch's current stream of it."""
-    if torch.cuda.current_device() == device.index:
-        check(call(torch.cuda.current_stream(device).cuda_stream))
+    """``call(stream handle)`` with ``device`` current, on torch's current stream of it. (The raw handle: a step of a small
+    batch takes the device some ten microseconds, and a stream object alone takes the host three.)"""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch._C._cuda_getDevice() == device.index:
+        check(call(stream))
     else:
         with torch.cuda.device(device):
-            check(call(torch.cuda.current_stream(device).cuda_stream))
+            check(call(stream))
 
 
 def _require(name: str, tensor: torch.Tensor, cache: Cache, dims: int) -> None:
     if tensor.device != cache.device:
         raise RuntimeError(f"{name} must live on the cache's device {cache.device}: there is no CPU path")
-    if tensor.dtype != cache.dtype or tensor.dim() != dims or tensor.shape[-1] != cache.head_dim or tensor.stride(-1) != 1:
+    if (tensor.dtype is not cache.dtype or tensor.dim() != dims or tensor.shape[-1] != cache.head_dim
+            or tensor.stride(-1) != 1):
         raise ValueError(f"{name} must be a {dims}-dimensional {cache.dtype} tensor of contiguous rows of {cache.head_dim}")
 
 
-def _require_indices(name: str, tensor: torch.Tensor, cache: Cache, shape, dtypes=(torch.int32,)) -> None:
+def _require_indices(name: str, tensor: torch.Tensor, cache: Cache, count: int | None = None, wide: bool = False) -> None:
     if tensor.device != cache.device:
         raise RuntimeError(f"{name} must live on the cache's device {cache.device}: there is no CPU path")
-    if tensor.dtype not in dtypes or tuple(tensor.shape) != tuple(shape) or not tensor.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous tensor of shape {list(shape)} and type "
-                         + " or ".join(str(d).removeprefix("torch.") for d in dtypes))
+    if (not (tensor.dtype is torch.int32 or wide and tensor.dtype is torch.int64) or tensor.dim() != 1
+            or count is not None and tensor.shape[0] != count or not tensor.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {'int32 or int64' if wide else 'int32'} vector"
+                         + (f" of {count} entries" if count is not None else ""))
 
 
 def _rows(entry, cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, status, *more) -> None:
+    tokens = slots.shape[0]
     for name, tensor in (("k", k), ("v", v)):
         _require(name, tensor, cache, 3)
-        if tensor.shape[1] != cache.kv_heads or tensor.shape[0] != slots.shape[0]:
-            raise ValueError(f"{name} must hold {slots.shape[0]} tokens of {cache.kv_heads} heads, one token a slot")
+        if tensor.shape[1] != cache.kv_heads or tensor.shape[0] != tokens:
+            raise ValueError(f"{name} must hold {tokens} tokens of {cache.kv_heads} heads, one token a slot")
+    k_strides, v_strides = k.stride(), v.stride()
     _on(cache.device, lambda stream: entry(
-        cache.view, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
-        slots.element_size(), slots.shape[0], *more, stream, status.data_ptr() if status is not None else None))
+        cache.view, k.data_ptr(), v.data_ptr(), k_strides[0], k_strides[1], v_strides[0], v_strides[1], slots.data_ptr(),
+        4 if slots.dtype is torch.int32 else 8, tokens, *more, stream, status.data_ptr() if status is not None else None))
 
 
 def write(cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, status: torch.Tensor | None = None) -> None:
     """Quantise the tokens ``k[i], v[i]`` (``[tokens, kv_heads, head_dim]``, any strides that are multiples of 8 elements) into
     the slots ``slots[i]`` = page * page_size + place (int32 or int64); a negative slot skips its token. Slots that are not
     negative must be distinct: of one named twice the row is unspecified."""
-    _require_indices("slots", slots, cache, (slots.numel(),), (torch.int32, torch.int64))
+    _require_indices("slots", slots, cache, wide=True)
     _rows(library().fk_cache_write, cache, k, v, slots, status)
 
 
@@ -133,7 +139,7 @@ def read(cache: Cache, slots: torch.Tensor, k: torch.Tensor | None = None, v: to
     """``(k, v)``, ``[tokens, kv_heads, head_dim]``: what the rows at ``slots`` (int32 or int64, may repeat) stand for, rounded once.
     Rows of negative slots are zero in new tensors and left as they were in ``k`` and ``v`` that are given (which may be
     strided, as views of the planes ``flash_forward.run`` takes)."""
-    _require_indices("slots", slots, cache, (slots.numel(),), (torch.int32, torch.int64))
+    _require_indices("slots", slots, cache, wide=True)
     if (k is None) != (v is None):
         raise ValueError("k and v are given together or not at all")
     fresh = k is None
@@ -165,11 +171,11 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
     batch, queries, heads, head_dim = q.shape
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"{heads} query heads do not divide over {cache.kv_heads} kv heads")
-    _require_indices("lengths", lengths, cache, (batch,))
+    _require_indices("lengths", lengths, cache, batch)
     if table is not None:
         if table.device != cache.device:
             raise RuntimeError(f"table must live on the cache's device {cache.device}: there is no CPU path")
-        if (table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0
+        if (table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0
                 or (table.shape[1] > 1 and table.stride(1) != 1)):
             raise ValueError("table must be an int32 [batch, pages] tensor of contiguous rows of one page or more")
     if window is not None and not 1 <= window < 1 << 31:
@@ -190,8 +196,9 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
         if out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape")
     lse = torch.empty(shape[:3], dtype=torch.float32, device=cache.device)
+    strides = q.stride()
     _on(cache.device, lambda stream: library().fk_cache_attention(
-        cache.view, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), out.data_ptr(), lse.data_ptr(),
+        cache.view, q.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(), lse.data_ptr(),
         lengths.data_ptr(), table.data_ptr() if table is not None else None, table.stride(0) if table is not None else 0,
         table.shape[1] if table is not None else 0, batch, queries, heads,
         head_dim ** -0.5 if scale is None else scale, window or 0, sinks, workspace.data_ptr(),
