@@ -442,8 +442,8 @@ struct AttentionShape {
     static constexpr bool kMergeInRing = kMergeBytes <= kStageBytes;
     static constexpr uint32_t kScratchBytes = kMergeInRing ? 0 : kMergeBytes;
     static constexpr uint32_t kWarpBytes = kStages * kStageBytes + kScratchBytes;
-    // Registers a thread: 128, or 168 for more than one row tile or two groups.
-    static constexpr uint32_t kMostThreads = 32 * (NT == 1 && kGroups <= 2 ? 16 : 12);
+    // Registers a thread: 128, or 168 where a lane holds more outputs or groups.
+    static constexpr uint32_t kMostThreads = 32 * (D * NT <= 128 && kGroups <= 2 ? 16 : 12);
     static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
     static constexpr uint32_t most_warps(uint32_t copying) {
         return kMostThreads / 32 - copying < kMostByMemory ? kMostThreads / 32 - copying : kMostByMemory;
@@ -459,9 +459,9 @@ struct Extent {
     __device__ __forceinline__ int32_t token(int32_t at) const { return at < kept ? at : at + skipped; }
 };
 
-__device__ __forceinline__ Extent extent_of(const AttentionArguments& args, uint32_t b, uint32_t* status) {
+__device__ __forceinline__ Extent extent_of(const AttentionArguments& args, uint32_t b, int32_t length, uint32_t* status) {
     Extent e;
-    e.length = max(args.lengths[b], 0);
+    e.length = max(length, 0);
     const int32_t capacity = static_cast<int32_t>(args.table_pages * args.page_size);
     if (e.length > capacity) {
         note(status, kBadLength, b, static_cast<uint32_t>(e.length));
@@ -582,6 +582,16 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     uint8_t* const ring = shared + Shape::kQueryBytes;
     const uint32_t stage_bytes = warps * Shape::kStageBytes, value_codes = warps * Shape::kCodeBytes;
 
+    int32_t length_here = lane < args.batch ? args.lengths[lane] : 0;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < kStages; ++i) {
+            mbar_init(smem_u32(barriers + 2 * i), args.copying);
+            mbar_init(smem_u32(barriers + 2 * i + 1), warps);
+        }
+        stop_flag = cuts[0].parts = cuts[1].parts = 0;
+    }
+    fence_mbarrier_init();
+
     // ---- this block's share: units of unit_tokens tokens, sequence by sequence, (kv head, row tile) by (kv head,
     // row tile), cut evenly over the blocks whatever the lengths are. A segment, one sequence's units of one (kv
     // head, row tile), begins with args.segment_cost units of no work: what beginning and ending it takes. Every warp
@@ -590,8 +600,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     const auto cost_of = [&](const Extent& e) {
         return max(args.unit.quotient(static_cast<uint32_t>(e.visible()) + unit_tokens - 1), 1u) + args.segment_cost;
     };
-    uint32_t mine = lane < args.batch ? cost_of(extent_of(args, lane, status)) : 0, total = mine;
-    for (uint32_t i = lane + 32; i < args.batch; i += 32) total += cost_of(extent_of(args, i, status));
+    uint32_t mine = lane < args.batch ? cost_of(extent_of(args, lane, length_here, status)) : 0, total = mine;
+    for (uint32_t i = lane + 32; i < args.batch; i += 32) total += cost_of(extent_of(args, i, args.lengths[i], status));
     total = __reduce_add_sync(0xffffffffu, total) * segments;
     const uint32_t blocks = min(gridDim.x, max(total >> args.least_units, 1u));
     if (blockIdx.x >= blocks) return;
@@ -605,7 +615,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     const uint32_t end = at + share + (blockIdx.x < longer ? 1 : 0);
     uint32_t b = 0, before = 0;
     for (uint32_t chunk = 0;; chunk += 32) {
-        if (chunk) mine = chunk + lane < args.batch ? cost_of(extent_of(args, chunk + lane, nullptr)) : 0;
+        if (chunk) {
+            length_here = chunk + lane < args.batch ? args.lengths[chunk + lane] : 0;
+            mine = chunk + lane < args.batch ? cost_of(extent_of(args, chunk + lane, length_here, nullptr)) : 0;
+        }
         uint32_t sum = mine * segments;
 #pragma unroll
         for (uint32_t d = 1; d < 32; d *= 2) {
@@ -618,24 +631,17 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             const uint32_t found = __ffs(past) - 1;
             b = chunk + found;
             before += __shfl_sync(0xffffffffu, sum - mine * segments, found);
+            length_here = __shfl_sync(0xffffffffu, length_here, found);
             break;
         }
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
 
-    if (threadIdx.x == 0) {
-        for (uint32_t i = 0; i < kStages; ++i) {
-            mbar_init(smem_u32(barriers + 2 * i), args.copying);
-            mbar_init(smem_u32(barriers + 2 * i + 1), warps);
-        }
-        stop_flag = cuts[0].parts = cuts[1].parts = 0;
-    }
-    fence_mbarrier_init();
     __syncthreads();
     const StallSite site{status, &stop_flag, 0};
     bool live = true;  // until a wait gives up: nothing is waited for after that
 
-    Extent extent = extent_of(args, b, nullptr);
+    Extent extent = extent_of(args, b, length_here, nullptr);
     uint32_t cost = cost_of(extent);
     uint32_t segment = (at - before) / cost;
     uint32_t offset = (at - before) - segment * cost;  // of `at` in its segment
@@ -664,7 +670,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         if (++segment == segments) {
             segment = 0;
             ++b;
-            extent = extent_of(args, b, nullptr);
+            extent = extent_of(args, b, args.lengths[b], nullptr);
             cost = cost_of(extent);
         }
         return find_piece();
@@ -1536,7 +1542,7 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     args.least_units = 1;
     args.unit = cache::Divider(static_cast<uint32_t>(unit_tokens));
     args.tiles = cache::Divider(args.row_tiles);
-    args.segment_cost = 1;
+    args.segment_cost = share == 1 ? 2 : 1;
     const uint64_t most_units = segments * ((static_cast<uint64_t>(args.table_pages) * args.page_size + unit_tokens - 1) / unit_tokens + args.segment_cost);
     if (most_units >= (1ull << 31))
         return fk_fail(FK_ERR_SHAPE, "%u sequences of up to %llu tokens on %u heads are more than a launch counts", args.batch,
