@@ -969,10 +969,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
             // subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
             float2 x[2][NT][2];  // [step of 16 tokens][row tile][token of the fragment's upper or lower half] (two rows)
-            const auto products = [&](uint32_t h, uint32_t g, const uint32_t (&a)[2][kKeyWords], float (&part)[NT][4]) {
+            // One step's products, or for several row tiles both steps' for each load of a query fragment.
+            const auto products = [&](uint32_t g, const auto& a, auto& part, auto steps) {
 #pragma unroll
-                for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w) {
-                    const uint32_t y0 = a[0][w] >> 8, y1 = a[1][w] >> 8;
+                for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w)
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n) {
                         uint32_t f[4];
@@ -980,11 +980,15 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             ld_shared_v4(smem_u32(shared_q + (n * kKeyWords + w) * 32 + lane), f);
                         else
                             f[0] = qf[2 * w][0], f[1] = qf[2 * w][1], f[2] = qf[2 * w + 1][0], f[3] = qf[2 * w + 1][1];
-                        mma_16x8x16(part[n], a[0][w] & 0x000f000fu, a[1][w] & 0x000f000fu, a[0][w] & 0x00f000f0u,
-                                    a[1][w] & 0x00f000f0u, f[0], f[1]);
-                        mma_16x8x16(part[n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, f[2], f[3]);
+#pragma unroll
+                        for (uint32_t h = 0; h < decltype(steps)::value; ++h) {
+                            const uint32_t y0 = a[h][0][w] >> 8, y1 = a[h][1][w] >> 8;
+                            mma_16x8x16(part[h][n], a[h][0][w] & 0x000f000fu, a[h][1][w] & 0x000f000fu, a[h][0][w] & 0x00f000f0u,
+                                        a[h][1][w] & 0x00f000f0u, f[0], f[1]);
+                            mma_16x8x16(part[h][n], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, f[2],
+                                        f[3]);
+                        }
                     }
-                }
             };
             const auto load_keys = [&](uint32_t h, uint32_t (&a)[2][kKeyWords]) {
 #pragma unroll
@@ -1008,18 +1012,23 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     }
                 }
             };
+            constexpr uint32_t kTogether = NT > 1 ? 2 : 1;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                uint32_t a[2][kKeyWords], pairs[2][kGroups];
-                load_keys(h, a);
+            for (uint32_t h0 = 0; h0 < 2; h0 += kTogether) {
+                uint32_t a[kTogether][2][kKeyWords], pairs[kTogether][2][kGroups];
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half)
-                    load_words(pairs[half], key_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
+                for (uint32_t h = 0; h < kTogether; ++h) {
+                    load_keys(h0 + h, a[h]);
+#pragma unroll
+                    for (uint32_t half = 0; half < 2; ++half)
+                        load_words(pairs[h][half], key_params + (16 * (h0 + h) + 8 * half + own_token) * (kGroups * 4));
+                }
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g) {
-                    float part[NT][4] = {};
-                    products(h, g, a, part);
-                    add_up(h, g, pairs, part);
+                    float part[kTogether][NT][4] = {};
+                    products(g, a, part, std::integral_constant<uint32_t, kTogether>{});
+#pragma unroll
+                    for (uint32_t h = 0; h < kTogether; ++h) add_up(h0 + h, g, pairs[h], part[h]);
                 }
             }
 
@@ -1330,40 +1339,44 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             }
             continue;
         }
-        // Warp w puts parts w, w + warps, ... together; a lane's loads of a part are all on their way at once.
-        constexpr uint32_t kItems = kRows * D / 128;
-        float4 y[kItems] = {};
-        float2 all[kItems];
+        // Warp w puts parts w, w + warps, ... together; a lane's loads of a part, eight rows' at most, are all on their way at once.
+        float* const merged = reinterpret_cast<float*>(memory + warp * kMergePitch);
+        constexpr uint32_t kItems = 8 * D / 128;
+#pragma unroll 1
+        for (uint32_t first = 0; first < rows_here; first += 8) {
+            float4 y[kItems] = {};
+            float2 all[kItems];
 #pragma unroll
-        for (uint32_t k = 0; k < kItems; ++k) all[k] = make_float2(-INFINITY, 0.0f);
-        for (uint32_t p = warp; p < piece.parts; p += warps) {
-            const float* const its = args.partials + (2 * (piece.owner + p) + (p == 0)) * static_cast<size_t>(kPartialFloats);
-            float4 z[kItems];
-            float2 stat[kItems];
+            for (uint32_t k = 0; k < kItems; ++k) all[k] = make_float2(-INFINITY, 0.0f);
+#pragma unroll 1
+            for (uint32_t p = warp; p < piece.parts; p += warps) {
+                const float* const its = args.partials + (2 * (piece.owner + p) + (p == 0)) * static_cast<size_t>(kPartialFloats);
+                float4 z[kItems];
+                float2 stat[kItems];
 #pragma unroll
-            for (uint32_t k = 0; k < kItems; ++k) {
-                const uint32_t row = (lane + 32 * k) / (D / 4), d = (lane + 32 * k) % (D / 4) * 4;
-                stat[k] = make_float2(-INFINITY, 0.0f);
-                if (row < rows_here) {
-                    stat[k] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
-                    z[k] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
+                for (uint32_t k = 0; k < kItems; ++k) {
+                    const uint32_t row = first + (lane + 32 * k) / (D / 4), d = (lane + 32 * k) % (D / 4) * 4;
+                    stat[k] = make_float2(-INFINITY, 0.0f);
+                    if (row < rows_here) {
+                        stat[k] = __ldcg(reinterpret_cast<const float2*>(its + kMostRows * 128 + 2 * row));
+                        z[k] = __ldcg(reinterpret_cast<const float4*>(its + row * D + d));
+                    }
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < kItems; ++k) {
+                    if (stat[k].x == -INFINITY) continue;
+                    const float m = fmaxf(all[k].x, stat[k].x), keep = ex2_approx(all[k].x - m), factor = ex2_approx(stat[k].x - m);
+                    y[k] = make_float4(fmaf(z[k].x, factor, y[k].x * keep), fmaf(z[k].y, factor, y[k].y * keep),
+                                       fmaf(z[k].z, factor, y[k].z * keep), fmaf(z[k].w, factor, y[k].w * keep));
+                    all[k] = make_float2(m, fmaf(stat[k].y, factor, all[k].y * keep));
                 }
             }
 #pragma unroll
             for (uint32_t k = 0; k < kItems; ++k) {
-                if (stat[k].x == -INFINITY) continue;
-                const float m = fmaxf(all[k].x, stat[k].x), keep = ex2_approx(all[k].x - m), factor = ex2_approx(stat[k].x - m);
-                y[k] = make_float4(fmaf(z[k].x, factor, y[k].x * keep), fmaf(z[k].y, factor, y[k].y * keep),
-                                   fmaf(z[k].z, factor, y[k].z * keep), fmaf(z[k].w, factor, y[k].w * keep));
-                all[k] = make_float2(m, fmaf(stat[k].y, factor, all[k].y * keep));
+                const uint32_t row = first + (lane + 32 * k) / (D / 4), d = (lane + 32 * k) % (D / 4) * 4;
+                *reinterpret_cast<float4*>(merged + row * kPitch + d) = y[k];
+                if (d == 0) *reinterpret_cast<float2*>(merged + kRows * kPitch + 2 * row) = all[k];
             }
-        }
-        float* const merged = reinterpret_cast<float*>(memory + warp * kMergePitch);
-#pragma unroll
-        for (uint32_t k = 0; k < kItems; ++k) {
-            const uint32_t row = (lane + 32 * k) / (D / 4), d = (lane + 32 * k) % (D / 4) * 4;
-            *reinterpret_cast<float4*>(merged + row * kPitch + d) = y[k];
-            if (d == 0) *reinterpret_cast<float2*>(merged + kRows * kPitch + 2 * row) = all[k];
         }
         sync_computing(warps * 32);
         put_together(memory, kMergePitch, piece, nullptr);
