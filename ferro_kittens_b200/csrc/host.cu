@@ -451,6 +451,8 @@ static const char* stall_role(uint32_t code) {
         case 0x407: return "flash backward MMA warp waiting for dS";
         case 0x408: return "flash backward element-wise warp waiting for dP";
         case 0x4ff: return "flash backward found its shared memory base off a 1024-byte boundary";
+        case 0x504: return "cache attention computing warp waiting for a stage of tokens";
+        case 0x505: return "cache attention copying warp waiting for a stage to be free";
         case 0x312: return "row-kernel copy warp waiting for the compute warps to finish a tile";
         case 0x313: return "row-kernel compute warp waiting for a tile to land";
         case 0x314: return "row-kernel compute warp waiting for the other warps' partial sums";

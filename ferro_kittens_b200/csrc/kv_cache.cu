@@ -2,6 +2,9 @@
 // attention of a sequence's newest tokens over its rows. No counterpart in the reference, whose attention
 // reads whole bf16 planes (examples/src/flash_forward.rs:151-158); the format is stated in the header.
 
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -444,9 +447,10 @@ struct AttentionShape {
     static constexpr uint32_t kWarpBytes = kStages * kStageBytes + kScratchBytes;
     // Registers a thread: 128, or 168 where a lane holds more outputs or groups.
     static constexpr uint32_t kMostThreads = 32 * (D * NT <= 128 && kGroups <= 2 ? 16 : 12);
-    static constexpr uint32_t kMostByMemory = (227 * 1024 - 2048 - kQueryBytes) / kWarpBytes;
-    static constexpr uint32_t most_warps(uint32_t copying) {
-        return kMostThreads / 32 - copying < kMostByMemory ? kMostThreads / 32 - copying : kMostByMemory;
+    /// Computing warps of each of `share` blocks on an SM: 228 KiB, of which every block takes 1 KiB, and its static part.
+    static constexpr uint32_t most_warps(uint32_t share, uint32_t copying) {
+        const uint32_t by_memory = (228 * 1024 / share - 2048 - kQueryBytes) / kWarpBytes, by_threads = kMostThreads / 32 / share - copying;
+        return by_threads < by_memory ? by_threads : by_memory;
     }
     static constexpr uint32_t shared_bytes(uint32_t warps) { return kQueryBytes + warps * kWarpBytes; }
 };
@@ -1458,6 +1462,11 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
         if (stride % 8)
             return fk_fail(FK_ERR_ALIGNMENT, "a stride of %lld elements is no multiple of 8: rows move 16 bytes at a time",
                            static_cast<long long>(stride));
+    if (!write)
+        for (uint32_t i = 0; i < 4; ++i)
+            if ((i % 2 ? cache->kv_heads : tokens) > 1 && std::abs(strides[i]) < cache->head_dim)
+                return fk_fail(FK_ERR_SHAPE, "a stride of %lld elements lays rows of %u over one another",
+                               static_cast<long long>(strides[i]), cache->head_dim);
     if (static_cast<uint64_t>(tokens) * cache->kv_heads >= (1ull << 31))
         return fk_fail(FK_ERR_SHAPE, "%u tokens x %u heads is more than 2^31 - 1 rows", tokens, cache->kv_heads);
     DeviceFacts facts;
@@ -1531,8 +1540,9 @@ template <int D, int G, int NT, bool BF16>
 static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& facts, void* stream, uint32_t* device_status) {
     using Shape = cache::AttentionShape<D, G, NT>;
     const auto kernel = cache::attention_kernel<D, G, NT, BF16>;
+    constexpr uint32_t kCopyingAlone = 4;
     uint32_t limit = 0;
-    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(Shape::most_warps(1)), &limit);
+    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(Shape::most_warps(1, kCopyingAlone)), &limit);
     if (admitted != FK_OK) return admitted;
     args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
@@ -1547,9 +1557,8 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     // A bulk copy takes its warp some 150 cycles, whatever its size, so four warps copy for a block that is alone on its SM (131072
     // tokens of one sequence in pages of 16, 32, 64: 75, 53 and 48 us; with two 102, 66 and 49). Small blocks spare one (384
     // segments of 2000 tokens in pages of 16 and 32: 54 and 43 us; with two 56 and 49).
-    args.copying = share == 1 ? 4 : 1;
-    const uint32_t by_threads = Shape::kMostThreads / 32 / share - args.copying, by_memory = Shape::kMostByMemory / share;
-    const uint32_t warps = by_threads < by_memory ? by_threads : by_memory;
+    args.copying = share == 1 ? kCopyingAlone : 1;
+    const uint32_t warps = Shape::most_warps(share, args.copying);
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * share;
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
     args.least_units = 1;
@@ -1578,6 +1587,8 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
         return fk_fail(FK_ERR_SHAPE, "%u query heads do not divide over %u kv heads", heads, cache->kv_heads);
     if (batch == 0 || queries == 0) return FK_OK;
     if (!q || !out || !lengths || !workspace) return fk_fail(FK_ERR_INVALID, "an operand pointer is null");
+    if (q == out) return fk_fail(FK_ERR_INVALID, "the output may not lie over the queries");
+    if (!std::isfinite(scale)) return fk_fail(FK_ERR_INVALID, "the score scale %f is not finite", scale);
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15u)
         return fk_fail(FK_ERR_ALIGNMENT, "queries, output and workspace must be 16-byte aligned");
     if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(table)) & 3u)

@@ -265,6 +265,38 @@ def test_attention_lengths_and_pages(device, page_size, length):
     _check_attention(device, cache, q, lengths, _tables(device, 1, per, per + 2, length))
 
 
+@pytest.mark.parametrize("head_dim,group", [(128, 128), (128, 32), (64, 64)])
+@pytest.mark.parametrize("page_size,window,sinks", [(1, None, 0), (5, 90, 3), (10, None, 0), (24, 200, 33), (100, 37, 1)])
+def test_attention_rows_that_do_not_begin_on_16_bytes(device, head_dim, group, page_size, window, sinks):
+    """Parameters of 4 and 8 bytes a row whose runs begin and end anywhere."""
+    lengths = torch.tensor([333, 12, 480], dtype=torch.int32, device=device)
+    per = -(-480 // page_size)
+    cache = _random_cache(device, 3 * per, page_size, 3, head_dim, group, torch.bfloat16, 17)
+    q = torch.randn(3, 2, 9, head_dim, device=device).bfloat16()
+    _check_attention(device, cache, q, lengths, _tables(device, 3, per, 3 * per), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_attention_drawn(device, seed):
+    """Everything at once, drawn: formats, heads, ragged lengths with empty ones, pages, windows, strides of the table."""
+    rng = np.random.default_rng(seed)
+    head_dim, group, dtype = FORMATS[seed % len(FORMATS)]
+    kv_heads, ratio, queries = int(rng.integers(1, 4)), int(rng.choice([1, 2, 3, 6, 8, 12])), int(rng.choice([1, 1, 2, 5]))
+    batch, page_size = int(rng.choice([1, 3, 9])), int(rng.choice([1, 7, 16, 32, 48, 64, 200]))
+    lengths = [int(n) for n in np.exp(rng.uniform(0, np.log(900), batch))]
+    if batch > 1:
+        lengths[int(rng.integers(batch))] = 0
+    per = -(-max(lengths) // page_size) + int(rng.integers(0, 3))
+    per = max(per, 1)
+    cache = _random_cache(device, batch * per + 1, page_size, kv_heads, head_dim, group, dtype, seed)
+    wide = torch.full((batch, per + 3), 1 << 30, dtype=torch.int32, device=device)
+    wide[:, :per] = _tables(device, batch, per, batch * per + 1, seed)
+    window, sinks = (int(rng.integers(1, 400)), int(rng.choice([0, 1, 4, 60]))) if rng.random() < 0.4 else (None, 0)
+    q = torch.randn(batch, queries, kv_heads * ratio, head_dim, device=device).to(dtype) * float(rng.choice([0.3, 1.5, 4.0]))
+    _check_attention(device, cache, q, torch.tensor(lengths, dtype=torch.int32, device=device), wide[:, :per], window=window,
+                     sinks=sinks)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 3), (64, 4), (100, 0), (128, 130), (5000, 4), (37, 1000)])
 @pytest.mark.parametrize("queries", [1, 4])
 def test_attention_window_and_sinks(device, window, sinks, queries):
@@ -402,6 +434,38 @@ def test_long_and_many_sequences(device, batch, kv_heads, ratio, length, ragged)
     for _ in range(3):  # the same bits every time, through a workspace that is used again
         again, lse_again = kv_cache.attend(q, cache, lengths, table, workspace=workspace)
         assert torch.equal(again, out) and torch.equal(lse_again, lse)
+
+
+def test_more_sequences_than_blocks_count(device):
+    """Thousands of sequences, most of them empty or of a token or two."""
+    batch = 5000
+    cache = _random_cache(device, 40, 16, 1, 64, 32, torch.bfloat16, 6)
+    lengths = torch.zeros(batch, dtype=torch.int32)
+    lengths[::7], lengths[3::1000], lengths[-1] = 1, 300, 2
+    table = (torch.arange(batch)[:, None] * 3 + torch.arange(20)).remainder(40).int()
+    q = torch.randn(batch, 1, 3, 64, device=device).bfloat16()
+    out, lse = kv_cache.attend(q, cache, lengths.to(device), table.to(device))
+    some = [0, 1, 3, 7, 1003, 2499, 3003, 4900, 4998, 4999]
+    _compare(cache, q[some], lengths[some], table[some], None, None, 0, out[some], lse[some])
+    empty = lengths == 0
+    assert (out[empty.to(device)] == 0).all() and torch.isneginf(lse[empty.to(device)]).all()
+
+
+def test_rows_that_hold_nan_or_infinite_queries_spoil_no_others(device):
+    cache = _random_cache(device, 10, 16, 2, 128, 64, torch.bfloat16, 3)
+    table, lengths = _tables(device, 2, 5, 10), torch.tensor([77, 30], dtype=torch.int32, device=device)
+    for heads in (8, 24):
+        q = torch.randn(2, 1, heads, 128, device=device).bfloat16()
+        want = kv_cache.attend(q, cache, lengths, table)
+        bad = q.clone()
+        bad[0, 0, 1, 5], bad[1, 0, heads - 1, 0] = float("nan"), float("inf")
+        out, lse = kv_cache.attend(bad, cache, lengths, table)
+        assert torch.isnan(out[0, 0, 1]).all() and torch.isnan(out[1, 0, heads - 1]).all()
+        rest = torch.ones(2, 1, heads, dtype=torch.bool, device=device)
+        rest[0, 0, 1] = rest[1, 0, heads - 1] = False
+        # The others' queries may be scaled by another power of two: the same numbers but for fp32 sums' last bits.
+        assert torch.allclose(out[rest].float(), want[0][rest].float(), rtol=2.0 ** -7, atol=2.0 ** -12)
+        assert torch.allclose(lse[rest], want[1][rest], rtol=0, atol=2.0 ** -14)
 
 
 def test_rows_past_four_gibibytes(device):
@@ -556,9 +620,11 @@ def test_refusals_with_tensors(device):
     with pytest.raises(ValueError):
         kv_cache.attend(q, cache, lengths, table[:, :0])
     for more in ({"window": 0}, {"window": -1}, {"sinks": -1}, {"workspace": torch.zeros(16, device="cpu")},
-                 {"out": q.half()}, {"out": q[:, :, :2]}):
-        with pytest.raises((ValueError, RuntimeError)):
+                 {"out": q.half()}, {"out": q[:, :, :2]}, {"out": q}, {"scale": float("nan")}):
+        with pytest.raises((ValueError, RuntimeError)):  # FerroKittensError is a RuntimeError
             kv_cache.attend(q, cache, lengths, table, **more)
+    with pytest.raises(FerroKittensError, match="over one another"):
+        kv_cache.read(cache, slots, x[:1].expand(4, 2, 128), x)
     with pytest.raises(FerroKittensError, match="workspace of 16 bytes"):
         kv_cache.attend(q, cache, lengths, table, workspace=torch.zeros(16, dtype=torch.uint8, device=device))
     for sizes in ({"head_dim": 96}, {"group": 16}, {"head_dim": 64, "group": 128}, {"dtype": torch.float32}):

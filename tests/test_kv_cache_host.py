@@ -28,10 +28,10 @@ def _read(cache, k=BASE, v=BASE, strides=(256, 128, 256, 128), slots=BASE, slot_
     return library().fk_cache_read(ctypes.byref(cache) if cache else None, k, v, *strides, slots, slot_bytes, tokens, 0, None, None)
 
 
-def _attend(cache, q=BASE, strides=(1024, 1024, 128), out=BASE, lse=BASE, lengths=BASE, table=BASE, table_pages=2, batch=3,
-            queries=1, heads=8, workspace=BASE, workspace_bytes=1 << 30):
+def _attend(cache, q=BASE, strides=(1024, 1024, 128), out=BASE + (1 << 20), lse=BASE, lengths=BASE, table=BASE, table_pages=2, batch=3,
+            queries=1, heads=8, scale=0.1, workspace=BASE, workspace_bytes=1 << 30):
     return library().fk_cache_attention(ctypes.byref(cache) if cache else None, q, *strides, out, lse, lengths, table, table_pages,
-                                        table_pages, batch, queries, heads, 0.1, 0, 0, workspace, workspace_bytes, None, None)
+                                        table_pages, batch, queries, heads, scale, 0, 0, workspace, workspace_bytes, None, None)
 
 
 @pytest.mark.parametrize("entry", [_write, _read, _attend])
@@ -67,12 +67,22 @@ def test_rows_refused(entry, changed, code, word):
 @pytest.mark.parametrize("changed,code,word", [
     ({"heads": 7}, FK_ERR_SHAPE, "7 query heads"), ({"heads": 0}, FK_ERR_SHAPE, "0 query heads"), ({"q": None}, FK_ERR_INVALID, "null"),
     ({"out": None}, FK_ERR_INVALID, "null"), ({"lengths": None}, FK_ERR_INVALID, "null"), ({"workspace": None}, FK_ERR_INVALID, "null"),
-    ({"q": BASE + 8}, FK_ERR_ALIGNMENT, "16-byte"), ({"lse": BASE + 2}, FK_ERR_ALIGNMENT, "4-byte"),
+    ({"out": BASE}, FK_ERR_INVALID, "over the queries"), ({"q": BASE + 8}, FK_ERR_ALIGNMENT, "16-byte"), ({"lse": BASE + 2}, FK_ERR_ALIGNMENT, "4-byte"),
     ({"strides": (1024, 1020, 128)}, FK_ERR_ALIGNMENT, "1020"), ({"table_pages": 0}, FK_ERR_SHAPE, "no columns"),
     ({"table": None, "batch": 5}, FK_ERR_SHAPE, "own a page each"), ({"table_pages": 1 << 30}, FK_ERR_SHAPE, "tokens a sequence")])
 def test_attention_refused(changed, code, word):
     assert _attend(_cache(), **changed) == code
     assert word in last_error()
+
+
+@pytest.mark.parametrize("strides", [(0, 128, 256, 128), (256, 128, 256, 0), (64, 128, 256, 128), (256, 128, 256, 120)])
+def test_rows_read_over_one_another_are_refused(strides):
+    assert _read(_cache(), strides=strides) == FK_ERR_SHAPE and "over one another" in last_error()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_scales_that_are_not_finite_are_refused(scale):
+    assert _attend(_cache(), scale=scale) == FK_ERR_INVALID and "not finite" in last_error()
 
 
 def test_empty_calls_need_no_device():
