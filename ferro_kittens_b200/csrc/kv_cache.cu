@@ -452,6 +452,14 @@ struct AttentionShape {
         const uint32_t by_memory = (228 * 1024 / share - 2048 - kQueryBytes) / kWarpBytes, by_threads = kMostThreads / 32 / share - copying;
         return by_threads < by_memory ? by_threads : by_memory;
     }
+    // A block alone on its SM has four copying warps, which need few registers: theirs go to the computing warps.
+    static constexpr uint32_t kCopyingAlone = 4;
+    static constexpr uint32_t kCopyingRegisters = 56;
+    static constexpr uint32_t kLaunchRegisters = 65536 / kMostThreads / 8 * 8;
+    static constexpr uint32_t kComputingRegisters =
+        (kLaunchRegisters * kMostThreads - kCopyingRegisters * 32 * kCopyingAlone) / (kMostThreads - 32 * kCopyingAlone) / 8 * 8;
+    static_assert(most_warps(1, kCopyingAlone) * 32 == kMostThreads - 32 * kCopyingAlone && kMostThreads % 128 == 0,
+                  "registers change hands between whole warpgroups");
     static constexpr uint32_t shared_bytes(uint32_t warps) { return kQueryBytes + warps * kWarpBytes; }
 };
 
@@ -566,7 +574,7 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
     if (d == 0 && args.lse) args.lse[place] = empty ? -INFINITY : (stat.x + log2f(stat.y)) * 0.6931471805599453f;
 }
 
-template <int D, int G, int NT, bool BF16>
+template <int D, int G, int NT, bool BF16, bool ALONE>
 __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     attention_kernel(const __grid_constant__ AttentionArguments args, uint32_t* status) {
     using E = Element<BF16>;
@@ -691,6 +699,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     };
 
     if (warp >= warps) {
+        if constexpr (ALONE) setmaxnreg_dec<Shape::kCopyingRegisters>();
         // ---- copies: tokens that follow each other in a page are one run, copied in bulk, codes and parameters. (Parameters
         // of runs that do not begin and end on 16 bytes go token by token.) Lane r works out run r of a unit; the pages of the
         // next unit's runs are asked for before the present one's are copied, by one thread after another's numbers.
@@ -796,6 +805,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         return;
     }
 
+    if constexpr (ALONE) setmaxnreg_inc<Shape::kComputingRegisters>();
     const uint32_t l4 = lane / 4, c4 = lane % 4;
     const auto load_row = [&](uint32_t n, uint4 (&raw)[kKeyWords]) {
         const uint32_t r = first_row + 8 * n + l4, t = args.ratio.quotient(min(r, args.rows - 1));
@@ -1539,11 +1549,6 @@ extern "C" uint64_t fk_cache_attention_workspace_bytes(uint32_t sm_count) {
 template <int D, int G, int NT, bool BF16>
 static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& facts, void* stream, uint32_t* device_status) {
     using Shape = cache::AttentionShape<D, G, NT>;
-    const auto kernel = cache::attention_kernel<D, G, NT, BF16>;
-    constexpr uint32_t kCopyingAlone = 4;
-    uint32_t limit = 0;
-    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(Shape::most_warps(1, kCopyingAlone)), &limit);
-    if (admitted != FK_OK) return admitted;
     args.row_tiles = (args.rows + Shape::kRows - 1) / Shape::kRows;
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
     // How many warps share a piece. One block an SM, of all the warps it holds, leaves the fewest parts to put together: for
@@ -1557,7 +1562,7 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     // A bulk copy takes its warp some 150 cycles, whatever its size, so four warps copy for a block that is alone on its SM (131072
     // tokens of one sequence in pages of 16, 32, 64: 75, 53 and 48 us; with two 102, 66 and 49). Small blocks spare one (384
     // segments of 2000 tokens in pages of 16 and 32: 54 and 43 us; with two 56 and 49).
-    args.copying = share == 1 ? kCopyingAlone : 1;
+    args.copying = share == 1 ? Shape::kCopyingAlone : 1;
     const uint32_t warps = Shape::most_warps(share, args.copying);
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * share;
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
@@ -1570,6 +1575,10 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
         return fk_fail(FK_ERR_SHAPE, "%u sequences of up to %llu tokens on %u heads are more than a launch counts", args.batch,
                        static_cast<unsigned long long>(args.table_pages) * args.page_size, args.kv_heads);
     const uint32_t grid = most_units < resident ? static_cast<uint32_t>(most_units) : resident;
+    const auto kernel = share == 1 ? cache::attention_kernel<D, G, NT, BF16, true> : cache::attention_kernel<D, G, NT, BF16, false>;
+    uint32_t limit = 0;
+    const int admitted = fk_admit_shared_plan(reinterpret_cast<const void*>(kernel), Shape::shared_bytes(warps), &limit);
+    if (admitted != FK_OK) return admitted;
     kernel<<<grid, (warps + args.copying) * 32, Shape::shared_bytes(warps), static_cast<cudaStream_t>(stream)>>>(args, device_status);
     FK_CUDA(cudaGetLastError());
     return FK_OK;
