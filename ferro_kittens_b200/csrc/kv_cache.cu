@@ -1,6 +1,8 @@
 // The key/value cache in 4 bits, for sm_100a: quantising tokens as they are written, reading rows back, and
 // attention of a sequence's newest tokens over its rows. No counterpart in the reference, whose attention
 // reads whole bf16 planes (examples/src/flash_forward.rs:151-158); the format is stated in the header.
+//
+// All three are bound by memory on paper. Shares below are of a plain copy's rate, 6.55 TB/s.
 
 #include <algorithm>
 #include <cmath>
@@ -300,7 +302,10 @@ __device__ __forceinline__ uint32_t group_codes(const uint4 x, uint32_t params, 
 }
 
 // One lane holds 8 channels (16 bytes) of a row's key and of its value, D / 8 lanes a row, ROWS rows of its own at a time: slots,
-// then rows, of all of them are on their way before the first is worked on.
+// then rows, of all of them are on their way before the first is worked on. The group's ends meet by shuffles of packed pairs;
+// everything behind them is on packed fp32 pairs, without a division, and exact (see above). What bounds it is the issue of
+// instructions (0.81 a cycle and scheduler, 175 a warp for 8 channels of its lanes): 150001 tokens of 8 heads of 64 fp16 values take 114 us, 54 %
+// of the copy rate; 8191 tokens of 8 heads of 128 bf16 values 17 us.
 template <int D, int G, int ROWS, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constant__ RowArguments args,
                                                             uint32_t* status) {
@@ -342,7 +347,9 @@ __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constan
 }
 
 // The same lanes the other way: a code in the low mantissa bits of a power of two, less that power, is exact,
-// and one fused multiply-add in the cache's type rounds low + code * scale once.
+// and one fused multiply-add in the cache's type rounds low + code * scale once. 65536 tokens of 8 heads of 128 bf16 values take
+// 64 us, 82 % of the copy rate (four fifths of the bytes are writes). Two rows a thread and blocks of 128 threads: 71 us with
+// 256 threads, 75 with one row, 74 and 87 with four and eight (registers that hold rows in flight cost threads).
 template <int D, int G, int ROWS, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant__ RowArguments args,
                                                            uint32_t* status) {
@@ -406,7 +413,6 @@ struct AttentionArguments {
     float scale;
     int32_t window, sinks;
     Divider page, ratio, unit, tiles;  // by page_size, heads / kv_heads, a unit's tokens, row_tiles
-    uint32_t least_units;   // units a block takes before another block is put to work, as a power of two
     uint32_t segment_cost;  // what beginning and ending a segment takes, in units
     uint32_t copying;       // warps that copy: 1, 2 (a side each) or 4 (every other run of a side each)
     uint32_t* arrivals;    // workspace: a counter for each block, then the partial results
@@ -466,6 +472,7 @@ struct AttentionShape {
 /// What of a sequence is read: its tokens, less those between the sinks and the window that no query row sees.
 struct Extent {
     int32_t length, first;  // tokens; the first query's position (0 if it lies before the first token)
+    int32_t start;          // the first token that some row's window reaches
     int32_t kept, skipped;  // tokens read before the gap, and the gap's length, both multiples of 16: parameters are copied by 16 bytes
     __device__ __forceinline__ int32_t visible() const { return length - skipped; }
     __device__ __forceinline__ int32_t token(int32_t at) const { return at < kept ? at : at + skipped; }
@@ -480,9 +487,9 @@ __device__ __forceinline__ Extent extent_of(const AttentionArguments& args, uint
         e.length = capacity;
     }
     e.first = max(e.length - static_cast<int32_t>(args.queries), 0);
-    const int32_t start = args.window ? max(e.first + 1 - args.window, 0) : 0;
-    e.kept = min((min(args.sinks, start) + 15) & ~15, start & ~15);
-    e.skipped = (start & ~15) - e.kept;
+    e.start = args.window ? max(e.first + 1 - args.window, 0) : 0;
+    e.kept = min((min(args.sinks, e.start) + 15) & ~15, e.start & ~15);
+    e.skipped = (e.start & ~15) - e.kept;
     return e;
 }
 
@@ -574,6 +581,34 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
     if (d == 0 && args.lse) args.lse[place] = empty ? -INFINITY : (stat.x + log2f(stat.y)) * 0.6931471805599453f;
 }
 
+// Attention. Of one sequence and kv head (a segment), for up to 8 NT of its query rows: with key codes c, scale s, low l of each
+// group g of channels, values alike (c', s', l'), and F = scale * log2(e),
+//   x_j = sum_g (s_jg * sum_{d in g} q_d c_jd + l_jg * sum_{d in g} q_d),  p_j = 2^(F (x_j - x_ref)),
+//   O_d = (sum_j (p_j s'_jg) (c'_jd - 8) + sum_j p_j (l'_jg + 8 s'_jg)) / sum_j p_j
+// so that the matrix instructions only ever see codes, which are exact fp16 subnormals as they lie in the cache, and no code is
+// ever multiplied out. Scores and outputs are computed transposed (tokens, then channels, are the rows of the m16n8k16
+// fragments, query rows the columns): eight rows fill the instruction, a lane holds two tokens' parameters, and a code that is
+// unpacked once serves all of them. Sums, references and the l terms are fp32; p s' is rounded to fp16 (relative 2^-11, of terms
+// that count from the middle of the codes), queries are exact in fp16 over 27 binades.
+//
+// A block computes with most of its warps, each 32 tokens of a unit at a time, and copies with the rest through a ring of stages
+// on barriers (bulk copies of a page's run at a time; every wait is bounded). The units of all sequences, heads and row tiles
+// form one line, cut evenly over the blocks on the device, since the lengths live there: a block's share may begin and end inside
+// a segment. Warps' parts of a piece meet in shared memory, blocks' parts of a segment in the workspace, where the block that
+// comes last adds them up in the order of the line: the same bits every time.
+//
+// What bounds it: for an SM's part of the copy rate (23 bytes a cycle) the 16 tokens of a warp's step, 2304 bytes of a 128-wide
+// head in groups of 64, may take 98 cycles. All told a step is 324 warp instructions, 81 cycles of the four schedulers; 149 of
+// them are masks, shifts and permutes on the ALU, which takes one every other cycle: 75 cycles; 18 are matrix products of 8 cycles: 37.
+// Four warps a scheduler, all of them on dependent chains (masks, products, exponentials, products), issue in 60 % of the cycles
+// and keep the ALU busy for 55 %: the kernel is bound by latency and issue, not by memory (51 % of its peak, or 67 % of the copy
+// rate without the profiler). Of 128-wide heads in groups of 64, one query a sequence: 32 ragged sequences of up to 30000 tokens, 8 kv
+// heads with 8 query heads each, 129 us (67 % of the copy rate); one of 131072 tokens 44 us (52 %); 48 of up to 4096 tokens
+// 44 us (41 %); one of 777 with 4 query heads each 14 us, all of it beginnings and ends: lengths, queries, first copies, merging.
+// Tried and slower or no faster: parameters widened to floats in shared memory (its wavefronts are then 80 % of what it can do),
+// every warp sending its own copies (a bulk copy takes its warp some 150 cycles), small runs copied 16 bytes a lane, 2 or 4
+// stages instead of 3, a third or fourth step's registers (spills). Tiles of 32 rows missed the tolerance: without room to centre
+// the codes, the product's truncated sums lose what the subtraction of the middle leaves.
 template <int D, int G, int NT, bool BF16, bool ALONE>
 __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     attention_kernel(const __grid_constant__ AttentionArguments args, uint32_t* status) {
@@ -615,7 +650,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     uint32_t mine = lane < args.batch ? cost_of(extent_of(args, lane, length_here, status)) : 0, total = mine;
     for (uint32_t i = lane + 32; i < args.batch; i += 32) total += cost_of(extent_of(args, i, args.lengths[i], status));
     total = __reduce_add_sync(0xffffffffu, total) * segments;
-    const uint32_t blocks = min(gridDim.x, max(total >> args.least_units, 1u));
+    const uint32_t blocks = min(gridDim.x, max(total / 2, 1u));
     if (blockIdx.x >= blocks) return;
     // The first `longer` blocks take a unit more than the others.
     const uint32_t share = total / blocks, longer = total - share * blocks;
@@ -752,7 +787,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     const bool sound = there && page < args.pages;
                     if (there && !sound) {
                         bad = true;
-                        if (first_copying) note(status, kBadPage, b, page);
+                        // (Of a page that only fills up 16 tokens beside the gap no row sees anything: it may be gone.)
+                        const int32_t begin = static_cast<int32_t>(run.entry * args.page_size + run.inside);
+                        const bool seen = begin < args.sinks || begin + static_cast<int32_t>(run.length) > extent.start;
+                        if (first_copying && seen) note(status, kBadPage, b, page);
                     }
                     const uint32_t row = (page * args.kv_heads + kv_head) * args.page_size + run.inside;
                     for (uint32_t left = __ballot_sync(0xffffffffu, sound) & own_runs; left; left &= left - 1) {
@@ -1554,8 +1592,8 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     // How many warps share a piece. One block an SM, of all the warps it holds, leaves the fewest parts to put together: for
     // segments fewer than the SMs, or than twice the SMs and long. Smaller blocks overlap one's beginnings and ends with others'
     // units: two an SM while each can take a whole segment, three beyond. (128-wide heads, 8 rows, groups of 64: 256 segments of
-    // 15000 tokens 135 us against 143 with two blocks; 296 of 2000 27.6 us with two, 34.2 with three, 35.5 with one; 384 of
-    // 2000 39.6 with three, 42.0 with two; 1024 of 300 30.3 with three, 35.0 with two, 47.9 with one.)
+    // 15000 tokens, before a lone block's registers were handed over, 135 us against 143 with two blocks; 296 of 2000 27.6 us with two,
+    // 34.2 with three, 35.5 with one; 384 of 2000 39.6 with three, 42.0 with two; 1024 of 300 30.3 with three, 35.0 with two, 47.9 with one.)
     const uint64_t sms = static_cast<uint64_t>(facts.sm_count);
     const bool lengthy = static_cast<uint64_t>(args.table_pages) * args.page_size > 8192;
     const uint32_t share = segments <= sms || (lengthy && segments < 2 * sms) ? 1 : segments <= 2 * sms ? 2 : 3;
@@ -1566,7 +1604,6 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     const uint32_t warps = Shape::most_warps(share, args.copying);
     const uint32_t resident = static_cast<uint32_t>(facts.sm_count) * share;
     const uint64_t unit_tokens = warps * cache::kWarpTokens;
-    args.least_units = 1;
     args.unit = cache::Divider(static_cast<uint32_t>(unit_tokens));
     args.tiles = cache::Divider(args.row_tiles);
     args.segment_cost = share == 1 ? 2 : 1;

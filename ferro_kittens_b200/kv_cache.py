@@ -158,7 +158,8 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
     ``q`` is ``[batch, queries, heads, head_dim]``, or ``[batch, heads, head_dim]`` for single tokens, with strides that are
     multiples of 8 elements; head h reads kv head ``h // (heads // kv_heads)``. ``lengths`` (int32 ``[batch]``) counts each
     sequence's tokens, the ``queries`` newest included, whose keys and values have been written; ``table`` (int32
-    ``[batch, pages]``) names its pages in order, and without one sequence b owns page b. Query t sits at
+    ``[batch, pages]``) names its pages in order (any number will do for pages that no row sees), and without one sequence b
+    owns page b. Query t sits at
     ``i = length - queries + t`` and sees the tokens ``j <= i``; with a ``window``, those with ``j > i - window`` and the first
     ``sinks``. Returns ``(out, lse)``: ``out`` like ``q``, packed, and ``lse`` fp32 natural-log normalisers ``[batch, (queries,) heads]``;
     a row that sees nothing is zero, its lse -inf.

@@ -365,6 +365,7 @@ int fk_groupnorm_tile(const void* source, void* destination, uint32_t rows, floa
  *
  * head_dim is 64 or 128, group 32, 64 or 128 and at most head_dim, element FK_BF16 or FK_F16 (of the
  * parameters and of the tensors that are written, read or asked with). Buffers are 16-byte aligned.
+ * Pages of 4 tokens or a multiple keep every row's parameters on 16 bytes for the attention's copies; others work, slower.
  * A slot is page * page_size + place. Indices live on the device, so a bad one is found there: it is
  * skipped (nothing is read or written out of bounds) and noted in `device_status`, which may be null
  * (fk_status_check then says FK_ERR_INVALID with the index). All calls are asynchronous on `stream`. */
@@ -390,7 +391,8 @@ int fk_cache_write(const fk_cache_t* cache, const void* k, const void* v, int64_
                    uint32_t slot_bytes, uint32_t tokens, void* stream, uint32_t* device_status);
 
 /* Read rows back: k[i, head, :] and v[i, head, :] become the values of slot slots[i] (which may repeat), rounded
- * once to the cache's type. Rows of negative slots are left as they were, or zeroed with `clear_skipped`. */
+ * once to the cache's type. Rows of negative slots are left as they were, or zeroed with `clear_skipped`.
+ * Rows may not lie over one another: strides of more than one token or head are head_dim or more. */
 int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_stride, int64_t k_head_stride,
                   int64_t v_token_stride, int64_t v_head_stride, const void* slots, uint32_t slot_bytes,
                   uint32_t tokens, int clear_skipped, void* stream, uint32_t* device_status);
@@ -398,19 +400,20 @@ int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_str
 /* Attention of each sequence's newest tokens over its rows of the cache, theirs included.
  *   q        [batch, queries, heads, head_dim], strides in elements, multiples of 8; heads is a multiple of
  *            kv_heads, and query head h reads kv head h / (heads / kv_heads)
- *   out      packed [batch, queries, heads, head_dim] of the cache's type; lse null or packed
+ *   out      packed [batch, queries, heads, head_dim] of the cache's type, not over q; lse null or packed
  *            [batch, queries, heads] fp32 (natural log)
  *   lengths  [batch] int32: tokens of each sequence, its `queries` newest among them; 0 or less is an empty
  *            sequence, and one shorter than `queries` has its first rows before its first token
- *   table    row b (of table_pages entries, table_stride apart) names sequence b's pages in order, and entries behind its
- *            length are never read; null: sequence b owns page b
+ *   table    row b (of table_pages entries, table_stride apart) names sequence b's pages in order; entries behind its
+ *            length are never read, and those of pages that no row sees may name any; null: sequence b owns page b
  * Query t of a sequence sits at i = length - queries + t and sees token j when j <= i and (window == 0, or
  * j > i - window, or j < sinks). A row that sees nothing is zero, its lse -inf. Tokens that no row of a sequence
- * sees are not read, and what a row does not see may hold anything, NaN included.
+ * sees are not read (but for the few that fill up 16 at the sinks' end and the window's beginning), and what a row does not
+ * see may hold anything, NaN included. `scale` is finite, of either sign.
  * Scores, softmax statistics and sums are fp32; a weight times its group's scale is rounded to fp16 (11 bits,
  * scaled so that the range always fits) for the product with the value codes, which are exact.
  * `workspace` is fk_cache_attention_workspace_bytes(sm_count) bytes, 16-byte aligned, ALL ZERO before its first
- * use; every call leaves its counters zero again, so it is cleared once. Calls that share a workspace must not
+ * use; every call leaves its counters zero again, so it is cleared once (and after a reported stall). Calls that share a workspace must not
  * overlap on the device (two streams, or two captured graphs that may run together, want one each). */
 uint64_t fk_cache_attention_workspace_bytes(uint32_t sm_count);
 int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_t q_batch_stride, int64_t q_token_stride,

@@ -346,6 +346,40 @@ def test_what_a_row_does_not_see_may_hold_anything(device):
     assert torch.equal(again[0][:, 0], want[0][:, 0])
 
 
+@pytest.mark.parametrize("page_size", [1, 4, 20, 64])
+@pytest.mark.parametrize("window,sinks,queries", [(21, 0, 1), (21, 2, 1), (1, 5, 1), (30, 17, 3)])
+def test_pages_that_no_row_sees_may_be_gone(device, page_size, window, sinks, queries):
+    lengths = [200, 199, 64]
+    per = -(-200 // page_size)
+    cache = _random_cache(device, 3 * per, page_size, 2, 128, 64, torch.bfloat16, 4)
+    table = _tables(device, 3, per, 3 * per)
+    q = torch.randn(3, queries, 8, 128, device=device).bfloat16()
+    at = torch.tensor(lengths, dtype=torch.int32, device=device)
+    want = kv_cache.attend(q, cache, at, table, window=window, sinks=sinks)
+    first, last = {}, {}
+    for b, n in enumerate(lengths):
+        for page in range(per):
+            tokens = range(page * page_size, min((page + 1) * page_size, n))
+            seen = [j for j in tokens if j < sinks or j > n - queries - window]
+            if not seen:
+                table[b, page] = -1 if page % 2 else 1 << 30
+            elif tokens[0] > n - queries - window:
+                last[b] = page
+            else:
+                first[b] = page
+    status = gemm.new_status(device)
+    for x, y in zip(kv_cache.attend(q, cache, at, table, window=window, sinks=sinks, status=status), want):
+        assert torch.equal(x, y)
+    gemm.check_status(status)
+    # One that some row sees may not.
+    page = last.get(1, first.get(1))
+    table[1, page] = -1
+    status = gemm.new_status(device)
+    kv_cache.attend(q, cache, at, table, window=window, sinks=sinks, status=status)
+    with pytest.raises(FerroKittensError, match="in the table of sequence 1"):
+        gemm.check_status(status)
+
+
 def test_bad_pages_and_lengths_are_noted_and_skipped(device):
     cache = _random_cache(device, 8, 16, 1, 128, 64, torch.bfloat16, 4)
     table = torch.tensor([[1, 2, 3], [4, 8, 5]], dtype=torch.int32, device=device)
