@@ -271,4 +271,36 @@ inline void groupnorm_tile(void* stream, uint64_t source, uint64_t destination, 
 
 }  // namespace rows
 
+/// The key/value cache in 4 bits (no counterpart in the crate; format and rules beside fk_cache_t).
+namespace kv_cache {
+
+inline std::size_t workspace_bytes(uint32_t sm_count) {
+    return static_cast<std::size_t>(fk_cache_attention_workspace_bytes(sm_count));
+}
+/// Tokens [tokens, kv_heads, head_dim], packed, into their slots (int32; negative ones skipped).
+inline void write(void* stream, const fk_cache_t& cache, uint64_t k, uint64_t v, const int32_t* slots, uint32_t tokens,
+                  uint32_t* status = nullptr) {
+    const int64_t head = cache.head_dim, token = head * cache.kv_heads;
+    check(fk_cache_write(&cache, reinterpret_cast<const void*>(k), reinterpret_cast<const void*>(v), token, head, token, head, slots, 4,
+                         tokens, stream, status));
+}
+/// Rows back into packed [tokens, kv_heads, head_dim]; those of negative slots are left as they were.
+inline void read(void* stream, const fk_cache_t& cache, uint64_t k, uint64_t v, const int32_t* slots, uint32_t tokens,
+                 uint32_t* status = nullptr) {
+    const int64_t head = cache.head_dim, token = head * cache.kv_heads;
+    check(fk_cache_read(&cache, reinterpret_cast<void*>(k), reinterpret_cast<void*>(v), token, head, token, head, slots, 4, tokens, 0,
+                        stream, status));
+}
+/// Attention of packed queries [batch, queries, heads, head_dim]; `table` is [batch, table_pages], or null.
+inline void attend(void* stream, const fk_cache_t& cache, uint64_t q, uint64_t out, float* lse, const int32_t* lengths,
+                   const int32_t* table, uint32_t table_pages, uint32_t batch, uint32_t queries, uint32_t heads, float scale,
+                   uint32_t window, uint32_t sinks, void* workspace, std::size_t workspace_size, uint32_t* status = nullptr) {
+    const int64_t head = cache.head_dim, token = head * heads;
+    check(fk_cache_attention(&cache, reinterpret_cast<const void*>(q), token * queries, token, head, reinterpret_cast<void*>(out), lse,
+                             lengths, table, table_pages, table_pages, batch, queries, heads, scale, window, sinks, workspace,
+                             workspace_size, stream, status));
+}
+
+}  // namespace kv_cache
+
 }  // namespace kittens
