@@ -607,7 +607,7 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
 // 44 us (41 %); one of 777 with 4 query heads each 14 us, all of it beginnings and ends: lengths, queries, first copies, merging.
 // Tried and slower or no faster: parameters widened to floats in shared memory (its wavefronts are then 80 % of what it can do),
 // every warp sending its own copies (a bulk copy takes its warp some 150 cycles), small runs copied 16 bytes a lane, 2 or 4
-// stages instead of 3, a third or fourth step's registers (spills). Tiles of 32 rows missed the tolerance: without room to centre
+// stages instead of 3, the next piece's queries held in registers (spills). Tiles of 32 rows missed the tolerance: without room to centre
 // the codes, the product's truncated sums lose what the subtraction of the middle leaves.
 template <int D, int G, int NT, bool BF16, bool ALONE>
 __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
