@@ -1416,7 +1416,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 }
 #pragma unroll
                 for (uint32_t k = 0; k < kItems; ++k) {
-                    if (stat[k].x == -INFINITY) continue;
+                    // A part without a visible token. (One whose scores are all NaN has no reference either, but a sum.)
+                    if (stat[k].y == 0.0f) continue;
                     const float m = fmaxf(all[k].x, stat[k].x), keep = ex2_approx(all[k].x - m), factor = ex2_approx(stat[k].x - m);
                     y[k] = make_float4(fmaf(z[k].x, factor, y[k].x * keep), fmaf(z[k].y, factor, y[k].y * keep),
                                        fmaf(z[k].z, factor, y[k].z * keep), fmaf(z[k].w, factor, y[k].w * keep));

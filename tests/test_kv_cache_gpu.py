@@ -502,6 +502,26 @@ def test_rows_that_hold_nan_or_infinite_queries_spoil_no_others(device):
         assert torch.allclose(lse[rest], want[1][rest], rtol=0, atol=2.0 ** -14)
 
 
+@pytest.mark.parametrize("heads", [4, 20])
+@pytest.mark.parametrize("length", [1, 600, 3000, 20000])
+def test_a_row_of_nothing_but_nan_stays_nan(device, heads, length):
+    """However many parts its segment is put together from, and whether the query or all keys made it NaN."""
+    page_size = 64
+    per = -(-length // page_size)
+    cache = _random_cache(device, per, page_size, 1, 128, 64, torch.bfloat16, 3)
+    table = _tables(device, 1, per, per)
+    at = torch.tensor([length], dtype=torch.int32, device=device)
+    q = torch.randn(1, 1, heads, 128, device=device).bfloat16()
+    q[0, 0, 2, 7] = float("nan")
+    out, lse = kv_cache.attend(q, cache, at, table)
+    bad = torch.arange(heads, device=device) == 2
+    assert torch.isnan(out[0, 0, bad]).all() and torch.isnan(lse[0, 0, bad]).all()
+    assert torch.isfinite(out[0, 0, ~bad]).all() and torch.isfinite(lse[0, 0, ~bad]).all()
+    cache.k_params[..., 0, :] = float("nan")
+    out, lse = kv_cache.attend(q, cache, at, table)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+
+
 def test_rows_past_four_gibibytes(device):
     """A cache whose codes pass 2^32 bytes on each side: the last pages, written, read and attended to."""
     page_size, kv_heads = 1024, 8
