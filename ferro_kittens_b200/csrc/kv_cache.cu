@@ -616,7 +616,6 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     using Shape = AttentionShape<D, G, NT>;
     constexpr uint32_t kGroups = Shape::kGroups, kRows = Shape::kRows, kPitch = Shape::kPitch;
     constexpr uint32_t kKeyWords = D / 32, kValueWords = D / 64, kTiles = D / 16;
-    constexpr bool kEights = NT == 1;  // see `eights` below
     extern __shared__ __align__(16) uint8_t shared[];
     __shared__ uint64_t barriers[2 * kStages];  // of each stage: it is full; it is free again
     __shared__ uint32_t bad_pages[kStages];     // whether a stage has places whose page lies outside the cache
@@ -979,7 +978,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 
         // Pairs are a fragment's two rows. Scores and peaks are the products' sums; times to_log2 they are powers of two, and
         // minus_peak is -peak in powers of two, 0 while peak is -inf.
-        float out[kTiles][NT][4] = {}, eights[kEights ? kGroups : 1][NT][4] = {};
+        float out[kTiles][NT][4] = {};
         float2 lows[kGroups][NT] = {}, peak[NT], minus_peak[NT] = {}, sum[NT] = {};
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) peak[n] = make_float2(-INFINITY, -INFINITY);
@@ -1021,8 +1020,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
             // subnormal), one in the next nibble code * 2^-20: masks alone unpack them, and products are exact.
             float2 x[2][NT][2];  // [step of 16 tokens][row tile][token of the fragment's upper or lower half] (two rows)
-            // One step's products, or for several row tiles both steps' for each load of a query fragment.
-            const auto products = [&](uint32_t g, const auto& a, auto& part, auto steps) {
+            // Both steps' products, for each load of a query fragment. (With 8 rows, whose fragments stay in registers, it is the
+            // two chains that count: 46.4 us for one sequence of 131072 against 48.7 step by step.)
+            const auto products = [&](uint32_t g, const uint32_t (&a)[2][2][kKeyWords], float (&part)[2][NT][4]) {
 #pragma unroll
                 for (uint32_t w = g * (G / 32); w < (g + 1) * (G / 32); ++w)
 #pragma unroll
@@ -1033,7 +1033,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         else
                             f[0] = qf[2 * w][0], f[1] = qf[2 * w][1], f[2] = qf[2 * w + 1][0], f[3] = qf[2 * w + 1][1];
 #pragma unroll
-                        for (uint32_t h = 0; h < decltype(steps)::value; ++h) {
+                        for (uint32_t h = 0; h < 2; ++h) {
                             const uint32_t y0 = a[h][0][w] >> 8, y1 = a[h][1][w] >> 8;
                             mma_16x8x16(part[h][n], a[h][0][w] & 0x000f000fu, a[h][1][w] & 0x000f000fu, a[h][0][w] & 0x00f000f0u,
                                         a[h][1][w] & 0x00f000f0u, f[0], f[1]);
@@ -1064,24 +1064,20 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     }
                 }
             };
-            constexpr uint32_t kTogether = NT > 1 ? 2 : 1;
+            uint32_t a[2][2][kKeyWords], pairs[2][2][kGroups];
 #pragma unroll
-            for (uint32_t h0 = 0; h0 < 2; h0 += kTogether) {
-                uint32_t a[kTogether][2][kKeyWords], pairs[kTogether][2][kGroups];
+            for (uint32_t h = 0; h < 2; ++h) {
+                load_keys(h, a[h]);
 #pragma unroll
-                for (uint32_t h = 0; h < kTogether; ++h) {
-                    load_keys(h0 + h, a[h]);
+                for (uint32_t half = 0; half < 2; ++half)
+                    load_words(pairs[h][half], key_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
+            }
 #pragma unroll
-                    for (uint32_t half = 0; half < 2; ++half)
-                        load_words(pairs[h][half], key_params + (16 * (h0 + h) + 8 * half + own_token) * (kGroups * 4));
-                }
+            for (uint32_t g = 0; g < kGroups; ++g) {
+                float part[2][NT][4] = {};
+                products(g, a, part);
 #pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g) {
-                    float part[kTogether][NT][4] = {};
-                    products(g, a, part, std::integral_constant<uint32_t, kTogether>{});
-#pragma unroll
-                    for (uint32_t h = 0; h < kTogether; ++h) add_up(h0 + h, g, pairs[h], part[h]);
-                }
+                for (uint32_t h = 0; h < 2; ++h) add_up(h, g, pairs[h], part[h]);
             }
 
             // ---- what rarely happens, all in one place: tokens that some row may not see; a score more than kSlack above its
@@ -1194,10 +1190,6 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         const float factor = keep[i % 2] * shrink;
 #pragma unroll
                         for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= factor;
-                        if constexpr (kEights) {
-#pragma unroll
-                            for (uint32_t g = 0; g < kGroups; ++g) eights[g][n][i] *= factor;
-                        }
                     }
                 }
             }
@@ -1229,18 +1221,11 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     }
                 }
                 // ---- O^T += V^T . (P scale)^T. Two tokens' nibbles of a channel side by side are a pair of the first
-                // operand; the odd fragment rows' channels come 16 times too large. Codes count from their middle, 8,
-                // with 8 * weight in fp32 in `lows`. For one row tile `eights`, a product with a constant, sums 8 * weight
-                // as rounded, to be taken off at the end; for more, whose registers are full, the codes are made normal
-                // numbers and 8 is subtracted from them.
-                if constexpr (kEights) {
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g)
-#pragma unroll
-                        for (uint32_t n = 0; n < NT; ++n)
-                            mma_16x8x16(eights[g][n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u,
-                                        weights[g][n][0], weights[g][n][1]);
-                }
+                // operand; the odd fragment rows' channels come 16 times too large. Codes are made normal numbers that count
+                // from their middle, 8, with 8 * weight in fp32 in `lows`: a token of nearly all the weight and a value near the
+                // middle adds nothing to what the product truncates. (A product with a constant 8, to be taken off at the
+                // end, saves the additions and 4 to 10 % of the time, but the truncations of its sum and of the codes' differ by up to 2^-13
+                // of a scale, more than everything else there.)
                 uint32_t v[4][kValueWords];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) load_words(v[i], values + (16 * h + 8 * (i / 2) + 2 * c4 + ((i ^ (c4 >> 1)) & 1u)) * (D / 2) + l4 * (D / 16));
@@ -1254,12 +1239,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         for (uint32_t byte = 0; byte < 2; ++byte) {
                             const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
                             uint32_t codes[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
-                            if constexpr (!kEights) {
-                                codes[0] = add_f16x2(codes[0] | 0x64006400u, 0xe408e408u);  // 1024 + code - 1032
-                                codes[1] = add_f16x2(codes[1] | 0x64006400u, 0xe480e480u);  // 1024 + 16 code - 1152
-                                codes[2] = add_f16x2(codes[2] | 0x64006400u, 0xe408e408u);
-                                codes[3] = add_f16x2(codes[3] | 0x64006400u, 0xe480e480u);
-                            }
+                            codes[0] = add_f16x2(codes[0] | 0x64006400u, 0xe408e408u);  // 1024 + code - 1032
+                            codes[1] = add_f16x2(codes[1] | 0x64006400u, 0xe480e480u);  // 1024 + 16 code - 1152
+                            codes[2] = add_f16x2(codes[2] | 0x64006400u, 0xe408e408u);
+                            codes[3] = add_f16x2(codes[3] | 0x64006400u, 0xe480e480u);
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n)
                                 mma_16x8x16(out[j][n], codes[0], codes[1], codes[2], codes[3], weights[g][n][0], weights[g][n][1]);
@@ -1308,13 +1291,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 #pragma unroll
                     for (uint32_t j = 0; j < kTiles; ++j) {
                         const uint32_t g = 16 * j / G;
-                        float y = out[j][n][e], odd_y = out[j][n][2 + e] * 0.0625f;
-                        if constexpr (kEights) {
-                            y = (y - eights[g][n][e]) * 0x1p24f;
-                            odd_y = (odd_y - eights[g][n][e]) * 0x1p24f;
-                        }
-                        merged[row * kPitch + 16 * j + l4] = fmaf(y, unfit, low[g]);
-                        merged[row * kPitch + 16 * j + 8 + l4] = fmaf(odd_y, unfit, low[g]);
+                        merged[row * kPitch + 16 * j + l4] = fmaf(out[j][n][e], unfit, low[g]);
+                        merged[row * kPitch + 16 * j + 8 + l4] = fmaf(out[j][n][2 + e] * 0.0625f, unfit, low[g]);
                     }
                     if (l4 == 0) {
                         stats[2 * row] = (e ? peak[n].y : peak[n].x) * to_log2;

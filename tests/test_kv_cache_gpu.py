@@ -297,6 +297,25 @@ def test_attention_drawn(device, seed):
                      sinks=sinks)
 
 
+@pytest.mark.parametrize("head_dim,group,dtype", FORMATS)
+@pytest.mark.parametrize("ratio", [3, 12])
+def test_a_token_of_nearly_all_the_weight_whose_value_is_zero(device, head_dim, group, dtype, ratio):
+    """Its code is the middle, 8, and its smallest value -8 scales: what the others add must not drown in what cancels."""
+    g = torch.Generator(device=device)
+    g.manual_seed(5)
+    cache = _random_cache(device, 3, 64, 1, head_dim, group, dtype, 5)
+    for page, token in ((0, 46), (1, 7), (2, 30)):
+        cache.k_codes[page, 0, token] = 0xff
+        cache.v_codes[page, 0, token] = 0x88
+        cache.k_params[page, 0, token, :, 0], cache.k_params[page, 0, token, :, 1] = 0.25, -1.5
+        cache.v_params[page, 0, token, :, 0], cache.v_params[page, 0, token, :, 1] = 0.25, -2.0
+    # The token's key is 2.25 in every channel, so that queries of one sign give it scores 5 to 12 above the others'.
+    for size in (0.2, 0.3, 0.45):
+        q = (size * 128 / head_dim * (0.5 + torch.rand(3, 1, ratio, head_dim, device=device, generator=g))).to(dtype)
+        _check_attention(device, cache, q, torch.tensor([50, 31, 64], dtype=torch.int32, device=device),
+                         torch.tensor([[0], [1], [2]], dtype=torch.int32, device=device))
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (2, 3), (64, 4), (100, 0), (128, 130), (5000, 4), (37, 1000)])
 @pytest.mark.parametrize("queries", [1, 4])
 def test_attention_window_and_sinks(device, window, sinks, queries):
