@@ -144,8 +144,8 @@ def read(cache: Cache, slots: torch.Tensor, k: torch.Tensor | None = None, v: to
         raise ValueError("k and v are given together or not at all")
     fresh = k is None
     if fresh:
-        k, v = (torch.empty((slots.shape[0], cache.kv_heads, cache.head_dim), dtype=cache.dtype, device=cache.device)
-                for _ in range(2))
+        k = slots.new_empty((slots.shape[0], cache.kv_heads, cache.head_dim), dtype=cache.dtype)
+        v = torch.empty_like(k)
     _rows(library().fk_cache_read, cache, k, v, slots, status, int(fresh))
     return k, v
 
@@ -189,14 +189,14 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
         raise ValueError(f"the workspace must be a contiguous tensor on {cache.device}")
     shape = (batch, queries, heads, head_dim)
     if out is None:
-        out = torch.empty(shape, dtype=cache.dtype, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         if squeeze and out.dim() == 3:
             out = out.unsqueeze(1)
         _require("out", out, cache, 4)
         if out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape")
-    lse = torch.empty(shape[:3], dtype=torch.float32, device=cache.device)
+    lse = lengths.new_empty(shape[:3], dtype=torch.float32)
     strides = q.stride()
     _on(cache.device, lambda stream: library().fk_cache_attention(
         cache.view, q.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(), lse.data_ptr(),
