@@ -533,6 +533,12 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
     return d;
 }
+/// (x & mask) | more in one instruction, which the compiler otherwise makes two of where both are constants.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t more) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(more));
+    return d;
+}
 __device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -1229,8 +1235,10 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 // operand; the odd fragment rows' channels come 16 times too large. Codes are made normal numbers that count
                 // from their middle, 8, with 8 * weight in fp32 in `lows`: a token of nearly all the weight and a value near the
                 // middle adds nothing to what the product truncates. (A product with a constant 8, to be taken off at the
-                // end, saves the additions and 4 to 10 % of the time, but the truncations of its sum and of the codes' differ by up to 2^-13
+                // end, saves the additions and up to 3 % of the time, but the truncations of its sum and of the codes' differ by up to 2^-13
                 // of a scale, more than everything else there.)
+                uint32_t thousands = 0x64006400u;
+                asm("" : "+r"(thousands));  // two constants in one instruction: one of them in a register
                 uint32_t v[4][kValueWords];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) load_words(v[i], values + (16 * h + 8 * (i / 2) + 2 * c4 + ((i ^ (c4 >> 1)) & 1u)) * (D / 2) + l4 * (D / 16));
@@ -1243,11 +1251,11 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 #pragma unroll
                         for (uint32_t byte = 0; byte < 2; ++byte) {
                             const uint32_t j = 4 * w + 2 * half + byte, g = 16 * j / G;
-                            uint32_t codes[4] = {lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u};
-                            codes[0] = add_f16x2(codes[0] | 0x64006400u, 0xe408e408u);  // 1024 + code - 1032
-                            codes[1] = add_f16x2(codes[1] | 0x64006400u, 0xe480e480u);  // 1024 + 16 code - 1152
-                            codes[2] = add_f16x2(codes[2] | 0x64006400u, 0xe408e408u);
-                            codes[3] = add_f16x2(codes[3] | 0x64006400u, 0xe480e480u);
+                            const uint32_t codes[4] = {
+                                add_f16x2(and_or(lo, 0x000f000fu, thousands), 0xe408e408u),  // 1024 + code - 1032
+                                add_f16x2(and_or(lo, 0x00f000f0u, thousands), 0xe480e480u),  // 1024 + 16 code - 1152
+                                add_f16x2(and_or(hi, 0x000f000fu, thousands), 0xe408e408u),
+                                add_f16x2(and_or(hi, 0x00f000f0u, thousands), 0xe480e480u)};
 #pragma unroll
                             for (uint32_t n = 0; n < NT; ++n)
                                 mma_16x8x16(out[j][n], codes[0], codes[1], codes[2], codes[3], weights[g][n][0], weights[g][n][1]);
