@@ -608,17 +608,17 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
 // comes last adds them up in the order of the line: the same bits every time.
 //
 // What bounds it: for an SM's part of the copy rate (23 bytes a cycle) the 16 tokens of a warp's step, 2304 bytes of a 128-wide
-// head in groups of 64, may take 98 cycles. All told a step is 324 warp instructions, 81 cycles of the four schedulers; 149 of
-// them are masks, shifts and permutes on the ALU, which takes one every other cycle: 75 cycles; 18 are matrix products of 8 cycles: 37.
-// Four warps a scheduler, all of them on dependent chains (masks, products, exponentials, products), issue in 60 % of the cycles
-// and keep the ALU busy for 55 %: the kernel is bound by latency and issue, not by memory (51 % of its peak, or 67 % of the copy
-// rate without the profiler). Of 128-wide heads in groups of 64, one query a sequence: 32 ragged sequences of up to 30000 tokens, 8 kv
-// heads with 8 query heads each, 129 us (67 % of the copy rate); one of 131072 tokens 44 us (52 %); 48 of up to 4096 tokens
-// 44 us (41 %); one of 777 with 4 query heads each 14 us, all of it beginnings and ends: lengths, queries, first copies, merging.
+// head in groups of 64, may take 98 cycles. All told a step is 349 warp instructions, 87 cycles of the four schedulers; 147 of
+// them are masks, shifts and permutes on the ALU, which takes one every other cycle: 74 cycles; 16 are matrix products of 8 cycles: 33.
+// Four warps a scheduler, all of them on dependent chains (masks, products, exponentials, products), issue in 62 % of the cycles
+// and keep the ALU busy for 52 %: the kernel is bound by latency and issue, not by memory (50 % of its peak under the profiler). Of
+// 128-wide heads in groups of 64, one query a sequence: 32 ragged sequences of up to 30000 tokens, 8 kv heads with 8 query heads
+// each, 134 us (65 % of the copy rate); one of 131072 tokens 46 us (50 %); 48 of up to 4096 tokens 44 us (42 %); one
+// of 777 with 4 query heads each 14 us, all of it beginnings and ends: lengths, queries, first copies, merging.
 // Tried and slower or no faster: parameters widened to floats in shared memory (its wavefronts are then 80 % of what it can do),
 // every warp sending its own copies (a bulk copy takes its warp some 150 cycles), small runs copied 16 bytes a lane, 2 or 4
-// stages instead of 3, the next piece's queries held in registers (spills). Tiles of 32 rows missed the tolerance: without room to centre
-// the codes, the product's truncated sums lose what the subtraction of the middle leaves.
+// stages instead of 3, the next piece's queries held in registers (spills). Tiles of 32 rows missed the tolerance: they left no
+// registers to centre the codes in.
 template <int D, int G, int NT, bool BF16, bool ALONE>
 __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     attention_kernel(const __grid_constant__ AttentionArguments args, uint32_t* status) {
