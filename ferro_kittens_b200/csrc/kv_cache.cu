@@ -269,13 +269,14 @@ __device__ __forceinline__ uint32_t group_codes(const uint4 x, uint32_t params, 
         nearest = fmaxf(nearest, fmaxf(rest.x, rest.y));
     }
     // t is exact but where a value or the smallest one all but vanishes in it: there its rounding may have made a half step of the
-    // remainder. Where the scale was cut short (of a span of a few subnormals) codes pass 15, and far scales leave fp32's range
+    // remainder. (Of one channel's, while another's may lie above half a step, by what the guess is low: so the largest remainder
+    // says where none can be.) Where the scale was cut short (of a span of a few subnormals) codes pass 15, and far scales leave fp32's range
     // in t or in 1 / scale. All these go the long way, far scales lifted by 2^100 or halved (exactly).
     uint32_t small = E::min_magnitude(E::min_magnitude(words[0], words[1]), E::min_magnitude(words[2], words[3]));
     small = E::min_magnitude(small, __byte_perm(small, params, 0x7632));  // with its other half, and the smallest value
     const float vanishing = fminf(fabsf(E::low(small)), fabsf(E::high(small)));
     const bool far = scale < 0x1p-100f || scale > 0x1p100f;
-    if (scale > 0.0f && ((nearest == half_step && vanishing < span * E::kVanishes) || span >= 15.5f * scale || far)) {
+    if (scale > 0.0f && ((nearest >= half_step && vanishing < span * E::kVanishes) || span >= 15.5f * scale || far)) {
         const float lift = scale > 0x1p100f ? 0.5f : scale < 0x1p-100f ? 0x1p100f : 1.0f;
         const float step = scale * lift, origin = -low * lift, lifted_half = 0.5f * step;
         const float lifted_inverse = __frcp_rn(step);
