@@ -443,9 +443,10 @@ template <int D, int G, int NT>
 struct AttentionShape {
     static constexpr uint32_t kGroups = D / G;
     static constexpr uint32_t kRows = 8 * NT;
-    // One row tile's queries stay in registers; of more, the fragments and sums lie in shared memory.
+    // One row tile's queries stay in registers; of more, the fragments, the groups' sums and what makes powers of two of the rows'
+    // scores lie in shared memory.
     static constexpr bool kSharedQueries = NT > 1;
-    static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 : 0;
+    static constexpr uint32_t kQueryBytes = kSharedQueries ? kRows * D * 2 + kRows * kGroups * 4 + kRows * 4 : 0;
     // For each computing warp: its tokens in each stage. The merge of the warps' results lies over the piece's last stage, which
     // is given back after it, or (where rows are more than fit there) beside.
     static constexpr uint32_t kCodeBytes = kWarpTokens * D / 2;
@@ -632,7 +633,6 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     __shared__ uint32_t bad_pages[kStages];     // whether a stage has places whose page lies outside the cache
     __shared__ uint32_t stop_flag, complete[2];
     __shared__ Cut cuts[2];              // the parts of segments that are cut over blocks: the one this share begins in, ends in
-    __shared__ uint32_t tile_most[NT];   // largest magnitudes of the tile's queries
     // The first warps compute, the last ones copy.
     const uint32_t warps = blockDim.x / 32 - args.copying, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t unit_tokens = warps * kWarpTokens;
@@ -856,6 +856,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 
     if constexpr (ALONE) setmaxnreg_inc<Shape::kComputingRegisters>();
     const uint32_t l4 = lane / 4, c4 = lane % 4;
+    // Row l4 of tile n, and its largest magnitude (a NaN's aside; 0 if there is an infinity: the row is NaN whatever it is scaled by).
     const auto load_row = [&](uint32_t n, uint4 (&raw)[kKeyWords]) {
         const uint32_t r = first_row + 8 * n + l4, t = args.ratio.quotient(min(r, args.rows - 1));
         const uint8_t* const q = args.q + b * args.q_batch_stride + t * args.q_token_stride +
@@ -868,7 +869,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));
         }
-        return most < INFINITY ? most : 0.0f;  // a row that holds an infinity says nothing about others
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        return most < INFINITY ? most : 0.0f;
     };
     // A piece's queries, on their way to the nearest cache while the piece before is put together.
     const auto fetch_rows = [&]() {
@@ -913,16 +916,29 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     bool more = find_piece();
     while (more) {
         // ---- queries as the second operand of the scores' product: lane (l4, c4) holds row l4 of each 8, in the
-        // channel order of the key codes. The tile is scaled by a power of two so that its largest value lies in
-        // [2^14, 2^15): its fp16 form is exact over 27 binades, and the second register of each pair carries 1/16 for
-        // the codes that stay in the upper nibble. q_sum is a group's sum, for the smallest values; to_log2 makes scores
-        // of the products, in powers of two.
+        // channel order of the key codes. Each row is scaled by a power of two of its own, so that its largest value lies in
+        // [2^14, 2^15) whatever the other rows hold. The second register of each pair carries 1/16 for the codes that stay in the
+        // upper nibble, so its fp16 form is exact down to 2^-27 of the largest value in bf16 and 2^-24 in fp16, and below that
+        // off by 2^-35 of the largest value. q_sum is a group's sum, for the smallest values; to_log2 makes scores of a row's products, in
+        // powers of two.
         uint32_t qf[Shape::kSharedQueries ? 1 : D / 16][2];
         float q_sum[Shape::kSharedQueries ? 1 : kGroups][2];
         uint4* const shared_q = reinterpret_cast<uint4*>(shared);
         float* const shared_sums = reinterpret_cast<float*>(shared + kRows * D * 2);
+        float* const shared_log2 = shared_sums + kRows * kGroups;
         const auto power_for = [](float most) {
             return most == 0.0f ? 127 : min(268 - static_cast<int32_t>(__float_as_uint(most) >> 23), 254);
+        };
+        // (With a scale of 0 every finite score is 0, whatever the keys.)
+        const auto factor_for = [&](int32_t power) {
+            return args.scale == 0.0f ? 0.0f : args.scale < 0.0f ? -power_of_two(power) : power_of_two(power);
+        };
+        // |scale| log2(e) 2^24 / 2^(power - 127), in two steps that stay inside fp32's range, and kept off its ends: zero or an infinity
+        // would make NaN of a hidden token's -inf or of equal scores' difference.
+        const auto log2_for = [&](int32_t power) {
+            const int32_t exponent = 151 - power, half = exponent / 2;
+            const float x = fabsf(args.scale) * 1.4426950408889634f * power_of_two(127 + half) * power_of_two(127 + exponent - half);
+            return fminf(fmaxf(x, 1e-37f), 0x1p126f);
         };
         const auto convert_row = [&](const uint4 (&raw)[kKeyWords], float up, uint4 (&f)[kKeyWords], float (&sums)[kGroups]) {
 #pragma unroll
@@ -947,34 +963,29 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 sums[g] *= 0x1p-24f;
             }
         };
-        int32_t power;
+        float2 to_log2[NT];
         {
             uint4 raw[kKeyWords], f[kKeyWords];
             if constexpr (Shape::kSharedQueries) {
                 for (uint32_t n = warp; n < NT; n += warps) {
-                    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(load_row(n, raw)));
-                    if (lane == 0) tile_most[n] = most;
-                }
-                sync_computing(warps * 32);
-                uint32_t most = 0;
-#pragma unroll
-                for (uint32_t n = 0; n < NT; ++n) most = max(most, tile_most[n]);
-                power = power_for(__uint_as_float(most));
-                for (uint32_t n = warp; n < NT; n += warps) {
                     float sums[kGroups] = {};
-                    load_row(n, raw);
-                    convert_row(raw, args.scale < 0.0f ? -power_of_two(power) : power_of_two(power), f, sums);
+                    const int32_t power = power_for(load_row(n, raw));
+                    convert_row(raw, factor_for(power), f, sums);
 #pragma unroll
                     for (uint32_t w = 0; w < kKeyWords; ++w) shared_q[(n * kKeyWords + w) * 32 + lane] = f[w];
+                    if (c4 == 0) {
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g)
-                        if (c4 == 0) shared_sums[g * kRows + 8 * n + l4] = sums[g];
+                        for (uint32_t g = 0; g < kGroups; ++g) shared_sums[g * kRows + 8 * n + l4] = sums[g];
+                        shared_log2[8 * n + l4] = log2_for(power);
+                    }
                 }
                 sync_computing(warps * 32);
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) to_log2[n] = *reinterpret_cast<const float2*>(shared_log2 + 8 * n + 2 * c4);
             } else {
-                power = power_for(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(load_row(0, raw)))));
+                const int32_t power = power_for(load_row(0, raw));
                 float sums[kGroups] = {};
-                convert_row(raw, args.scale < 0.0f ? -power_of_two(power) : power_of_two(power), f, sums);
+                convert_row(raw, factor_for(power), f, sums);
 #pragma unroll
                 for (uint32_t w = 0; w < kKeyWords; ++w)
                     qf[2 * w][0] = f[w].x, qf[2 * w][1] = f[w].y, qf[2 * w + 1][0] = f[w].z, qf[2 * w + 1][1] = f[w].w;
@@ -982,18 +993,17 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 for (uint32_t g = 0; g < kGroups; ++g)
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) q_sum[g][e] = __shfl_sync(0xffffffffu, sums[g], 8 * c4 + 4 * e);
+                const float own = log2_for(power);
+                to_log2[0] = make_float2(__shfl_sync(0xffffffffu, own, 8 * c4), __shfl_sync(0xffffffffu, own, 8 * c4 + 4));
             }
         }
-        // (Zero would make NaN of a hidden token's -inf.)
-        const float to_log2 = fmaxf(fabsf(args.scale) * 1.4426950408889634f * 0x1p24f * power_of_two(254 - power), 1e-37f);
-        const float slack = __fdividef(kSlack, to_log2);
 
-        // Pairs are a fragment's two rows. Scores and peaks are the products' sums; times to_log2 they are powers of two, and
-        // minus_peak is -peak in powers of two, 0 while peak is -inf.
+        // Pairs are a fragment's two rows. Scores are the products' sums; times to_log2 they are powers of two. minus_peak is the
+        // row's reference in powers of two, negative, and ceiling the score 2^kSlack above it: 0 and -inf while nothing is seen.
         float out[kTiles][NT][4] = {};
-        float2 lows[kGroups][NT] = {}, peak[NT], minus_peak[NT] = {}, sum[NT] = {};
+        float2 lows[kGroups][NT] = {}, ceiling[NT], minus_peak[NT] = {}, sum[NT] = {};
 #pragma unroll
-        for (uint32_t n = 0; n < NT; ++n) peak[n] = make_float2(-INFINITY, -INFINITY);
+        for (uint32_t n = 0; n < NT; ++n) ceiling[n] = make_float2(-INFINITY, -INFINITY);
         int32_t top = 0;  // biased exponent of the largest value scale so far
         float fit = power_of_two(254), limit = 0x1p-126f;  // limit: the least scale that would raise top
 
@@ -1105,7 +1115,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             };
             look();
 #pragma unroll
-            for (uint32_t n = 0; n < NT; ++n) grows |= largest[n].x > peak[n].x + slack || largest[n].y > peak[n].y + slack;
+            for (uint32_t n = 0; n < NT; ++n) grows |= largest[n].x > ceiling[n].x || largest[n].y > ceiling[n].y;
             if (is_masked || __any_sync(0xffffffffu, grows)) {
                 if (is_masked) {
                     uint32_t real = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1;
@@ -1181,18 +1191,24 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                 }
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n) {
-                    float keep[2], m[2] = {largest[n].x, largest[n].y}, was[2] = {peak[n].x, peak[n].y};
+                    float keep[2], m[2] = {largest[n].x, largest[n].y};
 #pragma unroll
                     for (uint32_t e = 0; e < 2; ++e) {
                         m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 4));
                         m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 8));
                         m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 16));
-                        keep[e] = m[e] > was[e] ? ex2_approx((was[e] - m[e]) * to_log2) : 1.0f;
-                        m[e] = fmaxf(m[e], was[e]);
+                        // While a row has seen nothing its scores are -inf: so are its exponentials, with nothing taken off.
+                        float& minus = e ? minus_peak[n].y : minus_peak[n].x;
+                        float& over = e ? ceiling[n].y : ceiling[n].x;
+                        const float its_log2 = e ? to_log2[n].y : to_log2[n].x;
+                        const float power = m[e] * its_log2, was = over == -INFINITY ? -INFINITY : -minus;
+                        keep[e] = 1.0f;
+                        if (power > was) {
+                            keep[e] = ex2_approx(was - power);
+                            minus = -power;
+                            over = m[e] + __fdividef(kSlack, its_log2);
+                        }
                     }
-                    peak[n] = make_float2(m[0], m[1]);
-                    // While a row has seen nothing its scores are -inf: so are its exponents, with nothing taken off.
-                    minus_peak[n] = make_float2(m[0] == -INFINITY ? 0.0f : -m[0] * to_log2, m[1] == -INFINITY ? 0.0f : -m[1] * to_log2);
                     const float2 keep2 = make_float2(keep[0], keep[1]);
                     sum[n] = __fmul2_rn(sum[n], keep2);
 #pragma unroll
@@ -1217,7 +1233,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     load_words(pairs, value_params + (16 * h + 8 * half + own_token) * (kGroups * 4));
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n) {
-                        const float2 power = __ffma2_rn(x[h][n][half], make_float2(to_log2, to_log2), minus_peak[n]);
+                        const float2 power = __ffma2_rn(x[h][n][half], to_log2[n], minus_peak[n]);
                         p[n] = make_float2(ex2_approx(power.x), ex2_approx(power.y));
                         sum[n] = __fadd2_rn(sum[n], p[n]);
                     }
@@ -1309,7 +1325,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                         merged[row * kPitch + 16 * j + 8 + l4] = fmaf(out[j][n][2 + e] * 0.0625f, unfit, low[g]);
                     }
                     if (l4 == 0) {
-                        stats[2 * row] = (e ? peak[n].y : peak[n].x) * to_log2;
+                        stats[2 * row] = (e ? ceiling[n].y : ceiling[n].x) == -INFINITY ? -INFINITY : -(e ? minus_peak[n].y : minus_peak[n].x);
                         stats[2 * row + 1] = s;
                     }
                 }

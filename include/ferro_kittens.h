@@ -409,7 +409,9 @@ int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_str
  * Query t of a sequence sits at i = length - queries + t and sees token j when j <= i and (window == 0, or
  * j > i - window, or j < sinks). A row that sees nothing is zero, its lse -inf. Tokens that no row of a sequence
  * sees are not read (but for the few that fill up 16 at the sinks' end and the window's beginning), and what a row does not
- * see may hold anything, NaN included. `scale` is finite, of either sign.
+ * see may hold anything, NaN included. `scale` is finite, of either sign; a row's queries are scaled by a power of two of their
+ * own, so that its result does not depend on the sizes of other rows' (one whose largest query times `scale` passes 2^115 is outside
+ * what its fp32 scores hold).
  * Scores, softmax statistics and sums are fp32; a weight times its group's scale is rounded to fp16 (11 bits,
  * scaled so that the range always fits) for the product with the value codes, which are exact.
  * `workspace` is fk_cache_attention_workspace_bytes(sm_count) bytes, 16-byte aligned, ALL ZERO before its first
