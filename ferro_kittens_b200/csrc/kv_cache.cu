@@ -145,6 +145,14 @@ struct Element<false> {
     }
 };
 
+/// Whether a group's parameters give finite values to weigh, their middle, low + 8 * scale, among them (that of written ones lies
+/// between the smallest and the largest value).
+template <bool BF16>
+__device__ __forceinline__ bool usable_params(uint32_t pair) {
+    using E = Element<BF16>;
+    return E::finite(pair) && fabsf(fmaf(8.0f, E::low(pair), E::high(pair))) < __uint_as_float(0x7f800000u);
+}
+
 /// The 8 x 8 matrix of nibbles held one row a lane by eight neighbouring lanes, transposed (its own inverse):
 /// halves, bytes, then nibbles change places with the lane 4, 2 and 1 away.
 __device__ __forceinline__ uint32_t transpose_nibbles(uint32_t x, uint32_t lane) {
@@ -430,12 +438,18 @@ constexpr uint32_t kMostBlocksPerSm = 3;
 constexpr uint32_t kMostRows = 16;
 /// Floats of one block's part of a segment: rows of outputs, then (peak, total) of each row.
 constexpr uint32_t kPartialFloats = kMostRows * (128 + 2);
-/// How far (in powers of two) a score may lie above its row's reference before the reference is moved. Weights reach
-/// 2^kSlack, so weight * scale, in fp16, has the largest scale at 2^kFit: 2^15 at most, and under 2^-14 (where fp16 loses
-/// bits) only weights 2^-21 of the reference's.
-constexpr float kSlack = 8.0f;
-constexpr int32_t kFit = 6;
-constexpr int32_t kFitBiased = 254 + kFit;  // less a scale's biased exponent: that of the power that brings it to 2^kFit
+/// How far (in powers of two) a score may lie above its row's reference before the reference is moved: weights reach 2^kSlack.
+constexpr float kSlack = 6.0f;
+/// Each group of channels has a power of two, `fit`, that brings its value scales into [kLeast, kMost) for the product with the codes:
+/// weight * scale * fit is under 2^15. A weight loses bits to fp16's subnormals under 2^-14 only, and errs by at most 2^-24 there, as its
+/// scale's product with the row's largest weight, 1 or more. Tokens of scales outside the window are multiplied in fp32.
+constexpr float kLeast = 0.5f, kMost = 512.0f;
+constexpr int32_t kFitBiased = 254 + 4;  // less a scale's biased exponent: that of the power that brings it into [2^4, 2^5)
+constexpr int32_t kMostFit = 253;        // biased exponents of powers whose inverses are normal numbers, too
+/// That many tokens of 32 outside the window move it: their scales' mean exponent to 2^4. (32 sequences of up to 30000 tokens take 137 us,
+/// 196 with one token in 32 outside.)
+constexpr uint32_t kManyFar = 8;
+constexpr int32_t kFarthest = 80;  // how far (in powers of two) a scale may lie above the window's middle, for fp32's range
 constexpr uint32_t kStallFull = 0x504;  // a computing warp waiting for a stage of tokens
 constexpr uint32_t kStallFree = 0x505;  // a copying warp waiting for a stage to be free
 
@@ -601,7 +615,8 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
 // ever multiplied out. Scores and outputs are computed transposed (tokens, then channels, are the rows of the m16n8k16
 // fragments, query rows the columns): eight rows fill the instruction, a lane holds two tokens' parameters, and a code that is
 // unpacked once serves all of them. Sums, references and the l terms are fp32; p s' is rounded to fp16 (relative 2^-11, of terms
-// that count from the middle of the codes), queries are exact in fp16 over 27 binades.
+// that count from the middle of the codes, or 2^-24 of s' and the row's largest p: see kLeast), queries are of a power of two for each
+// row.
 //
 // A block computes with most of its warps, each 32 tokens of a unit at a time, and copies with the rest through a ring of stages
 // on barriers (bulk copies of a page's run at a time; every wait is bounded). The units of all sequences, heads and row tiles
@@ -1004,8 +1019,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         float2 lows[kGroups][NT] = {}, ceiling[NT], minus_peak[NT] = {}, sum[NT] = {};
 #pragma unroll
         for (uint32_t n = 0; n < NT; ++n) ceiling[n] = make_float2(-INFINITY, -INFINITY);
-        int32_t top = 0;  // biased exponent of the largest value scale so far
-        float fit = power_of_two(254), limit = 0x1p-126f;  // limit: the least scale that would raise top
+        float fit[kGroups] = {};  // 0 before the group's first scale
 
         // Rows of S^T: the tokens of fragment rows 2c and 2c + 1 are 2c and 2c + 1, in this order for c < 2 and in the other
         // for the rest, so that neither the keys' loads (both rows at once) nor the values' (one of each c) crowd the same banks.
@@ -1031,12 +1045,15 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                                    (args.window && extent.token(place + 31) >= args.sinks &&
                                     extent.token(place) <= extent.length - 1 - args.window);
 
-            float widest = 0.0f;  // of the value scales, lane = token
+            bool grows = false;
             {
-                uint32_t pairs[kGroups];
+                uint32_t pairs[kGroups];  // lane = token
                 load_words(pairs, value_params + lane * (kGroups * 4));
 #pragma unroll
-                for (uint32_t g = 0; g < kGroups; ++g) widest = fmaxf(widest, fabsf(E::low(pairs[g])));
+                for (uint32_t g = 0; g < kGroups; ++g) {
+                    const float fitted = fabsf(E::low(pairs[g])) * fit[g];
+                    grows |= !(fitted >= kLeast && fitted < kMost);
+                }
             }
 
             // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
@@ -1104,9 +1121,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 
             // ---- what rarely happens, all in one place: tokens that some row may not see; a score more than kSlack above its
             // row's reference, the score that its exponentials are taken from (so that weights stay under 2^kSlack); a
-            // value scale over the largest so far, which fixes the power of two that lets weight * scale fit fp16.
+            // value scale outside its group's window.
             float2 largest[NT];
-            bool grows = widest >= limit;
             const auto look = [&]() {
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
@@ -1118,7 +1134,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             for (uint32_t n = 0; n < NT; ++n) grows |= largest[n].x > ceiling[n].x || largest[n].y > ceiling[n].y;
             if (is_masked || __any_sync(0xffffffffu, grows)) {
                 if (is_masked) {
-                    uint32_t real = here >= 32 ? 0xffffffffu : here <= 0 ? 0u : (1u << here) - 1;
+                    const int32_t own = extent.token(place + static_cast<int32_t>(lane));
+                    uint32_t real = __ballot_sync(0xffffffffu, static_cast<int32_t>(lane) < here &&
+                                                                   (!args.window || own >= extent.start || own < args.sinks));
                     if (bad_pages[stage])
                         real &= __ballot_sync(0xffffffffu, static_cast<int32_t>(lane) < here && page_at(place + lane) < args.pages);
 #pragma unroll
@@ -1136,14 +1154,14 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             }
                         }
                     // Values that are not finite make NaN of the groups of the rows that see them, and of no others: a
-                    // weight of zero would make NaN of them too.
+                    // weight of zero would make NaN of them too. What no row sees is none at all.
                     uint32_t pairs[kGroups];
                     load_words(pairs, value_params + lane * (kGroups * 4));
                     bool finite = true;
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; ++g) {
                         if (!(real >> lane & 1u)) pairs[g] = 0;
-                        finite = finite && E::finite(pairs[g]);
+                        finite = finite && usable_params<BF16>(pairs[g]);
                     }
                     if (!__all_sync(0xffffffffu, finite)) {
 #pragma unroll
@@ -1152,42 +1170,22 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                             for (uint32_t k = 0; k < 4; ++k) {
                                 const uint32_t its = 8 * k + own_token;
                                 const uint32_t pair = reinterpret_cast<const uint32_t*>(value_params)[its * kGroups + g];
-                                if ((real >> its & 1u) && !E::finite(pair))
+                                if ((real >> its & 1u) && !usable_params<BF16>(pair))
 #pragma unroll
                                     for (uint32_t n = 0; n < NT; ++n) {
                                         if (x[k / 2][n][k % 2].x != -INFINITY) lows[g][n].x = __uint_as_float(0x7fffffffu);
                                         if (x[k / 2][n][k % 2].y != -INFINITY) lows[g][n].y = __uint_as_float(0x7fffffffu);
                                     }
                             }
-                            if (!E::finite(pairs[g])) pairs[g] = 0;
+                            if (!usable_params<BF16>(pairs[g])) pairs[g] = 0;
                         }
                     }
                     __syncwarp();
-                    widest = 0.0f;
 #pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g) {
-                        reinterpret_cast<uint32_t*>(value_params)[lane * kGroups + g] = pairs[g];
-                        widest = fmaxf(widest, fabsf(E::low(pairs[g])));
-                    }
+                    for (uint32_t g = 0; g < kGroups; ++g) reinterpret_cast<uint32_t*>(value_params)[lane * kGroups + g] = pairs[g];
                     fence_proxy_async_shared();  // what is copied there next comes by another way than these stores
                     __syncwarp();
                     look();
-                }
-                if (!(widest < INFINITY)) {  // an infinity says nothing about the others
-                    uint32_t pairs[kGroups];
-                    load_words(pairs, value_params + lane * (kGroups * 4));
-                    widest = 0.0f;
-#pragma unroll
-                    for (uint32_t g = 0; g < kGroups; ++g)
-                        if (E::finite(pairs[g])) widest = fmaxf(widest, fabsf(E::low(pairs[g])));
-                }
-                const int32_t unit_top = static_cast<int32_t>(__reduce_max_sync(0xffffffffu, __float_as_uint(widest)) >> 23);
-                float shrink = 1.0f;
-                if (unit_top > top) {
-                    shrink = power_of_two(max(127 + min(kFitBiased - unit_top, 254) - min(kFitBiased - top, 254), 0));
-                    top = unit_top;
-                    fit = power_of_two(min(kFitBiased - top, 254));
-                    limit = power_of_two(top + 1);
                 }
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n) {
@@ -1215,10 +1213,88 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     for (uint32_t g = 0; g < kGroups; ++g) lows[g][n] = __fmul2_rn(lows[g][n], keep2);
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i) {
-                        const float factor = keep[i % 2] * shrink;
 #pragma unroll
-                        for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= factor;
+                        for (uint32_t j = 0; j < kTiles; ++j) out[j][n][i] *= keep[i % 2];
                     }
+                }
+                // ---- scales outside their group's window: it is moved if they are many, and what still lies outside is
+                // multiplied here, in fp32, by the weights as they are (so that a scale has no say in rows that do not see its token), and
+                // counts as zero below.
+                uint32_t pairs[kGroups];
+                load_words(pairs, value_params + lane * (kGroups * 4));
+                bool any_far = false;
+#pragma unroll
+                for (uint32_t g = 0; g < kGroups; ++g) {
+                    constexpr uint32_t kGroupTiles = G / 16;
+                    const float size = fabsf(E::low(pairs[g]));
+                    const bool counts = size > 0.0f && usable_params<BF16>(pairs[g]);  // (Others that a row sees make NaN of it.)
+                    const auto lie_far = [&]() {
+                        const float fitted = size * fit[g];
+                        return __ballot_sync(0xffffffffu, counts && !(fitted >= kLeast && fitted < kMost));
+                    };
+                    uint32_t far = lie_far();
+                    if (far == 0) continue;
+                    const int32_t was = __float_as_int(fit[g]) >> 23;
+                    if (was == 0 || __popc(far) >= kManyFar || __any_sync(0xffffffffu, counts && size * fit[g] >= 0x1p87f)) {
+                        const uint32_t exponent = counts ? max(__float_as_uint(size) >> 23, 1u) : 0u;
+                        const uint32_t together = __reduce_add_sync(0xffffffffu, exponent), all = __popc(__ballot_sync(0xffffffffu, counts));
+                        const int32_t middle = max(static_cast<int32_t>((2 * together + all) / (2 * all)),
+                                                   static_cast<int32_t>(__reduce_max_sync(0xffffffffu, exponent)) - kFarthest);
+                        int32_t power = min(kFitBiased - middle, kMostFit);
+                        if (was) {
+                            float most = 0.0f;  // of the sums so far, which a window further down would raise: to 2^100 at most
+#pragma unroll
+                            for (uint32_t j = g * kGroupTiles; j < (g + 1) * kGroupTiles; ++j)
+#pragma unroll
+                                for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (uint32_t i = 0; i < 4; ++i) most = fmaxf(most, fabsf(out[j][n][i]));
+                            const int32_t room = 227 - static_cast<int32_t>(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
+                            power = min(power, was + max(room, 0));
+                            const float factor = power_of_two(min(max(127 + power - was, 0), 254));
+#pragma unroll
+                            for (uint32_t j = g * kGroupTiles; j < (g + 1) * kGroupTiles; ++j)
+#pragma unroll
+                                for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (uint32_t i = 0; i < 4; ++i) out[j][n][i] *= factor;
+                        }
+                        fit[g] = power_of_two(power);
+                        far = lie_far();
+                    }
+#pragma unroll 1
+                    for (uint32_t left = far; left; left &= left - 1) {
+                        const uint32_t its = __ffs(left) - 1, pair = __shfl_sync(0xffffffffu, pairs[g], its);
+                        const uint32_t holder = (its & 7u) ^ ((its & 7u) >> 2);  // its scores lie in lanes (holder, c4)
+                        const float low = fmaf(8.0f, E::low(pair), E::high(pair)), fitted = E::low(pair) * fit[g];
+                        uint32_t words[kValueWords];
+                        load_words(words, values + its * (D / 2) + l4 * (D / 16));
+#pragma unroll
+                        for (uint32_t n = 0; n < NT; ++n) {
+                            const float2 first = its & 8u ? x[0][n][1] : x[0][n][0], last = its & 8u ? x[1][n][1] : x[1][n][0];
+                            const float2 power = __ffma2_rn(its & 16u ? last : first, to_log2[n], minus_peak[n]);
+                            const float2 p = make_float2(__shfl_sync(0xffffffffu, ex2_approx(power.x), 4 * holder + c4),
+                                                         __shfl_sync(0xffffffffu, ex2_approx(power.y), 4 * holder + c4));
+                            if (l4 == holder) lows[g][n] = __ffma2_rn(p, make_float2(low, low), lows[g][n]);
+                            const float2 weight = __fmul2_rn(p, make_float2(fitted, fitted));
+#pragma unroll
+                            for (uint32_t j = g * kGroupTiles; j < (g + 1) * kGroupTiles; ++j) {
+                                const uint32_t byte = words[j / 4] >> (8 * (j % 4));
+                                const float even = static_cast<float>(static_cast<int32_t>(byte & 15u) - 8);
+                                const float odd = 16.0f * static_cast<float>(static_cast<int32_t>(byte >> 4 & 15u) - 8);
+                                out[j][n][0] = fmaf(even, weight.x, out[j][n][0]);
+                                out[j][n][1] = fmaf(even, weight.y, out[j][n][1]);
+                                out[j][n][2] = fmaf(odd, weight.x, out[j][n][2]);
+                                out[j][n][3] = fmaf(odd, weight.y, out[j][n][3]);
+                            }
+                        }
+                    }
+                    if (far >> lane & 1u) reinterpret_cast<uint32_t*>(value_params)[lane * kGroups + g] = 0;
+                    any_far |= far != 0;
+                }
+                if (any_far) {
+                    fence_proxy_async_shared();
+                    __syncwarp();
                 }
             }
 
@@ -1239,7 +1315,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
                     }
 #pragma unroll
                     for (uint32_t g = 0; g < kGroups; ++g) {
-                        const float scale = E::low(pairs[g]), fitted = scale * fit, low = fmaf(8.0f, scale, E::high(pairs[g]));
+                        const float scale = E::low(pairs[g]), fitted = scale * fit[g], low = fmaf(8.0f, scale, E::high(pairs[g]));
 #pragma unroll
                         for (uint32_t n = 0; n < NT; ++n) {
                             lows[g][n].x = fmaf(p[n].x, low, lows[g][n].x);
@@ -1302,7 +1378,9 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         {
             float* const merged = reinterpret_cast<float*>(merge_memory + warp * merge_pitch);
             float* const stats = merged + kRows * kPitch;
-            const float unfit = power_of_two(254 - min(kFitBiased - top, 254));
+            float unfit[kGroups];
+#pragma unroll
+            for (uint32_t g = 0; g < kGroups; ++g) unfit[g] = power_of_two(254 - (__float_as_int(fit[g]) >> 23));
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
@@ -1321,8 +1399,8 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
 #pragma unroll
                     for (uint32_t j = 0; j < kTiles; ++j) {
                         const uint32_t g = 16 * j / G;
-                        merged[row * kPitch + 16 * j + l4] = fmaf(out[j][n][e], unfit, low[g]);
-                        merged[row * kPitch + 16 * j + 8 + l4] = fmaf(out[j][n][2 + e] * 0.0625f, unfit, low[g]);
+                        merged[row * kPitch + 16 * j + l4] = fmaf(out[j][n][e], unfit[g], low[g]);
+                        merged[row * kPitch + 16 * j + 8 + l4] = fmaf(out[j][n][2 + e] * 0.0625f, unfit[g], low[g]);
                     }
                     if (l4 == 0) {
                         stats[2 * row] = (e ? ceiling[n].y : ceiling[n].x) == -INFINITY ? -INFINITY : -(e ? minus_peak[n].y : minus_peak[n].x);

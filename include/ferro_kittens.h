@@ -412,8 +412,11 @@ int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_str
  * see may hold anything, NaN included. `scale` is finite, of either sign; a row's queries are scaled by a power of two of their
  * own, so that its result does not depend on the sizes of other rows' (one whose largest query times `scale` passes 2^115 is outside
  * what its fp32 scores hold).
- * Scores, softmax statistics and sums are fp32; a weight times its group's scale is rounded to fp16 (11 bits,
- * scaled so that the range always fits) for the product with the value codes, which are exact.
+ * Scores, softmax statistics and sums are fp32; a weight times its group's scale is rounded to fp16 for the product with the value
+ * codes, which are exact: by 2^-11 of itself, or 2^-24 of that scale times the row's largest weight, if that is more. That holds for
+ * scales however far apart: each group of channels is followed by itself, and tokens whose scale is some 20 times off the group's others
+ * are multiplied in fp32, which takes longer. (Parameters that no written row has, whose low + 8 * scale is not finite, may make NaN of the
+ * rows that see them.)
  * `workspace` is fk_cache_attention_workspace_bytes(sm_count) bytes, 16-byte aligned, ALL ZERO before its first
  * use; every call leaves its counters zero again, so it is cleared once (and after a reported stall). Calls that share a workspace must not
  * overlap on the device (two streams, or two captured graphs that may run together, want one each). */
