@@ -1580,6 +1580,51 @@ static int check_cache(const fk_cache_t* cache) {
     return FK_OK;
 }
 
+/// A tensor [tokens, heads, dim] of rows of `dim` neighbouring elements; strides in elements.
+struct Rows {
+    uintptr_t base;
+    int64_t token_stride, head_stride;
+    uint64_t tokens, heads;
+    int64_t dim;
+
+    /// The elements from the first row's begin that the rows lie in: [least, most).
+    __int128 least() const { return reach(std::min<int64_t>(token_stride, 0), std::min<int64_t>(head_stride, 0)); }
+    __int128 most() const { return reach(std::max<int64_t>(token_stride, 0), std::max<int64_t>(head_stride, 0)) + dim; }
+    __int128 reach(int64_t token, int64_t head) const {
+        return static_cast<__int128>(token) * (tokens - 1) + static_cast<__int128>(head) * (heads - 1);
+    }
+    /// Whether two rows `offset` elements and some whole strides apart (but not a row and itself) share an element.
+    bool meet(__int128 offset) const {
+        const bool by_token = tokens >= heads;  // steps of the other are gone through one by one
+        const __int128 a = by_token ? token_stride : head_stride, b = by_token ? head_stride : token_stride;
+        const __int128 a_count = by_token ? tokens : heads, b_count = by_token ? heads : tokens;
+        for (__int128 j = 1 - b_count; j < b_count; ++j) {
+            const __int128 rest = offset + j * b;  // the row nearest to -rest, by whole strides a, and its neighbours
+            const __int128 near = a ? -rest / a : 0;
+            for (__int128 i : {near - 1, near, near + 1}) {
+                if (i <= -a_count || i >= a_count || (offset == 0 && i == 0 && j == 0)) continue;
+                const __int128 apart = rest + i * a;
+                if (apart < dim && apart > -dim) return true;
+            }
+        }
+        return false;
+    }
+    bool over_one_another() const {
+        const uint64_t token = std::abs(token_stride), head = std::abs(head_stride);
+        const unsigned __int128 token_span = static_cast<unsigned __int128>(token) * (tokens - 1) + dim;
+        const unsigned __int128 head_span = static_cast<unsigned __int128>(head) * (heads - 1) + dim;
+        if ((heads == 1 || head >= static_cast<uint64_t>(dim)) && (tokens == 1 || token >= head_span)) return false;
+        if ((tokens == 1 || token >= static_cast<uint64_t>(dim)) && (heads == 1 || head >= token_span)) return false;
+        return meet(0);
+    }
+    /// Whether a row of `other` shares an element with one of these, as far as equal strides or begins tell.
+    bool over(const Rows& other) const {
+        const __int128 offset = (static_cast<__int128>(other.base) - static_cast<__int128>(base)) / 2;
+        if (offset + other.least() >= most() || least() >= offset + other.most()) return false;
+        return offset == 0 || (token_stride == other.token_stride && head_stride == other.head_stride && meet(offset));
+    }
+};
+
 /// `call(D, G, BF16)` with the cache's sizes and type as compile-time constants.
 template <typename Call>
 static int for_cache(const fk_cache_t* cache, Call call) {
@@ -1616,13 +1661,18 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
         if (stride % 8)
             return fk_fail(FK_ERR_ALIGNMENT, "a stride of %lld elements is no multiple of 8: rows move 16 bytes at a time",
                            static_cast<long long>(stride));
-    if (!write)
-        for (uint32_t i = 0; i < 4; ++i)
-            if ((i % 2 ? cache->kv_heads : tokens) > 1 && std::abs(strides[i]) < cache->head_dim)
-                return fk_fail(FK_ERR_SHAPE, "a stride of %lld elements lays rows of %u over one another",
-                               static_cast<long long>(strides[i]), cache->head_dim);
     if (static_cast<uint64_t>(tokens) * cache->kv_heads >= (1ull << 31))
         return fk_fail(FK_ERR_SHAPE, "%u tokens x %u heads is more than 2^31 - 1 rows", tokens, cache->kv_heads);
+    if (!write) {
+        const int64_t dim = cache->head_dim;
+        const Rows both[2] = {{reinterpret_cast<uintptr_t>(k), k_token_stride, k_head_stride, tokens, cache->kv_heads, dim},
+                              {reinterpret_cast<uintptr_t>(v), v_token_stride, v_head_stride, tokens, cache->kv_heads, dim}};
+        for (const Rows& rows : both)
+            if (rows.over_one_another())
+                return fk_fail(FK_ERR_SHAPE, "strides of %lld elements a token and %lld a head lay rows of %u over one another",
+                               static_cast<long long>(rows.token_stride), static_cast<long long>(rows.head_stride), cache->head_dim);
+        if (both[0].over(both[1])) return fk_fail(FK_ERR_INVALID, "keys and values read would lie over one another");
+    }
     DeviceFacts facts;
     const int known = device_facts(&facts);
     if (known != FK_OK) return known;

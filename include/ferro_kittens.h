@@ -392,7 +392,7 @@ int fk_cache_write(const fk_cache_t* cache, const void* k, const void* v, int64_
 
 /* Read rows back: k[i, head, :] and v[i, head, :] become the values of slot slots[i] (which may repeat), rounded
  * once to the cache's type. Rows of negative slots are left as they were, or zeroed with `clear_skipped`.
- * Rows may not lie over one another: strides of more than one token or head are head_dim or more. */
+ * Rows may not lie over one another, those of k over those of v neither. */
 int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_stride, int64_t k_head_stride,
                   int64_t v_token_stride, int64_t v_head_stride, const void* slots, uint32_t slot_bytes,
                   uint32_t tokens, int clear_skipped, void* stream, uint32_t* device_status);

@@ -80,6 +80,34 @@ def test_rows_read_over_one_another_are_refused(strides):
     assert _read(_cache(), strides=strides) == FK_ERR_SHAPE and "over one another" in last_error()
 
 
+@pytest.mark.parametrize("strides", [(128, 128, 256, 128), (256, 128, 128, 128), (256, 128, 192, 128), (256, 128, -128, 128),
+                                     (256, 128, 136, 256), (384, 256, 1 << 62, 64), (256, 128, 256, 256), (256, 128, 0, 128)])
+def test_strides_that_only_together_lay_rows_over_one_another_are_refused(strides):
+    """Tokens and heads each a row or more apart, but one token's last head on another token's first."""
+    assert _read(_cache(), strides=strides, v=BASE + (1 << 30), tokens=5) == FK_ERR_SHAPE and "over one another" in last_error()
+
+
+@pytest.mark.parametrize("heads,tokens", [(1, 4), (2, 3), (3, 5), (5, 2)])
+def test_rows_apart_are_told_from_rows_that_meet(heads, tokens):
+    """Every pair of strides up to some rows, against the elements themselves; what is let through fails for want of a device, or
+    (as keys over values) on purpose."""
+    for token in range(-640, 641, 64):
+        for head in range(-640, 641, 64):
+            firsts = sorted(token * t + head * h for t in range(tokens) for h in range(heads))
+            apart = all(y - x >= 64 for x, y in zip(firsts, firsts[1:]))
+            # Values elsewhere meet nothing; the keys' own place is refused in other words.
+            code = _read(_cache(head_dim=64, kv_heads=heads), strides=(token, head, token, head), tokens=tokens)
+            assert code == (FK_ERR_INVALID if apart else FK_ERR_SHAPE), (token, head)
+            assert "over one another" in last_error()
+
+
+@pytest.mark.parametrize("offset,strides", [(0, (256, 128, 256, 128)), (0, (256, 128, 512, 128)), (256, (256, 128, 256, 128)),
+                                            (16, (512, 128, 512, 128)), (-512, (256, 128, 256, 128)), (2 * 1024, (512, 256, 512, 256))])
+def test_keys_read_over_values_are_refused(offset, strides):
+    assert _read(_cache(), v=BASE + offset, strides=strides, tokens=5) == FK_ERR_INVALID
+    assert "keys and values" in last_error()
+
+
 @pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
 def test_scales_that_are_not_finite_are_refused(scale):
     assert _attend(_cache(), scale=scale) == FK_ERR_INVALID and "not finite" in last_error()
