@@ -1770,6 +1770,26 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     return FK_OK;
 }
 
+/// Whether a row of the queries (strides in elements of 2 bytes) lies in part in [begin, end).
+static bool queries_meet(const void* q, const int64_t (&strides)[3], uint32_t batch, uint32_t queries, uint32_t heads, uint32_t dim,
+                         uintptr_t begin, uintptr_t end) {
+    const uint64_t counts[3] = {batch, queries, heads};
+    const __int128 base = reinterpret_cast<uintptr_t>(q);
+    __int128 least = base, most = base + 2 * dim;
+    for (uint32_t i = 0; i < 3; ++i)
+        (strides[i] < 0 ? least : most) += static_cast<__int128>(2 * (counts[i] - 1)) * strides[i];
+    if (most <= begin || least >= end) return false;
+    // Rows with gaps that the other may lie in: one by one, which calls hardly ever come to.
+    for (uint32_t b = 0; b < batch; ++b)
+        for (uint32_t t = 0; t < queries; ++t)
+            for (uint32_t h = 0; h < heads; ++h) {
+                const __int128 row = base + 2 * (static_cast<__int128>(strides[0]) * b + static_cast<__int128>(strides[1]) * t +
+                                                 static_cast<__int128>(strides[2]) * h);
+                if (row < end && row + 2 * dim > begin) return true;
+            }
+    return false;
+}
+
 extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_t q_batch_stride,
                                   int64_t q_token_stride, int64_t q_head_stride, void* out, float* lse,
                                   const int32_t* lengths, const int32_t* table, int64_t table_stride,
@@ -1782,7 +1802,6 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
         return fk_fail(FK_ERR_SHAPE, "%u query heads do not divide over %u kv heads", heads, cache->kv_heads);
     if (batch == 0 || queries == 0) return FK_OK;
     if (!q || !out || !lengths || !workspace) return fk_fail(FK_ERR_INVALID, "an operand pointer is null");
-    if (q == out) return fk_fail(FK_ERR_INVALID, "the output may not lie over the queries");
     if (!std::isfinite(scale)) return fk_fail(FK_ERR_INVALID, "the score scale %f is not finite", scale);
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15u)
         return fk_fail(FK_ERR_ALIGNMENT, "queries, output and workspace must be 16-byte aligned");
@@ -1802,6 +1821,19 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
     if (capacity >= 0x7ffff000ull)
         return fk_fail(FK_ERR_SHAPE, "%u pages of %u tokens are more than 2^31 - 1 tokens a sequence", columns,
                        cache->page_size);
+    const uint64_t rows = static_cast<uint64_t>(queries) * (heads / cache->kv_heads);
+    const unsigned __int128 all_rows = static_cast<unsigned __int128>(rows) * cache->kv_heads * batch;
+    if (rows >= (1ull << 30) || all_rows >= (1ull << 32))
+        return fk_fail(FK_ERR_SHAPE, "%u sequences of %u queries of %u heads are more rows than a launch counts", batch, queries, heads);
+    const uint64_t asked = static_cast<uint64_t>(all_rows);
+    const uintptr_t out_end = reinterpret_cast<uintptr_t>(out) + 2 * asked * cache->head_dim;
+    const uintptr_t lse_begin = reinterpret_cast<uintptr_t>(lse), lse_end = lse_begin + 4 * asked;
+    if (queries_meet(q, strides, batch, queries, heads, cache->head_dim, reinterpret_cast<uintptr_t>(out), out_end))
+        return fk_fail(FK_ERR_INVALID, "the output may not lie over the queries");
+    if (lse && lse_begin < out_end && reinterpret_cast<uintptr_t>(out) < lse_end)
+        return fk_fail(FK_ERR_INVALID, "lse may not lie over the output");
+    if (lse && queries_meet(q, strides, batch, queries, heads, cache->head_dim, lse_begin, lse_end))
+        return fk_fail(FK_ERR_INVALID, "lse may not lie over the queries");
     DeviceFacts facts;
     const int known = device_facts(&facts);
     if (known != FK_OK) return known;
@@ -1809,9 +1841,6 @@ extern "C" int fk_cache_attention(const fk_cache_t* cache, const void* q, int64_
         return fk_fail(FK_ERR_SHAPE, "a workspace of %llu bytes is under the %llu of this device",
                        static_cast<unsigned long long>(workspace_bytes),
                        static_cast<unsigned long long>(fk_cache_attention_workspace_bytes(facts.sm_count)));
-    const uint64_t rows = static_cast<uint64_t>(queries) * (heads / cache->kv_heads);
-    if (rows >= (1ull << 30))
-        return fk_fail(FK_ERR_SHAPE, "%u queries of %u heads are more rows than a launch counts", queries, heads);
     cache::AttentionArguments args;
     args.codes[0] = static_cast<const uint8_t*>(cache->k_codes);
     args.codes[1] = static_cast<const uint8_t*>(cache->v_codes);

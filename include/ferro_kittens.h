@@ -400,8 +400,8 @@ int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_str
 /* Attention of each sequence's newest tokens over its rows of the cache, theirs included.
  *   q        [batch, queries, heads, head_dim], strides in elements, multiples of 8; heads is a multiple of
  *            kv_heads, and query head h reads kv head h / (heads / kv_heads)
- *   out      packed [batch, queries, heads, head_dim] of the cache's type, not over q; lse null or packed
- *            [batch, queries, heads] fp32 (natural log)
+ *   out      packed [batch, queries, heads, head_dim] of the cache's type; lse null or packed [batch, queries, heads]
+ *            fp32 (natural log); neither over a row of q or over the other
  *   lengths  [batch] int32: tokens of each sequence, its `queries` newest among them; 0 or less is an empty
  *            sequence, and one shorter than `queries` has its first rows before its first token
  *   table    row b (of table_pages entries, table_stride apart) names sequence b's pages in order; entries behind its

@@ -22,3 +22,26 @@ def test_keys_and_values_read_side_by_side(device):
         assert torch.equal(k, want[0]) and torch.equal(v, want[1])
     with pytest.raises(FerroKittensError, match="keys and values"):
         kv_cache.read(cache, slots, k, k)
+
+
+def test_an_output_between_the_queries_of_a_projection(device):
+    """Of [queries, keys, values] side by side, one sequence: the output may take the keys' place, and not a part of the queries'."""
+    cache = kv_cache.new(2, 64, 2, device=device)
+    slots = torch.arange(90, device=device)
+    kv_cache.write(cache, *(torch.randn(90, 2, 128, device=device).bfloat16() for _ in range(2)), slots)
+    lengths, table = torch.tensor([90], dtype=torch.int32, device=device), torch.tensor([[0, 1]], dtype=torch.int32, device=device)
+    wide = torch.randn(1, 1, 12, 128, device=device).bfloat16()
+    q = wide[:, :, :4]
+    want, _ = kv_cache.attend(q, cache, lengths, table)
+    got, _ = kv_cache.attend(q, cache, lengths, table, out=wide[:, :, 4:8])
+    assert got.data_ptr() == wide[:, :, 4:8].data_ptr() and torch.equal(got, want)
+    for begin in (0, 1, 3):
+        with pytest.raises(FerroKittensError, match="over the queries"):
+            kv_cache.attend(q, cache, lengths, table, out=wide[:, :, begin:begin + 4])
+    # Two sequences whose queries lie far apart: the output fits in the gap.
+    lengths, table = torch.tensor([90, 33], dtype=torch.int32, device=device), table.expand(2, 2).contiguous()
+    far = torch.randn(2, 5, 4, 128, device=device).bfloat16()
+    q = far[:, :1]
+    want, _ = kv_cache.attend(q, cache, lengths, table)
+    got, _ = kv_cache.attend(q, cache, lengths, table, out=far[0, 2:4].unsqueeze(1))
+    assert torch.equal(got, want)

@@ -108,6 +108,24 @@ def test_keys_read_over_values_are_refused(offset, strides):
     assert "keys and values" in last_error()
 
 
+@pytest.mark.parametrize("changed,word", [
+    ({"out": BASE + 16}, "output may not lie over the queries"), ({"out": BASE + 3 * 2048 - 16}, "output may not lie over the queries"),
+    ({"out": BASE - 3 * 2048 + 16}, "output may not lie over the queries"),
+    ({"out": BASE, "strides": (4096, 1024, 128)}, "output may not lie over the queries"),
+    ({"out": BASE + 3 * 2048, "strides": (-1024, 1024, 128), "q": BASE + 6 * 2048}, "output may not lie over the queries"),
+    ({"lse": BASE + 64}, "lse may not lie over the queries"), ({"lse": BASE + 3 * 2048 - 4}, "lse may not lie over the queries"),
+    ({"lse": BASE + (1 << 20) + 16}, "lse may not lie over the output"), ({"lse": BASE + (1 << 20) - 4}, "lse may not lie over the output")])
+def test_outputs_that_begin_inside_something_are_refused(changed, word):
+    """Three sequences of one query, 8 heads of 128: 2048 bytes each."""
+    assert _attend(_cache(), **changed) == FK_ERR_INVALID
+    assert word in last_error()
+
+
+@pytest.mark.parametrize("sizes", [{"queries": 1 << 28}, {"batch": 1 << 20, "queries": 1 << 12}, {"batch": 0xffffffff, "queries": 0xffffffff}])
+def test_more_rows_than_memory_holds_are_refused(sizes):
+    assert _attend(_cache(), **sizes) == FK_ERR_SHAPE and "more rows" in last_error()
+
+
 @pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
 def test_scales_that_are_not_finite_are_refused(scale):
     assert _attend(_cache(), scale=scale) == FK_ERR_INVALID and "not finite" in last_error()
