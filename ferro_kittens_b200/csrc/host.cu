@@ -470,7 +470,8 @@ extern "C" int fk_status_check(const uint32_t* device_status, void* stream) {
     if (words[0] == 0) return FK_OK;
     // The cache kernels note an index they had to skip, not a stall.
     if (words[0] == 0x501)
-        return fk_fail(FK_ERR_INVALID, "slot %u of token %u lies outside the cache", words[3], words[2]);
+        return fk_fail(FK_ERR_INVALID, "slot %llu of token %u lies outside the cache",
+                       static_cast<unsigned long long>(words[1]) << 32 | words[3], words[2]);
     if (words[0] == 0x502)
         return fk_fail(FK_ERR_INVALID, "page %u in the table of sequence %u lies outside the cache", words[3], words[2]);
     if (words[0] == 0x503)

@@ -26,12 +26,12 @@ enum NoteCode : uint32_t {
 
 /// Everything before this launch on its stream is done and seen (see `launch`).
 __device__ __forceinline__ void wait_for_earlier_launches() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-/// The first bad index of a launch goes into the caller's status words.
-__device__ __forceinline__ void note(uint32_t* status, uint32_t code, uint32_t where, uint32_t value) {
+/// The first bad index of a launch goes into the caller's status words: code, its upper half, where it stands, its lower half.
+__device__ __forceinline__ void note(uint32_t* status, uint32_t code, uint32_t where, uint64_t value) {
     if (status && atomicCAS(status, 0u, code) == 0u) {
-        status[1] = blockIdx.x;
+        status[1] = static_cast<uint32_t>(value >> 32);
         status[2] = where;
-        status[3] = value;
+        status[3] = static_cast<uint32_t>(value);
     }
 }
 
@@ -175,7 +175,7 @@ struct RowArguments {
     int64_t token_stride[2], head_stride[2];  // bytes
     const void* slots;
     uint32_t slots_wide;
-    uint32_t tokens, rows;  // rows = tokens * kv_heads
+    uint32_t rows;          // tokens * kv_heads
     uint64_t capacity;      // pages * page_size
     uint32_t page_size;
     Divider heads, page;
@@ -189,7 +189,7 @@ __device__ __forceinline__ bool cache_row(const RowArguments& args, uint32_t tok
                                          : static_cast<const int32_t*>(args.slots)[token];
     if (slot < 0) return false;
     if (static_cast<uint64_t>(slot) >= args.capacity) {
-        note(status, kBadSlot, token, static_cast<uint32_t>(slot));
+        note(status, kBadSlot, token, static_cast<uint64_t>(slot));
         return false;
     }
     const uint32_t page = args.page.quotient(static_cast<uint32_t>(slot));
@@ -1689,7 +1689,6 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
     args.head_stride[1] = 2 * v_head_stride;
     args.slots = slots;
     args.slots_wide = slot_bytes == 8;
-    args.tokens = tokens;
     args.rows = tokens * cache->kv_heads;
     args.capacity = static_cast<uint64_t>(cache->pages) * cache->page_size;
     args.page_size = cache->page_size;

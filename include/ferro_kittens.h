@@ -452,7 +452,7 @@ int fk_selftest_call_guard(int device, uint32_t hold_ms, uint64_t* entered_ns, u
 
 /* Read a kernel's 4 status words back (waiting on `stream` under the launch
  * deadline) and, when the first is non-zero, return FK_ERR_DEVICE_STALL with the role, block, stage and
- * parity in fk_last_error(). */
+ * parity in fk_last_error(), or FK_ERR_INVALID with an index that a cache kernel had to skip. */
 int fk_status_check(const uint32_t* device_status, void* stream);
 
 /* `Semaphore::wait_before(parity, ticks)` giving up (src/sync.rs:214-245), as a self-test: launches

@@ -3,7 +3,7 @@ that the device's size and the number of segments choose."""
 import pytest
 import torch
 
-from ferro_kittens_b200 import FerroKittensError, kv_cache
+from ferro_kittens_b200 import FerroKittensError, gemm, kv_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,15 @@ def test_an_output_between_the_queries_of_a_projection(device):
     want, _ = kv_cache.attend(q, cache, lengths, table)
     got, _ = kv_cache.attend(q, cache, lengths, table, out=far[0, 2:4].unsqueeze(1))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("slot,wide", [(1 << 40, True), ((7 << 32) + 3, True), ((1 << 63) - 1, True), (16, True), (16, False), ((1 << 31) - 1, False)])
+def test_a_bad_slot_is_reported_whole(device, slot, wide):
+    cache = kv_cache.new(2, 8, 1, device=device)
+    x = torch.randn(2, 1, 128, device=device).bfloat16()
+    slots = torch.tensor([3, slot], dtype=torch.int64 if wide else torch.int32, device=device)
+    for call in (lambda status: kv_cache.write(cache, x, x, slots, status), lambda status: kv_cache.read(cache, slots, status=status)):
+        status = gemm.new_status(device)
+        call(status)
+        with pytest.raises(FerroKittensError, match=f"slot {slot} of token 1 lies outside the cache"):
+            gemm.check_status(status)
