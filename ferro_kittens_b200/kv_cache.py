@@ -114,16 +114,27 @@ def _require_indices(name: str, tensor: torch.Tensor, cache: Cache, count: int |
                          + (f" of {count} entries" if count is not None else ""))
 
 
+def _status_words(status: torch.Tensor | None, device: torch.device) -> int | None:
+    """The address of a call's status words, which the kernels write where they find them."""
+    if status is None:
+        return None
+    if status.device != device:
+        raise RuntimeError(f"status must live on the cache's device {device}: its kernels write it")
+    if status.dtype is not torch.int32 or not status.is_contiguous() or status.numel() < 4:
+        raise ValueError("status must be a contiguous int32 tensor of 4 words or more (gemm.new_status makes one)")
+    return status.data_ptr()
+
+
 def _rows(entry, cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, status, *more) -> None:
     tokens = slots.shape[0]
     for name, tensor in (("k", k), ("v", v)):
         _require(name, tensor, cache, 3)
         if tensor.shape[1] != cache.kv_heads or tensor.shape[0] != tokens:
             raise ValueError(f"{name} must hold {tokens} tokens of {cache.kv_heads} heads, one token a slot")
-    k_strides, v_strides = k.stride(), v.stride()
+    k_strides, v_strides, words = k.stride(), v.stride(), _status_words(status, cache.device)
     _on(cache.device, lambda stream: entry(
         cache.view, k.data_ptr(), v.data_ptr(), k_strides[0], k_strides[1], v_strides[0], v_strides[1], slots.data_ptr(),
-        4 if slots.dtype is torch.int32 else 8, tokens, *more, stream, status.data_ptr() if status is not None else None))
+        4 if slots.dtype is torch.int32 else 8, tokens, *more, stream, words))
 
 
 def write(cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, status: torch.Tensor | None = None) -> None:
@@ -197,11 +208,11 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
         if out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and of q's shape")
     lse = lengths.new_empty(shape[:3], dtype=torch.float32)
-    strides = q.stride()
+    strides, words = q.stride(), _status_words(status, cache.device)
     _on(cache.device, lambda stream: library().fk_cache_attention(
         cache.view, q.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(), lse.data_ptr(),
         lengths.data_ptr(), table.data_ptr() if table is not None else None, table.stride(0) if table is not None else 0,
         table.shape[1] if table is not None else 0, batch, queries, heads,
         head_dim ** -0.5 if scale is None else scale, window or 0, sinks, workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), stream, status.data_ptr() if status is not None else None))
+        workspace.numel() * workspace.element_size(), stream, words))
     return (out.squeeze(1), lse.squeeze(1)) if squeeze else (out, lse)

@@ -57,3 +57,15 @@ def test_a_bad_slot_is_reported_whole(device, slot, wide):
         call(status)
         with pytest.raises(FerroKittensError, match=f"slot {slot} of token 1 lies outside the cache"):
             gemm.check_status(status)
+
+
+def test_status_words_elsewhere_are_refused_by_every_call(device):
+    cache = kv_cache.new(2, 8, 1, device=device)
+    x = torch.randn(2, 1, 128, device=device).bfloat16()
+    slots, lengths = torch.arange(2, device=device), torch.ones(2, dtype=torch.int32, device=device)
+    for status, error in ((torch.zeros(8, dtype=torch.int32), RuntimeError), (torch.zeros(8, dtype=torch.int64, device=device), ValueError),
+                          (torch.zeros(2, dtype=torch.int32, device=device), ValueError)):
+        for call in (lambda: kv_cache.write(cache, x, x, slots, status), lambda: kv_cache.read(cache, slots, status=status),
+                     lambda: kv_cache.attend(x, cache, lengths, status=status)):
+            with pytest.raises(error, match="status must"):
+                call()

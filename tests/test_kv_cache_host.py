@@ -160,3 +160,15 @@ def test_the_plain_rule():
         codes, scale, low = quantise(x, 64, dtype)
         back = np.repeat(low, 64) + codes * np.repeat(scale, 64)
         assert (np.abs(back - x) <= np.repeat(scale, 64) / 2).all() and codes.max() == 15 and codes.min() == 0
+
+
+def test_status_words_that_a_kernel_cannot_write_are_refused():
+    there, here = torch.device("cuda", 0), torch.device("cpu")
+    assert kv_cache._status_words(None, there) is None
+    with pytest.raises(RuntimeError, match="status must live on the cache's device cuda:0"):
+        kv_cache._status_words(torch.zeros(8, dtype=torch.int32), there)
+    for bad in (torch.zeros(8), torch.zeros(8, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros(8, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="4 words or more"):
+            kv_cache._status_words(bad, here)
+    words = torch.zeros(8, dtype=torch.int32)
+    assert kv_cache._status_words(words[4:], here) == words.data_ptr() + 16
