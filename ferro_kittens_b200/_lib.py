@@ -132,6 +132,7 @@ SIGNATURES = {
     "fk_wait_stream": (c_int, [c_void_p, c_uint32]),
     "fk_wait_event": (c_int, [c_void_p, c_uint32]),
     "fk_launch_budget_ms": (c_uint32, []),
+    "fk_selftest_grants": (c_uint32, [c_uint32]),
     "fk_selftest_deadline": (c_int, [c_uint32, c_uint32]),
     "fk_selftest_call_guard": (c_int, [c_int, c_uint32, POINTER(c_uint64), POINTER(c_uint64)]),
     "fk_status_check": (c_int, [c_void_p, c_void_p]),

@@ -270,6 +270,71 @@ int device_facts(DeviceFacts* out) {
 
 }  // namespace fk
 
+namespace {
+
+/// What has been granted to (kernel, device) pairs: open addressing, twice as many places as pairs at least. A pair that no
+/// memory can be had for is not remembered, and asked for again.
+class Grants {
+public:
+    /// The bytes granted, 0 of a pair that is not remembered.
+    uint32_t of(const void* kernel, int device) const {
+        return capacity_ ? places_[place(kernel, device)].bytes : 0;
+    }
+    void remember(const void* kernel, int device, uint32_t bytes) {
+        if (2 * (count_ + 1) > capacity_ && !grow()) return;
+        Grant& grant = places_[place(kernel, device)];
+        if (!grant.kernel) {
+            ++count_;
+            grant = Grant{kernel, device, bytes};
+        } else if (bytes > grant.bytes) {
+            grant.bytes = bytes;
+        }
+    }
+    void release() { free(places_); }
+
+private:
+    struct Grant {
+        const void* kernel;
+        int device;
+        uint32_t bytes;
+    };
+    /// Where the pair lies, or the free place it would take.
+    uint32_t place(const void* kernel, int device) const {
+        uint64_t hash = (reinterpret_cast<uintptr_t>(kernel) + static_cast<uint64_t>(device)) * 0x9e3779b97f4a7c15ull;
+        uint32_t at = static_cast<uint32_t>(hash >> 32) & (capacity_ - 1);
+        while (places_[at].kernel && (places_[at].kernel != kernel || places_[at].device != device)) at = (at + 1) & (capacity_ - 1);
+        return at;
+    }
+    bool grow() {
+        const Grants old = *this;
+        const uint32_t capacity = capacity_ ? 2 * capacity_ : 128;
+        Grant* const places = static_cast<Grant*>(calloc(capacity, sizeof(Grant)));
+        if (!places) return false;
+        places_ = places;
+        capacity_ = capacity;
+        for (uint32_t i = 0; i < old.capacity_; ++i)
+            if (old.places_[i].kernel) places_[place(old.places_[i].kernel, old.places_[i].device)] = old.places_[i];
+        free(old.places_);
+        return true;
+    }
+    Grant* places_ = nullptr;
+    uint32_t capacity_ = 0, count_ = 0;
+};
+
+}  // namespace
+
+extern "C" uint32_t fk_selftest_grants(uint32_t pairs) {
+    Grants grants;
+    const auto kernel = [](uint32_t i) { return reinterpret_cast<const void*>(static_cast<uintptr_t>(0x1000 + 16 * (i / 8))); };
+    for (uint32_t i = 0; i < pairs; ++i) grants.remember(kernel(i), static_cast<int>(i % 8), 1 + i);
+    for (uint32_t i = 0; i < pairs; i += 3) grants.remember(kernel(i), static_cast<int>(i % 8), 7);  // never lowers
+    uint32_t remembered = 0;
+    for (uint32_t i = 0; i < pairs; ++i) remembered += grants.of(kernel(i), static_cast<int>(i % 8)) == (i % 3 || 1 + i > 7 ? 1 + i : 7);
+    remembered -= grants.of(kernel(pairs + 8), 0) != 0;  // one that was not put in
+    grants.release();
+    return remembered;
+}
+
 // The admission is monotonic, so what has been granted to a (device, kernel) pair is remembered and a
 // repeated request within it costs a table look-up instead of two runtime queries.
 extern "C" int fk_admit_shared_plan(const void* kernel, uint32_t bytes, uint32_t* limit_out) {
@@ -283,19 +348,11 @@ extern "C" int fk_admit_shared_plan(const void* kernel, uint32_t bytes, uint32_t
         return fk_fail(FK_ERR_TOO_LARGE,
                        "shared plan of %u B is past this device's %d B opt-in limit per block", bytes,
                        limit);
-    struct Granted {
-        const void* kernel;
-        int device;
-        uint32_t bytes;
-    };
     static std::mutex guard;
-    static Granted granted[64];
-    static uint32_t count = 0;
+    static Grants granted;
     {
         std::lock_guard<std::mutex> lock(guard);
-        for (uint32_t i = 0; i < count; ++i)
-            if (granted[i].kernel == kernel && granted[i].device == facts.device && bytes <= granted[i].bytes)
-                return FK_OK;
+        if (bytes && bytes <= granted.of(kernel, facts.device)) return FK_OK;
     }
     cudaFuncAttributes attributes;
     FK_CUDA(cudaFuncGetAttributes(&attributes, kernel));
@@ -305,12 +362,7 @@ extern "C" int fk_admit_shared_plan(const void* kernel, uint32_t bytes, uint32_t
         now = bytes;
     }
     std::lock_guard<std::mutex> lock(guard);
-    for (uint32_t i = 0; i < count; ++i)
-        if (granted[i].kernel == kernel && granted[i].device == facts.device) {
-            if (now > granted[i].bytes) granted[i].bytes = now;
-            return FK_OK;
-        }
-    if (count < 64) granted[count++] = Granted{kernel, facts.device, now};
+    granted.remember(kernel, facts.device, now);
     return FK_OK;
 }
 

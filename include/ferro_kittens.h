@@ -446,8 +446,11 @@ uint32_t fk_launch_budget_ms(void);
  * (0xffffffff: for ever) and then "done": FK_OK, or FK_ERR_TIMEOUT after `budget_ms`.
  * fk_selftest_call_guard takes the per-device lock of the host-buffer entry points, holds it
  * for `hold_ms` and reports when it got and gave up the lock (steady-clock nanoseconds): two
- * threads calling it for one device must not overlap. */
+ * threads calling it for one device must not overlap. fk_selftest_grants puts `pairs` made-up (kernel,
+ * device) pairs into a table like the one fk_admit_shared_plan remembers its grants in, and returns how
+ * many it finds again: all of them. */
 int fk_selftest_deadline(uint32_t budget_ms, uint32_t ready_after_polls);
+uint32_t fk_selftest_grants(uint32_t pairs);
 int fk_selftest_call_guard(int device, uint32_t hold_ms, uint64_t* entered_ns, uint64_t* left_ns);
 
 /* Read a kernel's 4 status words back (waiting on `stream` under the launch
