@@ -114,6 +114,12 @@ def _require_indices(name: str, tensor: torch.Tensor, cache: Cache, count: int |
                          + (f" of {count} entries" if count is not None else ""))
 
 
+def _require_counts(**counts: int) -> None:
+    for name, count in counts.items():  # the entries take 32 bits, and would be given the rest of a longer number
+        if count >= 1 << 32:
+            raise ValueError(f"{count} {name} are more than a call counts")
+
+
 def _status_words(status: torch.Tensor | None, device: torch.device) -> int | None:
     """The address of a call's status words, which the kernels write where they find them."""
     if status is None:
@@ -131,6 +137,7 @@ def _rows(entry, cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
         _require(name, tensor, cache, 3)
         if tensor.shape[1] != cache.kv_heads or tensor.shape[0] != tokens:
             raise ValueError(f"{name} must hold {tokens} tokens of {cache.kv_heads} heads, one token a slot")
+    _require_counts(tokens=tokens)
     k_strides, v_strides, words = k.stride(), v.stride(), _status_words(status, cache.device)
     _on(cache.device, lambda stream: entry(
         cache.view, k.data_ptr(), v.data_ptr(), k_strides[0], k_strides[1], v_strides[0], v_strides[1], slots.data_ptr(),
@@ -190,6 +197,7 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
         if (table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.shape[1] == 0
                 or (table.shape[1] > 1 and table.stride(1) != 1)):
             raise ValueError("table must be an int32 [batch, pages] tensor of contiguous rows of one page or more")
+    _require_counts(sequences=batch, queries=queries, heads=heads, pages=table.shape[1] if table is not None else 0)
     if window is not None and not 1 <= window < 1 << 31:
         raise ValueError("a window is at least one token")
     if not 0 <= sinks < 1 << 31:

@@ -1,6 +1,7 @@
 """What the 4-bit cache's entries refuse before they reach a device, and the plain definition the GPU tests compare with."""
 import ctypes
 import re
+import types
 
 import numpy as np
 import pytest
@@ -172,3 +173,25 @@ def test_status_words_that_a_kernel_cannot_write_are_refused():
             kv_cache._status_words(bad, here)
     words = torch.zeros(8, dtype=torch.int32)
     assert kv_cache._status_words(words[4:], here) == words.data_ptr() + 16
+
+
+def _sizes_alone():
+    """What the checks look at of a cache, on the device whose tensors have sizes and no content."""
+    return types.SimpleNamespace(device=torch.device("meta"), dtype=torch.bfloat16, kv_heads=2, head_dim=128, view=None)
+
+
+def test_counts_past_32_bits_are_refused():
+    """They would reach the entries as what is left of them: 2^32 + 3 tokens as 3."""
+    cache, many = _sizes_alone(), (1 << 32) + 3
+    rows = torch.empty(1, 2, 128, dtype=torch.bfloat16, device="meta").expand(many, 2, 128)
+    slots = torch.empty(many, dtype=torch.int32, device="meta")
+    for call in (lambda: kv_cache.write(cache, rows, rows, slots), lambda: kv_cache.read(cache, slots, rows, rows)):
+        with pytest.raises(ValueError, match="4294967299 tokens are more than a call counts"):
+            call()
+    def attend(batch=1, queries=1, heads=4, pages=2):
+        q = torch.empty(1, 1, 1, 128, dtype=torch.bfloat16, device="meta").expand(batch, queries, heads, 128)
+        kv_cache.attend(q, cache, torch.empty(batch, dtype=torch.int32, device="meta"),
+                        torch.empty(batch, pages, dtype=torch.int32, device="meta"))
+    for name, count in (("batch", many), ("queries", many), ("heads", many + 1), ("pages", many)):
+        with pytest.raises(ValueError, match="more than a call counts"):
+            attend(**{name: count})
