@@ -24,7 +24,8 @@ enum NoteCode : uint32_t {
     kBadLength = 0x503,  // a length past the page table
 };
 
-/// Everything before this launch on its stream is done and seen (see `launch`).
+/// Everything before this launch on its stream is done and seen (see `launch`). Since the kernel has begun by then, nothing it reads counts
+/// as constant for its lifetime: no load here is a non-coherent one.
 __device__ __forceinline__ void wait_for_earlier_launches() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 /// The first bad index of a launch goes into the caller's status words: code, its upper half, where it stands, its lower half.
 __device__ __forceinline__ void note(uint32_t* status, uint32_t code, uint32_t where, uint64_t value) {
@@ -381,8 +382,8 @@ __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant
         if (!kept[r]) row = 0;
 #pragma unroll
         for (uint32_t which = 0; which < 2; ++which) {
-            word[r][which] = __ldg(args.codes[which] + row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block)));
-            pair[r][which] = __ldg(args.params[which] + row * (D / G) + block / (G / 8));
+            word[r][which] = args.codes[which][row * (D / 8) + (which == 0 ? key_word<D>(block) : value_word<D>(block))];
+            pair[r][which] = args.params[which][row * (D / G) + block / (G / 8)];
             if (!kept[r]) word[r][which] = pair[r][which] = 0;  // reads as zeros
         }
     }
@@ -750,9 +751,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
     };
 
     const auto page_at = [&](int32_t place) {
-        return args.table ? static_cast<uint32_t>(
-                                __ldg(args.table + b * args.table_stride + args.page.quotient(extent.token(place))))
-                          : b;
+        return args.table ? static_cast<uint32_t>(args.table[b * args.table_stride + args.page.quotient(extent.token(place))]) : b;
     };
     const auto next_stage = [&]() {
         stage = stage == kStages - 1 ? 0 : stage + 1;
@@ -795,7 +794,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             return false;
         };
         const auto page_of = [&](const Run& run) {
-            return args.table ? static_cast<uint32_t>(__ldg(args.table + b * args.table_stride + run.entry)) : b;
+            return args.table ? static_cast<uint32_t>(args.table[b * args.table_stride + run.entry]) : b;
         };
         for (bool more = find_piece(); more; more = next_piece()) {
             Run run;
@@ -879,7 +878,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         float most = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < kKeyWords; ++w) {
-            raw[w] = r < args.rows ? __ldg(reinterpret_cast<const uint4*>(q) + 4 * w + c4) : make_uint4(0, 0, 0, 0);
+            raw[w] = r < args.rows ? reinterpret_cast<const uint4*>(q)[4 * w + c4] : make_uint4(0, 0, 0, 0);
             const uint32_t words[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(fabsf(E::low(words[i])), fabsf(E::high(words[i]))));

@@ -69,3 +69,45 @@ def test_status_words_elsewhere_are_refused_by_every_call(device):
                      lambda: kv_cache.attend(x, cache, lengths, status=status)):
             with pytest.raises(error, match="status must"):
                 call()
+
+
+@pytest.mark.parametrize("ratio", [4, 12])
+def test_calls_in_a_row_see_what_those_before_them_wrote(device, ratio):
+    """Tables, lengths, slots, queries and rows that change in place between calls which follow each other without a pause, against the
+    same calls with a pause after each."""
+    batch, kv_heads, page_size, per, steps = 6, 2, 16, 12, 60
+    g = torch.Generator(device=device)
+    g.manual_seed(3)
+    def draw(*shape):
+        return torch.randn(*shape, device=device, generator=g).bfloat16()
+    orders = [torch.randperm(batch * per, device=device, generator=g).to(torch.int32).view(batch, per) for _ in range(steps)]
+    counts = [torch.randint(1, per * page_size, (batch,), device=device, generator=g, dtype=torch.int32) for _ in range(steps)]
+    places = [torch.randperm(batch * per * page_size, device=device, generator=g)[:50] for _ in range(steps)]
+    keys, values, asked = ([draw(*shape) for _ in range(steps)] for shape in ((50, kv_heads, 128), (50, kv_heads, 128),
+                                                                              (batch, 1, kv_heads * ratio, 128)))
+    rows = draw(batch * per * page_size, kv_heads, 128)
+
+    def run(pause):
+        cache, workspace = kv_cache.new(batch * per, page_size, kv_heads, device=device), kv_cache.workspace(device)
+        kv_cache.write(cache, rows, rows, torch.arange(batch * per * page_size, device=device))
+        table, lengths, slots, k, v, q = (torch.empty_like(x[0]) for x in (orders, counts, places, keys, values, asked))
+        seen = []
+        torch.cuda.synchronize()
+        for i in range(steps):
+            for ours, theirs in ((table, orders), (lengths, counts), (slots, places), (k, keys), (v, values), (q, asked)):
+                ours.copy_(theirs[i])
+            pause()
+            kv_cache.write(cache, k, v, slots)
+            pause()
+            seen += kv_cache.attend(q, cache, lengths, table, workspace=workspace)
+            pause()
+            seen += kv_cache.read(cache, slots)
+            pause()
+            q.mul_(0.5)
+            seen += kv_cache.attend(q, cache, lengths, table, window=20, sinks=3, workspace=workspace)
+            pause()
+        torch.cuda.synchronize()
+        return seen
+
+    for x, y in zip(run(lambda: None), run(torch.cuda.synchronize)):
+        assert torch.equal(x, y)
