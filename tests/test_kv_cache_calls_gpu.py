@@ -1,9 +1,12 @@
 """The 4-bit cache's calls: outputs beside one another in memory, what a bad index is reported as, and every variant of the attention
 that the device's size and the number of segments choose."""
+import numpy as np
 import pytest
 import torch
 
 from ferro_kittens_b200 import FerroKittensError, gemm, kv_cache
+
+from test_kv_cache_gpu import _compare, _random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +114,45 @@ def test_calls_in_a_row_see_what_those_before_them_wrote(device, ratio):
 
     for x, y in zip(run(lambda: None), run(torch.cuda.synchronize)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("head_dim,group", [(128, 128), (128, 64), (128, 32), (64, 64), (64, 32)])
+@pytest.mark.parametrize("ratio", [3, 12])
+@pytest.mark.parametrize("plan", ["one block", "one block for long tables", "two blocks", "three blocks"])
+def test_every_plan_of_the_attention(device, head_dim, group, dtype, ratio, plan):
+    """Segments (a sequence's kv head) up to the number of SMs, up to twice it with tables of more and of less than 8192 tokens, and
+    beyond: blocks alone on an SM, two and three of them, for 8 rows and for 16."""
+    sms = torch.cuda.get_device_properties(device).multi_processor_count
+    kv_heads = 2 if ratio == 3 else 1
+    segments = {"one block": sms - 3, "one block for long tables": 2 * sms - 2, "two blocks": sms + 2, "three blocks": 2 * sms + 9}[plan]
+    batch = -(-segments // kv_heads)
+    seed = 2 * head_dim + group + ratio + len(plan)
+    rng = np.random.default_rng(seed)
+    for page_size, window, sinks in ((16, None, 0), (48, 100, 5), (7, None, 0), (10, 37, 20)):
+        per = -(-(9000 if plan == "one block for long tables" else 400) // page_size)
+        pool = 6 * 48 // page_size
+        cache = _random_cache(device, pool, page_size, kv_heads, head_dim, group, dtype, seed)
+        lengths = torch.from_numpy(np.exp(rng.uniform(0, np.log(400), batch)).astype(np.int32))
+        lengths[rng.integers(batch)], lengths[-1] = 0, 399
+        table = torch.full((batch, per), -1, dtype=torch.int32)
+        used = -(-400 // page_size)
+        table[:, :used] = torch.from_numpy(rng.integers(0, pool, (batch, used)).astype(np.int32))
+        q = torch.randn(batch, 1, kv_heads * ratio, head_dim, device=device).to(dtype)
+        ours, workspace = table.to(device), kv_cache.workspace(device)
+        status = gemm.new_status(device)
+        out, lse = kv_cache.attend(q, cache, lengths.to(device), ours, window=window, sinks=sinks, workspace=workspace, status=status)
+        gemm.check_status(status)
+        some = sorted({0, batch - 1, int(lengths.argmin()), *rng.integers(0, batch, 5).tolist()})
+        _compare(cache, q[some], lengths[some], table[some], None, window, sinks, out[some], lse[some])
+        # A page outside the cache, of the newest tokens of one sequence: noted, and nothing to the others.
+        bad = int(rng.integers(batch))
+        bad = bad if int(lengths[bad]) else batch - 1
+        ours[bad, (int(lengths[bad]) - 1) // page_size] = pool
+        status = gemm.new_status(device)
+        again, lse_again = kv_cache.attend(q, cache, lengths.to(device), ours, window=window, sinks=sinks, workspace=workspace, status=status)
+        with pytest.raises(FerroKittensError, match=f"page {pool} in the table of sequence {bad} lies"):
+            gemm.check_status(status)
+        others = torch.arange(batch) != bad
+        assert torch.equal(again[others], out[others]) and torch.equal(lse_again[others], lse[others])
+        assert torch.isfinite(again).all()
