@@ -1671,6 +1671,19 @@ static int move_rows(bool write, const fk_cache_t* cache, const void* k, const v
                 return fk_fail(FK_ERR_SHAPE, "strides of %lld elements a token and %lld a head lay rows of %u over one another",
                                static_cast<long long>(rows.token_stride), static_cast<long long>(rows.head_stride), cache->head_dim);
         if (both[0].over(both[1])) return fk_fail(FK_ERR_INVALID, "keys and values read would lie over one another");
+    } else {
+        const uint64_t rows = static_cast<uint64_t>(cache->pages) * cache->page_size * cache->kv_heads;
+        const uint64_t codes = rows * (cache->head_dim / 2), params = rows * (cache->head_dim / cache->group) * 4;
+        const struct {
+            const void* at;
+            uint64_t bytes;
+        } buffers[4] = {{cache->k_codes, codes}, {cache->v_codes, codes}, {cache->k_params, params}, {cache->v_params, params}};
+        for (uint32_t i = 0; i < 4; ++i)
+            for (uint32_t j = 0; j < i; ++j) {
+                const uintptr_t x = reinterpret_cast<uintptr_t>(buffers[i].at), y = reinterpret_cast<uintptr_t>(buffers[j].at);
+                if (x < y + buffers[j].bytes && y < x + buffers[i].bytes)
+                    return fk_fail(FK_ERR_INVALID, "the cache's buffers lie over one another");
+            }
     }
     DeviceFacts facts;
     const int known = device_facts(&facts);

@@ -364,7 +364,7 @@ int fk_groupnorm_tile(const void* source, void* destination, uint32_t rows, floa
  *   values  a matrix [8][head_dim / 8] of nibbles; nibble [l][n] is channel 8 n + l
  *
  * head_dim is 64 or 128, group 32, 64 or 128 and at most head_dim, element FK_BF16 or FK_F16 (of the
- * parameters and of the tensors that are written, read or asked with). Buffers are 16-byte aligned.
+ * parameters and of the tensors that are written, read or asked with). Buffers are 16-byte aligned, and apart (a write says so).
  * Pages of 4 tokens or a multiple keep every row's parameters on 16 bytes for the attention's copies; others work, slower.
  * A slot is page * page_size + place. Indices live on the device, so a bad one is found there: it is
  * skipped (nothing is read or written out of bounds) and noted in `device_status`, which may be null

@@ -195,3 +195,17 @@ def test_counts_past_32_bits_are_refused():
     for name, count in (("batch", many), ("queries", many), ("heads", many + 1), ("pages", many)):
         with pytest.raises(ValueError, match="more than a call counts"):
             attend(**{name: count})
+
+
+@pytest.mark.parametrize("places", [(0, 2, 1, 3), (0, 1, 0, 3), (0, 1, 2, 1), (0, 0, 2, 3), (0, 1, 2, 2)])
+@pytest.mark.parametrize("shift", [0, -16, 16])
+def test_writes_to_buffers_over_one_another_are_refused(places, shift):
+    """Codes of 4 x 16 x 2 rows of 64 bytes and parameters of 8: buffers 8192 bytes apart, but for two."""
+    names = ("k_codes", "k_params", "v_codes", "v_params")
+    at = {name: BASE + (1 << 20) + 8192 * place for name, place in zip(names, places)}
+    if places == (0, 2, 1, 3):  # all apart: moved into a neighbour
+        at["v_codes"] -= 16 + abs(shift)
+    else:
+        at[names[max(i for i in range(4) if places.count(places[i]) > 1)]] += shift
+    assert _write(_cache(**at)) == FK_ERR_INVALID
+    assert "buffers lie over one another" in last_error()
