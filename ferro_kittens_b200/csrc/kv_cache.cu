@@ -1048,11 +1048,14 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
             {
                 uint32_t pairs[kGroups];  // lane = token
                 load_words(pairs, value_params + lane * (kGroups * 4));
+                float least = INFINITY, most = 0.0f;
 #pragma unroll
                 for (uint32_t g = 0; g < kGroups; ++g) {
-                    const float fitted = fabsf(E::low(pairs[g])) * fit[g];
-                    grows |= !(fitted >= kLeast && fitted < kMost);
+                    const float fitted = E::low(pairs[g]) * fit[g];
+                    least = fminf(least, fabsf(fitted));
+                    most = fmaxf(most, fabsf(fitted));
                 }
+                grows = least < kLeast || most >= kMost;
             }
 
             // ---- scores, transposed. A code in the low nibble of a half word IS the fp16 number code * 2^-24 (a
