@@ -316,8 +316,8 @@ __device__ __forceinline__ uint32_t group_codes(const uint4 x, uint32_t params, 
 // One lane holds 8 channels (16 bytes) of a row's key and of its value, D / 8 lanes a row, ROWS rows of its own at a time: slots,
 // then rows, of all of them are on their way before the first is worked on. The group's ends meet by shuffles of packed pairs;
 // everything behind them is on packed fp32 pairs, without a division, and exact (see above). What bounds it is the issue of
-// instructions (0.81 a cycle and scheduler, 175 a warp for 8 channels of its lanes): 150001 tokens of 8 heads of 64 fp16 values take 114 us, 54 %
-// of the copy rate; 8191 tokens of 8 heads of 128 bf16 values 17 us.
+// instructions (0.81 a cycle and scheduler, 175 a warp for 8 channels of its lanes): 150001 tokens of 8 heads of 64 fp16 values take 116 us, 53 %
+// of the copy rate; 8191 tokens of 8 heads of 128 bf16 values 16 us.
 template <int D, int G, int ROWS, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constant__ RowArguments args,
                                                             uint32_t* status) {
@@ -361,8 +361,9 @@ __global__ void __launch_bounds__(kRowThreads) write_kernel(const __grid_constan
 
 // The same lanes the other way: a code in the low mantissa bits of a power of two, less that power, is exact,
 // and one fused multiply-add in the cache's type rounds low + code * scale once. 65536 tokens of 8 heads of 128 bf16 values take
-// 64 us, 82 % of the copy rate (four fifths of the bytes are writes). Two rows a thread and blocks of 128 threads: 71 us with
-// 256 threads, 75 with one row, 74 and 87 with four and eight (registers that hold rows in flight cost threads).
+// 59 us, 90 % of the copy rate (four fifths of the bytes are writes). Two rows a thread and blocks of 128 threads: with non-coherent
+// loads 64 us, against 71 with 256 threads, 75 with one row, 74 and 87 with four and eight (registers that hold rows in flight cost
+// threads).
 template <int D, int G, int ROWS, bool BF16>
 __global__ void __launch_bounds__(kRowThreads) read_kernel(const __grid_constant__ RowArguments args,
                                                            uint32_t* status) {
@@ -626,12 +627,12 @@ __device__ __forceinline__ void finish_row(const AttentionArguments& args, const
 // comes last adds them up in the order of the line: the same bits every time.
 //
 // What bounds it: for an SM's part of the copy rate (23 bytes a cycle) the 16 tokens of a warp's step, 2304 bytes of a 128-wide
-// head in groups of 64, may take 98 cycles. All told a step is 349 warp instructions, 87 cycles of the four schedulers; 147 of
-// them are masks, shifts and permutes on the ALU, which takes one every other cycle: 74 cycles; 16 are matrix products of 8 cycles: 33.
-// Four warps a scheduler, all of them on dependent chains (masks, products, exponentials, products), issue in 62 % of the cycles
-// and keep the ALU busy for 52 %: the kernel is bound by latency and issue, not by memory (50 % of its peak under the profiler). Of
+// head in groups of 64, may take 98 cycles. All told a step is 363 warp instructions, 91 cycles of the four schedulers; 157 of
+// them are masks, shifts and permutes on the ALU, which takes one every other cycle: 78 cycles; 16 are matrix products of 8 cycles: 33.
+// Four warps a scheduler, all of them on dependent chains (masks, products, exponentials, products), issue in 63 % of the cycles
+// and keep the ALU busy for 54 %: the kernel is bound by latency and issue, not by memory (49 % of its peak under the profiler). Of
 // 128-wide heads in groups of 64, one query a sequence: 32 ragged sequences of up to 30000 tokens, 8 kv heads with 8 query heads
-// each, 134 us (65 % of the copy rate); one of 131072 tokens 46 us (50 %); 48 of up to 4096 tokens 44 us (42 %); one
+// each, 137 us (64 % of the copy rate); one of 131072 tokens 45 us (51 %); 48 of up to 4096 tokens 46 us (39 %); one
 // of 777 with 4 query heads each 14 us, all of it beginnings and ends: lengths, queries, first copies, merging.
 // Tried and slower or no faster: parameters widened to floats in shared memory (its wavefronts are then 80 % of what it can do),
 // every warp sending its own copies (a bulk copy takes its warp some 150 cycles), small runs copied 16 bytes a lane, 2 or 4
@@ -1013,7 +1014,7 @@ __global__ void __launch_bounds__(AttentionShape<D, G, NT>::kMostThreads, 1)
         }
 
         // Pairs are a fragment's two rows. Scores are the products' sums; times to_log2 they are powers of two. minus_peak is the
-        // row's reference in powers of two, negative, and ceiling the score 2^kSlack above it: 0 and -inf while nothing is seen.
+        // row's reference in powers of two, negated, and ceiling the score 2^kSlack above it: 0 and -inf while nothing is seen.
         float out[kTiles][NT][4] = {};
         float2 lows[kGroups][NT] = {}, ceiling[NT], minus_peak[NT] = {}, sum[NT] = {};
 #pragma unroll
@@ -1755,7 +1756,8 @@ static int launch_attention(cache::AttentionArguments& args, const DeviceFacts& 
     const uint64_t segments = static_cast<uint64_t>(args.batch) * args.kv_heads * args.row_tiles;
     // How many warps share a piece. One block an SM, of all the warps it holds, leaves the fewest parts to put together: for
     // segments fewer than the SMs, or than twice the SMs and long. Smaller blocks overlap one's beginnings and ends with others'
-    // units: two an SM while each can take a whole segment, three beyond. (128-wide heads, 8 rows, groups of 64: 256 segments of
+    // units: two an SM while each can take a whole segment, three beyond. How long segments are the host does not know, since the
+    // lengths live on the device: the table's width stands for it, and a table much wider than its sequences gets the longer ones' plan. (128-wide heads, 8 rows, groups of 64: 256 segments of
     // 15000 tokens, before a lone block's registers were handed over, 135 us against 143 with two blocks; 296 of 2000 27.6 us with two,
     // 34.2 with three, 35.5 with one; 384 of 2000 39.6 with three, 42.0 with two; 1024 of 300 30.3 with three, 35.0 with two, 47.9 with one.)
     const uint64_t sms = static_cast<uint64_t>(facts.sm_count);

@@ -349,7 +349,7 @@ int fk_groupnorm_tile(const void* source, void* destination, uint32_t rows, floa
  * No counterpart in the reference, whose attention (examples/src/flash_forward.rs:151-158) reads whole
  * planes of bf16 keys and values. A serving program keeps those of the tokens seen so far, and the time of
  * one decoding step is the time to read them: at 4 bits a value (4.5 with the parameters of groups of 64) a
- * step moves 3.5 times fewer bytes than from bf16.
+ * step moves 3.6 times fewer bytes than from bf16.
  *
  * The cache is four packed device buffers, one row per (page, kv head, place in the page):
  *   k_codes, v_codes    [pages, kv_heads, page_size, head_dim / 2] bytes, two codes each, low nibble first
@@ -357,15 +357,16 @@ int fk_groupnorm_tile(const void* source, void* destination, uint32_t rows, floa
  * A row's channels are cut into groups of `group`. Of a group, `low` is the smallest value, `scale` the
  * largest value of the cache's type not above (high - low) / 15 (so that nothing read back lies outside
  * [low, high]), and a channel's code 0..15 the number of k in 0..14 with x - low >= (k + 1/2) * scale, in exact
- * arithmetic. It stands for low + code * scale, at most scale / 2 from x (a group whose scale underflows the
- * type reads back as low). A group that holds a NaN or an infinity reads back as NaN throughout.
+ * arithmetic. It stands for low + code * scale, at most scale / 2 from x (or 15 of the type's smallest values, if that is more: a group whose
+ * scale underflows reads back as low). A group that holds a NaN or an infinity reads back as NaN throughout.
  * The order of a row's nibbles is the one the attention's matrix instructions want:
  *   keys    a matrix [4][head_dim / 32] of runs of 8 nibbles; run [c][w] holds channels 8 * (4 w + c) + 0..7
  *   values  a matrix [8][head_dim / 8] of nibbles; nibble [l][n] is channel 8 n + l
  *
  * head_dim is 64 or 128, group 32, 64 or 128 and at most head_dim, element FK_BF16 or FK_F16 (of the
  * parameters and of the tensors that are written, read or asked with). Buffers are 16-byte aligned, and apart (a write says so).
- * Pages of 4 tokens or a multiple keep every row's parameters on 16 bytes for the attention's copies; others work, slower.
+ * Pages of 4 tokens or a multiple keep every page's parameters on 16 bytes for the attention's copies; others work, slower (as does
+ * the end of a sequence in its last page, where its tokens' parameters are no multiple of 16 bytes).
  * A slot is page * page_size + place. Indices live on the device, so a bad one is found there: it is
  * skipped (nothing is read or written out of bounds) and noted in `device_status`, which may be null
  * (fk_status_check then says FK_ERR_INVALID with the index). All calls are asynchronous on `stream`. */
@@ -397,7 +398,9 @@ int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_str
                   int64_t v_token_stride, int64_t v_head_stride, const void* slots, uint32_t slot_bytes,
                   uint32_t tokens, int clear_skipped, void* stream, uint32_t* device_status);
 
-/* Attention of each sequence's newest tokens over its rows of the cache, theirs included.
+/* Attention of each sequence's newest tokens over its rows of the cache, theirs included: for decoding, and for the few tokens of a guess
+ * or a chunk. Each 16 rows (queries times heads / kv_heads) read the sequence once more, so a long prompt's many queries cost
+ * as many passes.
  *   q        [batch, queries, heads, head_dim], strides in elements, multiples of 8; heads is a multiple of
  *            kv_heads, and query head h reads kv head h / (heads / kv_heads)
  *   out      packed [batch, queries, heads, head_dim] of the cache's type; lse null or packed [batch, queries, heads]
@@ -405,7 +408,9 @@ int fk_cache_read(const fk_cache_t* cache, void* k, void* v, int64_t k_token_str
  *   lengths  [batch] int32: tokens of each sequence, its `queries` newest among them; 0 or less is an empty
  *            sequence, and one shorter than `queries` has its first rows before its first token
  *   table    row b (of table_pages entries, table_stride apart) names sequence b's pages in order; entries behind its
- *            length are never read, and those of pages that no row sees may name any; null: sequence b owns page b
+ *            length are never read, and those of pages that no row sees may name any; null: sequence b owns page b. Tables
+ *            of more than 8192 tokens a row are taken for long sequences' where the launch is planned: pass no more
+ *            columns than the longest sequence has
  * Query t of a sequence sits at i = length - queries + t and sees token j when j <= i and (window == 0, or
  * j > i - window, or j < sinks). A row that sees nothing is zero, its lse -inf. Tokens that no row of a sequence
  * sees are not read (but for the few that fill up 16 at the sinks' end and the window's beginning), and what a row does not
