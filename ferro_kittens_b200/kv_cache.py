@@ -156,7 +156,7 @@ def read(cache: Cache, slots: torch.Tensor, k: torch.Tensor | None = None, v: to
          status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(k, v)``, ``[tokens, kv_heads, head_dim]``: what the rows at ``slots`` (int32 or int64, may repeat) stand for, rounded once.
     Rows of negative slots are zero in new tensors and left as they were in ``k`` and ``v`` that are given (which may be
-    strided, as views of the planes ``flash_forward.run`` takes)."""
+    strided, as views of the planes ``flash_forward.run`` takes, but not lie over one another)."""
     _require_indices("slots", slots, cache, wide=True)
     if (k is None) != (v is None):
         raise ValueError("k and v are given together or not at all")
@@ -181,6 +181,10 @@ def attend(q: torch.Tensor, cache: Cache, lengths: torch.Tensor, table: torch.Te
     ``i = length - queries + t`` and sees the tokens ``j <= i``; with a ``window``, those with ``j > i - window`` and the first
     ``sinks``. Returns ``(out, lse)``: ``out`` like ``q``, packed, and ``lse`` fp32 natural-log normalisers ``[batch, (queries,) heads]``;
     a row that sees nothing is zero, its lse -inf.
+
+    ``out`` may not lie over ``q``. Each 16 rows (queries times heads per kv head) read the sequence once more: this is for few
+    new tokens, not for long prompts. ``table`` wants no more columns than the longest sequence has: past 8192 tokens the launch is planned
+    for long ones.
 
     A serving loop passes a ``workspace`` that it keeps (see :func:`workspace`); without one each call makes its own."""
     squeeze = q.dim() == 3

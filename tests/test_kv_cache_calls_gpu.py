@@ -156,3 +156,44 @@ def test_every_plan_of_the_attention(device, head_dim, group, dtype, ratio, plan
         others = torch.arange(batch) != bad
         assert torch.equal(again[others], out[others]) and torch.equal(lse_again[others], lse[others])
         assert torch.isfinite(again).all()
+
+
+def test_a_captured_step_on_two_streams(device):
+    """A step captured as two branches, copies and kernels in turn on each, that meet in an attention over what both wrote: replayed
+    with other contents, against the same calls one by one. (Its kernels' first calls, if no test ran before, fall into the capture.)"""
+    batch, kv_heads, ratio, page_size, per = 4, 2, 6, 16, 20
+    cache, plain = (kv_cache.new(batch * per, page_size, kv_heads, 64, 64, device=device) for _ in range(2))
+    table = torch.randperm(batch * per, device=device).to(torch.int32).view(batch, per)
+    lengths = torch.tensor([300, 1, 77, 320], dtype=torch.int32, device=device)
+    spaces = [kv_cache.workspace(device) for _ in range(2)]
+    half = batch * per * page_size // 2
+    slots = torch.randperm(2 * half, device=device)
+    source, rows = (torch.zeros(2 * half, kv_heads, 64, dtype=torch.bfloat16, device=device) for _ in range(2))
+    asked, q = (torch.zeros(batch, 2, kv_heads * ratio, 64, dtype=torch.bfloat16, device=device) for _ in range(2))
+    side = torch.cuda.Stream(device)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        rows.copy_(source)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            kv_cache.write(cache, rows[half:], rows[half:], slots[half:])
+            q.copy_(asked)
+            early = kv_cache.attend(q, plain, lengths, table, workspace=spaces[1])
+        kv_cache.write(cache, rows[:half], rows[:half], slots[:half])
+        back = kv_cache.read(cache, slots[:half])
+        main.wait_stream(side)
+        late = kv_cache.attend(q, cache, lengths, table, window=100, sinks=4, workspace=spaces[0])
+        late_too = kv_cache.attend(q, cache, lengths, table, workspace=spaces[0])
+    for _ in range(4):
+        source.copy_(torch.randn_like(source))
+        asked.copy_(torch.randn_like(asked))
+        graph.replay()
+        torch.cuda.synchronize()
+        kv_cache.write(plain, source, source, slots)
+        for x, y in zip((*late, *late_too, *back),
+                        (*kv_cache.attend(asked, plain, lengths, table, window=100, sinks=4), *kv_cache.attend(asked, plain, lengths, table),
+                         *kv_cache.read(plain, slots[:half]))):
+            assert torch.equal(x, y)
+        assert torch.isfinite(early[0]).all()

@@ -249,3 +249,21 @@ def test_scores_and_scales_that_drift_along_the_sequence(device, rise, ratio):
     for order in (table, table[:, :28].flip(1).contiguous()):
         out, lse = kv_cache.attend(q.bfloat16(), cache, lengths, order)
         _compare(cache, q.bfloat16(), lengths, order, None, None, 0, out, lse)
+
+
+@pytest.mark.parametrize("length,batch,ratio", [(9000, 1, 4), (9000, 1, 12), (2500, 5, 12), (700, 160, 3), (700, 310, 12)])
+def test_far_scales_in_parts_of_long_sequences(device, length, batch, ratio):
+    """Scales that drift over 2^40 along the sequence, differ by 2^12 between groups and jump by 2^25 at one token in a hundred, put
+    together from the parts of warps and blocks."""
+    page_size, per = 64, -(-length // 64)
+    cache = _ordinary(device, torch.bfloat16, 128, 64, 29, page_size, per)
+    drift = torch.linspace(-20, 20, per * page_size, device=device).view(per, 1, page_size, 1, 1)
+    jump = 25.0 * (torch.rand(per, 1, page_size, 1, 1, device=device) < 0.01)
+    between = torch.tensor([0.0, 12.0], device=device).view(1, 1, 1, 2, 1)
+    cache.v_params.copy_((cache.v_params.float() * torch.exp2(drift + jump + between)).bfloat16())
+    table = torch.arange(per, dtype=torch.int32, device=device).view(1, per).repeat(batch, 1)
+    lengths = torch.tensor([length - (i * 331) % length for i in range(batch)], dtype=torch.int32, device=device)
+    q = torch.randn(batch, 1, ratio, 128, device=device).bfloat16()
+    out, lse = kv_cache.attend(q, cache, lengths, table)
+    some = sorted({0, batch // 2, batch - 1})
+    _compare(cache, q[some], lengths[some], table[some], None, None, 0, out[some], lse[some])
